@@ -1,0 +1,110 @@
+/*
+ * linalg_b200.h — C ABI of the orthogonalised optimiser update and the grouped matrix products
+ * of the B200 (sm_100a) library. The conventions are chol_b200.h's: plain pointers, sizes and an
+ * opaque queue handle (a cudaStream_t as void*, NULL = the legacy default queue) in, an integer
+ * status out (CHOL_OK, CHOL_ERR_*; text from chol_strerror). All work is enqueued
+ * asynchronously; nothing is allocated; no C++ exception crosses this boundary. Every call takes
+ * its scratch from the caller, so calls on different queues do not interfere, and every call can
+ * be captured into a CUDA graph (chol_prepare and linalg_prepare once before the capture).
+ * The reference project has no counterpart to these entry points.
+ */
+#ifndef LINALG_B200_H
+#define LINALG_B200_H
+
+#include "chol_b200.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types. */
+#define LINALG_BF16 0
+#define LINALG_FP16 1
+#define LINALG_FP32 2
+
+/* Working precision of the Newton-Schulz iteration. */
+#define LINALG_PRECISION_AUTO 0 /* HALF for bf16 results, FULL for fp16 and fp32 results */
+#define LINALG_PRECISION_HALF 1 /* fp16 operands, FP32 accumulation: ~1e-3 of the result's norm */
+#define LINALG_PRECISION_FULL 2 /* operands split into two fp16 numbers (22 bits), three products
+                                   per product: ~4e-6 of the result's norm */
+
+#define LINALG_MAX_STEPS 32   /* Newton-Schulz steps of one call */
+#define LINALG_MAX_GROUPS 1024 /* groups of one grouped product */
+
+/* Per-device set-up (idempotent, thread-safe; every entry point calls it for the current
+   device). CHOL_ERR_DEVICE unless the device is sm_100. */
+CHOL_API int linalg_prepare(int device);
+
+/*
+ * A batch of row-major matrices: element (i, r, c) at data + i * stride + r * ld + c.
+ * ld >= cols; any alignment of the element type.
+ */
+typedef struct {
+  void* data;
+  int64_t ld, stride;
+  int type; /* LINALG_* */
+} linalg_matrix;
+
+/* Bytes of device workspace (256-byte aligned) of linalg_orthogonalize and linalg_muon_update
+   for `batch` m x n matrices at a working precision (HALF or FULL; AUTO counts as FULL). */
+CHOL_API size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n,
+                                               int precision);
+
+/*
+ * Newton-Schulz approximation of the polar factor of each matrix of a batch:
+ *   X = x / (||x||_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T
+ * (from the right with A = X^T X when m > n), and out = X. coefficients: 3 * steps host floats
+ * (a, b, c of each step). x and out may be the same array; partial overlap is not allowed.
+ * A matrix with a NaN or an infinity yields NaN; the other matrices of the batch are not
+ * affected. A zero matrix yields zeros.
+ */
+CHOL_API int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64_t batch,
+                                  int64_t m, int64_t n, int steps, const float* coefficients,
+                                  float eps, int precision, void* workspace,
+                                  size_t workspace_bytes, void* queue);
+
+/*
+ * One optimiser step on a batch of weights, in place:
+ *   momentum <- beta * momentum + (1 - beta) * grad
+ *   u        =  nesterov ? beta * momentum + (1 - beta) * grad : momentum
+ *   param    <- decay * param - rate * orthogonalize(u)
+ * The three arrays must not overlap. precision AUTO goes by param's type.
+ */
+CHOL_API int linalg_muon_update(const linalg_matrix* param, const linalg_matrix* grad,
+                                const linalg_matrix* momentum, int64_t batch, int64_t m,
+                                int64_t n, double beta, int nesterov, float decay, float rate,
+                                int steps, const float* coefficients, float eps, int precision,
+                                void* workspace, size_t workspace_bytes, void* queue);
+
+/*
+ * Rows grouped by an index, each group times its own matrix:
+ *   y[r] = x[r] W_e   for offsets[e] <= r < offsets[e + 1]
+ * x: rows x k, y: rows x n (one matrix each; .stride unused). w: `groups` matrices; w_rows_k != 0:
+ * k x n row-major, else n x k row-major (W_e transposed in memory). offsets: groups + 1 device
+ * integers (32 bits, or 64 with offsets64), non-decreasing, within [0, rows]; values that are
+ * not are clamped to the largest before them and to that range, so that no row outside the
+ * arrays is touched. Rows of no group (before offsets[0], from offsets[groups] on): set to zero
+ * with fill != 0, else left as they are. x, w, y share one type (bf16 or fp16); sums are FP32.
+ * x and w: base 16-byte aligned, ld and stride multiples of 8 (CHOL_ERR_UNSUPPORTED otherwise);
+ * y: any alignment. groups <= LINALG_MAX_GROUPS; sizes below 2^31.
+ */
+CHOL_API int linalg_grouped_matmul(const linalg_matrix* x, const linalg_matrix* w, int w_rows_k,
+                                   const linalg_matrix* y, const void* offsets, int offsets64,
+                                   int64_t groups, int64_t rows, int64_t k, int64_t n, int fill,
+                                   void* queue);
+
+/*
+ * The matrix of each group's outer products, the weight gradient of linalg_grouped_matmul:
+ *   dw_e = sum over offsets[e] <= r < offsets[e + 1] of a[r]^T b[r]     (k x n, row-major)
+ * a: rows x k, b: rows x n, dw: `groups` matrices; zeros for a group without rows. Rows of no
+ * group are not read. Types, alignment and offsets as above.
+ */
+CHOL_API int linalg_grouped_outer(const linalg_matrix* a, const linalg_matrix* b,
+                                  const linalg_matrix* dw, const void* offsets, int offsets64,
+                                  int64_t groups, int64_t rows, int64_t k, int64_t n, void* queue);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* LINALG_B200_H */

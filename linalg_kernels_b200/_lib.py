@@ -1,4 +1,5 @@
-"""ctypes binding of ``libchol_b200.so`` (the C ABI declared in include/chol_b200.h).
+"""ctypes binding of ``libchol_b200.so`` (the C ABI declared in include/chol_b200.h and
+include/linalg_b200.h).
 
 The library is loaded from the package directory. If it is missing, importing the
 compute entry points raises: there is no CPU or torch fallback on the product path.
@@ -43,6 +44,7 @@ _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); every function include/chol_b200.h declares
 SIGNATURES: dict[str, tuple] = {
@@ -71,6 +73,34 @@ SIGNATURES: dict[str, tuple] = {
     "chol_validate_f32": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
 }
 
+# element types and working precisions, as in include/linalg_b200.h
+LINALG_BF16, LINALG_FP16, LINALG_FP32 = 0, 1, 2
+LINALG_PRECISION_AUTO, LINALG_PRECISION_HALF, LINALG_PRECISION_FULL = 0, 1, 2
+LINALG_MAX_STEPS = 32
+LINALG_MAX_GROUPS = 1024
+
+
+class Matrix(ctypes.Structure):
+    """linalg_matrix: a batch of row-major matrices."""
+
+    _fields_ = [("data", _vp), ("ld", _i64), ("stride", _i64), ("type", _int)]
+
+
+_mp = ctypes.POINTER(Matrix)
+
+# name -> (restype, argtypes); every function include/linalg_b200.h declares
+LINALG_SIGNATURES: dict[str, tuple] = {
+    "linalg_prepare": (_int, [_int]),
+    "linalg_orthogonalize_workspace": (_sz, [_i64, _i64, _i64, _int]),
+    "linalg_orthogonalize": (_int, [_mp, _mp, _i64, _i64, _i64, _int, ctypes.POINTER(_f32), _f32,
+                                    _int, _vp, _sz, _vp]),
+    "linalg_muon_update": (_int, [_mp, _mp, _mp, _i64, _i64, _i64, _f64, _int, _f32, _f32, _int,
+                                  ctypes.POINTER(_f32), _f32, _int, _vp, _sz, _vp]),
+    "linalg_grouped_matmul": (_int, [_mp, _mp, _int, _mp, _vp, _int, _i64, _i64, _i64, _i64, _int,
+                                     _vp]),
+    "linalg_grouped_outer": (_int, [_mp, _mp, _mp, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -95,7 +125,7 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
                 f"{p} is missing: build it with `python -m linalg_kernels_b200.build` "
                 "(this package has no CPU fallback)")
         lib = ctypes.CDLL(str(p))
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **LINALG_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
@@ -128,6 +158,21 @@ def potrf_ws(a: int, l: int, batch: int, n: int, info: int, ws: int, ws_bytes: i
 
             _pyext = _via_ctypes
     return _pyext(a, l, batch, n, info, ws, ws_bytes, queue)
+
+
+_linalg = None
+
+
+def linalg():
+    """The fast-call binding (_cholpy) of the linalg_* entry points, as csrc/chol_pyext.c lists
+    their integer arguments. Built with the library; there is no slower stand-in."""
+    global _linalg
+    if _linalg is None:
+        load()
+        from . import _cholpy  # type: ignore
+
+        _linalg = _cholpy
+    return _linalg
 
 
 def strerror(status: int) -> str:

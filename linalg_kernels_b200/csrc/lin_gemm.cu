@@ -1,0 +1,840 @@
+// lin_gemm.cu — half-precision products on CTA pairs (tcgen05, cta_group::2), the engine of the
+// Newton-Schulz iteration and of the grouped products.
+//
+//   D = alpha * A B + beta * C,   A: M x K, B: K x N, both bf16 or both fp16, sums in FP32
+//
+// Each operand is read in the order it is stored in: "K-major" (the summed index contiguous) or
+// "MN-major" (the output's index contiguous), so X X^T, X^T X, S X, X S, x W, dy W^T and
+// x^T dy all run without a transposed copy.
+//
+// A pair of CTAs computes one 256 x BN tile (BN = 256 or 128): each CTA holds 128 rows of A, BN/2
+// rows of B and 128 x BN of the accumulator. The pair shares B, so a CTA writes and reads 32 KB of
+// shared memory per 64 of K at BN = 256 instead of 48 KB; at 512 cycles of tensor work
+// that is 128 bytes a cycle, what shared memory can give (one CTA alone would need 192).
+//
+//   warp 0       TMA producer: 128-byte-swizzled boxes of A and B into a ring of stages. Both CTAs'
+//                copies report to the full barrier of the pair's first CTA.
+//   warp 1       the first CTA's lane 0 issues tcgen05.mma (M256 x BN x K16); the commits free the
+//                stage in both CTAs.
+//   warp 2       TMEM allocation; with a ragged K: waits for each landed stage of its own CTA, zeroes
+//                the rows of a group's last block that belong to the next group (they may
+//                hold anything, NaN included), and reports to the first CTA.
+//   warps 4..11  epilogue: TMEM -> registers -> a 32 x 32 staging tile -> rows of 16-byte
+//                stores, overlapped with the next tile (two accumulators).
+//
+// The grid is persistent: one pair per two SMs, tiles round-robin. Groups' sizes are read from
+// device memory by every CTA, so the host needs no synchronisation.
+//
+// `split`: FP32 accuracy. An operand is a pair of fp16 planes, x = hi + lo (22 bits), and the
+// product is lo hi + hi lo + hi hi (lo lo, < 2^-22, is dropped). The accumulator rounds toward
+// zero at every MMA, an error that grows with the number of steps, so it is drained every 256 of
+// K into registers (rounded to nearest) with the small terms summed first: 16 full-size steps
+// per drain.
+//
+// Every wait is bounded (2 s of %globaltimer); one that runs out records
+// CHOL_ERR_WAIT_TIMEOUT in the library's status word and ends the launch.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "chol_tc_ptx.cuh"
+#include "lin_common.cuh"
+
+namespace lin {
+
+namespace {
+
+using namespace chol::tcx;
+using chol::fence_proxy_async_smem;
+using chol::smem_u32;
+
+constexpr int kBlockK = 64;     // 16-bit elements of K per stage: one 128-byte swizzle row
+constexpr int kTileM = 256;     // rows of a pair's tile
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
+constexpr int kEpiLd = 36;      // staging row stride in floats: conflict-free 16-byte access
+constexpr int kChunk = 4;       // split: K blocks per drained accumulator
+
+template <int BN>
+struct Cfg {
+  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr int A_BYTES = 128 * kBlockK * 2;
+  static constexpr int B_BYTES = BN / 2 * kBlockK * 2;
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int EPI = kEpiWarps * 32 * kEpiLd * 4;
+  static constexpr int TABLE = 2 * (kMaxGroups + 4) * 4;
+  static constexpr size_t SMEM = size_t(STAGES) * STAGE + EPI + 512 + TABLE + 1024;
+  static constexpr int TMEM_COLS = 2 * BN;
+};
+
+struct Args {
+  int m, n, k, batch;
+  int tiles_m, tiles_n, per_matrix;
+  int symmetric;
+  float alpha, beta;
+  const __half* c;
+  int64_t ldc, c_plane;
+  void* out;
+  int64_t ldo, out_stride;
+  int out_type;
+  int c_vec, out_vec;  // 16-byte access possible
+  float decay, rate;
+  const void* offsets;
+  int offsets64;
+  int total_rows;
+  int fill;
+  uint32_t idesc;
+};
+
+// ------------------------------- device helpers ---------------------------------------
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_leader(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait at cluster scope.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* status) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0;; ++it) {
+    if (try_wait_cluster(bar, parity)) return true;
+    if ((it & 255u) == 255u && global_ns() - t0 > kWaitLimitNs) {
+      atomicExch(status, CHOL_ERR_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+}
+// A copy of a pair: the barrier may be the other CTA's (a shared::cluster address).
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y,
+                                              int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
+// MN-major operand, 128-byte swizzle: boxes of 64 MN elements x 64 K rows (8 KB), the next box
+// 64 MN elements further; groups of 8 K rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc_mn(const void* smem_tile) {
+  const uint32_t addr = smem_u32(smem_tile);
+  uint64_t d = 0;
+  d |= uint64_t((addr >> 4) & 0x3FFF);
+  d |= uint64_t(8192 >> 4) << 16;
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;
+  return d;
+}
+
+struct Tile {
+  int index;      // matrix or group
+  int tm, tn;
+  int row0;       // first row of A (and of the output) of the group; 0 for kBatch
+  int rows;       // rows of the output in this matrix or group
+  int k0, k_len;  // the summed range
+};
+
+// The tiles of a launch, in the order every role walks them.
+template <int MODE>
+struct Walker {
+  const Args& g;
+  const int* start;  // kRagged*: first row of each group (and one past the last)
+  const int* first;  // kRaggedM: first tile of each group
+  int groups;        // kRaggedM: with the rows of no group
+  int cursor;
+  __device__ __forceinline__ Walker(const Args& args, const int* s, const int* f, int n)
+      : g(args), start(s), first(f), groups(n), cursor(0) {}
+  __device__ __forceinline__ int total() const {
+    return MODE == kRaggedM ? first[groups] : g.per_matrix * g.batch;
+  }
+  __device__ __forceinline__ void at(int t, Tile& w) {
+    if (MODE == kRaggedM) {
+      while (t >= first[cursor + 1]) ++cursor;
+      const int e = cursor;
+      w.row0 = e <= g.batch ? start[e] : 0;  // group batch: the rows behind the last group;
+      const int end = e <= g.batch ? (e < g.batch ? start[e + 1] : g.total_rows) : start[0];
+      w.rows = end - w.row0;                 // group batch + 1: those before the first
+      w.index = e;
+      w.k0 = 0;
+      w.k_len = e < g.batch ? g.k : 0;
+      const int tms = (w.rows + kTileM - 1) / kTileM;
+      const int r = t - first[e];
+      w.tn = r / tms;
+      w.tm = r - w.tn * tms;
+      return;
+    }
+    w.index = t / g.per_matrix;
+    const int r = t - w.index * g.per_matrix;
+    w.row0 = 0;
+    w.rows = g.m;
+    w.k0 = 0;
+    w.k_len = g.k;
+    if (MODE == kRaggedK) {
+      w.k0 = start[w.index];
+      w.k_len = start[w.index + 1] - w.k0;
+    }
+    if (g.symmetric) {
+      // row tile tm holds min(ratio * (tm + 1), tiles_n) column tiles; ratio = 256 / BN
+      const int ratio = g.symmetric;
+      int tm = int((sqrtf(8.f * float(r / ratio) + 1.f) - 1.f) * 0.5f);
+      while (ratio * (tm * (tm + 1) / 2) > r) --tm;
+      while (ratio * ((tm + 1) * (tm + 2) / 2) <= r) ++tm;
+      w.tm = tm;
+      w.tn = r - ratio * (tm * (tm + 1) / 2);
+    } else {
+      w.tn = r / g.tiles_m;
+      w.tm = r - w.tn * g.tiles_m;
+    }
+  }
+};
+
+// Eight consecutive results of one row to 16-bit or 32-bit memory, `count` of them valid.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int count, bool vec) {
+  if (vec && count == 8) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      alignas(16) T h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = from_float<T>(v[j]);
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = from_float<T>(v[j]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8], int count, bool vec) {
+  if (vec && count == 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      alignas(16) T h[8];
+      *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_weights(T* p, const float (&v)[8], int count, bool vec,
+                                              float decay, float rate) {
+  float w[8];
+  load8(p, w, count, vec);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = fmaf(-rate, v[j], decay * w[j]);
+  store8(p, w, count, vec);
+}
+
+// Results v of output row r, columns c.. of matrix i.
+template <int EPI, bool SPLIT>
+__device__ __forceinline__ void emit(const Args& g, int i, int64_t r, int c, const float (&v)[8],
+                                     int count) {
+  if (EPI == kPlanes) {
+    constexpr int P = SPLIT ? 2 : 1;
+    __half* o = static_cast<__half*>(g.out) + int64_t(i) * P * g.out_stride + r * g.ldo + c;
+    store8(o, v, count, g.out_vec);
+    if (SPLIT) {
+      float lo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
+      store8(o + g.out_stride, lo, count, g.out_vec);
+    }
+    return;
+  }
+  const int64_t at = int64_t(i) * g.out_stride + r * g.ldo + c;
+  if (EPI == kMuon) {
+    if (g.out_type == LINALG_BF16)
+      write_weights(static_cast<__nv_bfloat16*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
+    else if (g.out_type == LINALG_FP16)
+      write_weights(static_cast<__half*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
+    else
+      write_weights(static_cast<float*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
+    return;
+  }
+  if (g.out_type == LINALG_BF16)
+    store8(static_cast<__nv_bfloat16*>(g.out) + at, v, count, g.out_vec);
+  else if (g.out_type == LINALG_FP16)
+    store8(static_cast<__half*>(g.out) + at, v, count, g.out_vec);
+  else
+    store8(static_cast<float*>(g.out) + at, v, count, g.out_vec);
+}
+
+template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a,
+                   const __grid_constant__ CUtensorMap map_b, const Args g, int* status) {
+  using C = Cfg<BN>;
+  constexpr int S = C::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* epi = reinterpret_cast<float*>(smem + size_t(S) * C::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(S) * C::STAGE + C::EPI);
+  uint64_t* full = bars;             // [S] first CTA: a stage of both CTAs has landed
+  uint64_t* landed = bars + S;       // [S] kRaggedK: this CTA's part of the stage has landed
+  uint64_t* empty = bars + 2 * S;    // [S] the MMAs have read the stage
+  uint64_t* tfull = bars + 3 * S;    // [2] accumulator ready
+  uint64_t* tempty = tfull + 2;      // [2] first CTA: accumulator drained by both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  int* start = reinterpret_cast<int*>(smem + size_t(S) * C::STAGE + C::EPI + 512);
+  int* first = start + kMaxGroups + 4;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], MODE == kRaggedK ? 2 : 1);
+      mbar_init(&landed[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 2 * kEpiWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(uint32_t(C::TMEM_COLS))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  griddep_wait();  // before any read of what earlier kernels wrote
+  if (MODE != kBatch && warp == 0) {
+    // group starts: clamped to [0, total_rows], non-decreasing; kRaggedM: their first tiles
+    int high = 0;
+    for (int e0 = 0; e0 <= g.batch; e0 += 32) {
+      const int e = e0 + lane;
+      int64_t v = 0;
+      if (e <= g.batch)
+        v = g.offsets64 ? static_cast<const int64_t*>(g.offsets)[e]
+                        : int64_t(static_cast<const int32_t*>(g.offsets)[e]);
+      v = v < 0 ? 0 : (v > g.total_rows ? g.total_rows : v);
+      int x = int(v);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d && y > x) x = y;
+      }
+      if (x < high) x = high;
+      if (e <= g.batch) start[e] = x;
+      high = __shfl_sync(0xffffffffu, x, 31);
+    }
+    __syncwarp();
+    if (MODE == kRaggedM) {
+      const int groups = g.batch + (g.fill ? 2 : 0);
+      int base = 0;
+      for (int e0 = 0; e0 < groups; e0 += 32) {
+        const int e = e0 + lane;
+        int rows = 0;
+        if (e < g.batch)
+          rows = start[e + 1] - start[e];
+        else if (e < groups)
+          rows = e == g.batch ? g.total_rows - start[g.batch] : start[0];
+        const int tiles = (rows + kTileM - 1) / kTileM * g.tiles_n;
+        int x = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, d);
+          if (lane >= d) x += y;
+        }
+        if (e < groups) first[e] = base + x - tiles;
+        base += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) first[groups] = base;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  griddep_launch();
+  const uint32_t tmem = *tmem_slot;
+  const int pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+  Walker<MODE> walk(g, start, first, MODE == kRaggedM ? g.batch + (g.fill ? 2 : 0) : 0);
+  const int total = walk.total();
+  Tile w;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t kt = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs) {
+        walk.at(t, w);
+        const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
+        const int a_row = w.row0 + w.tm * kTileM + int(rank) * 128;
+        const int b_row = w.tn * BN + int(rank) * (BN / 2);
+        constexpr int planes = SPLIT ? 2 : 1;
+        const int za = MODE == kBatch ? w.index * planes : 0;
+        const int zb = MODE == kRaggedK ? 0 : w.index * planes;
+        const int steps = SPLIT ? 3 * num_k : num_k;
+        for (int i = 0; i < steps; ++i, ++kt) {
+          int kb = i, pa = 0, pb = 0;
+          if (SPLIT) {  // per chunk: lo hi, hi lo, hi hi
+            const int c0 = i / (3 * kChunk) * kChunk;
+            const int len = num_k - c0 < kChunk ? num_k - c0 : kChunk;
+            const int r = i - 3 * c0;
+            const int combo = r / len;
+            kb = c0 + r - combo * len;
+            pa = combo == 0;
+            pb = combo == 1;
+          }
+          const int s = int(kt % S);
+          if (kt >= uint32_t(S) && !wait_bar(&empty[s], ((kt / S) & 1u) ^ 1u, status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + size_t(s) * C::STAGE;
+          uint8_t* sb = sa + C::A_BYTES;
+          uint32_t bar;
+          if (MODE == kRaggedK) {
+            mbar_expect_tx(&landed[s], C::STAGE);
+            bar = smem_u32(&landed[s]);
+          } else {
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+            bar = leader_addr(&full[s]);
+          }
+          const int kx = w.k0 + kb * kBlockK;
+          if (AMN) {
+            tma_load_pair(sa, &map_a, a_row, kx, za + pa, bar);
+            tma_load_pair(sa + 8192, &map_a, a_row + 64, kx, za + pa, bar);
+          } else {
+            tma_load_pair(sa, &map_a, kx, a_row, za + pa, bar);
+          }
+          if (BMN) {
+            tma_load_pair(sb, &map_b, b_row, kx, zb + pb, bar);
+            if (BN == 256) tma_load_pair(sb + 8192, &map_b, b_row + 64, kx, zb + pb, bar);
+          } else {
+            tma_load_pair(sb, &map_b, kx, b_row, zb + pb, bar);
+          }
+        }
+      }
+      if (!ok && rank == 0) {
+        // copies still in flight write this pair's shared memory: give them time to land
+        for (uint32_t j = kt < uint32_t(S) ? 0 : kt - S; j < kt; ++j)
+          wait_bar(MODE == kRaggedK ? &landed[j % S] : &full[j % S], (j / S) & 1u, status);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (first CTA) ----------------
+    if (rank == 0 && lane == 0) {
+      uint32_t kt = 0, round = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs) {
+        walk.at(t, w);
+        const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
+        if (num_k == 0) continue;
+        const int chunks = SPLIT ? (num_k + kChunk - 1) / kChunk : 1;
+        for (int ch = 0; ch < chunks && ok; ++ch, ++round) {
+          const uint32_t buf = round & 1u;
+          if (round >= 2 && !wait_bar(&tempty[buf], ((round >> 1) & 1u) ^ 1u, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t acc = tmem + buf * uint32_t(BN);
+          const int c0 = SPLIT ? ch * kChunk : 0;
+          const int len = SPLIT ? (num_k - c0 < kChunk ? num_k - c0 : kChunk) : num_k;
+          const int steps = SPLIT ? 3 * len : len;
+          for (int i = 0; i < steps; ++i, ++kt) {
+            const int s = int(kt % S);
+            if (!wait_bar(&full[s], (kt / S) & 1u, status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint8_t* sa = smem + size_t(s) * C::STAGE;
+            const uint8_t* sb = sa + C::A_BYTES;
+            const uint64_t da = AMN ? sw128_desc_mn(sa) : sw128_desc(sa);
+            const uint64_t db = BMN ? sw128_desc_mn(sb) : sw128_desc(sb);
+            const int kb = c0 + (SPLIT ? i % len : i);
+            const int left = w.k_len - kb * kBlockK;  // the last block: only its 16-wide slabs
+            const int slabs = left >= kBlockK ? kBlockK / 16 : (left + 15) / 16;
+#pragma unroll
+            for (int kk = 0; kk < kBlockK / 16; ++kk) {
+              if (kk >= slabs) break;
+              mma_pair(acc, da + uint64_t(kk * (AMN ? 2048 : 32) / 16),
+                       db + uint64_t(kk * (BMN ? 2048 : 32) / 16), g.idesc, (i | kk) ? 1u : 0u);
+            }
+            commit_pair(&empty[s]);
+          }
+          if (ok) commit_pair(&tfull[buf]);
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ---------------- kRaggedK: end of a group's last block ----------------
+    if (MODE == kRaggedK) {
+      uint32_t kt = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs) {
+        walk.at(t, w);
+        const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
+        for (int i = 0; i < num_k; ++i, ++kt) {
+          const int s = int(kt % S);
+          ok = wait_bar(&landed[s], (kt / S) & 1u, status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int left = w.k_len - i * kBlockK;
+          if (left < kBlockK && (left & 15)) {
+            // K rows left .. the end of their 16-wide slab are read by the MMA: zero them
+            const int z0 = left, count = ((left + 15) & ~15) - left;
+            uint8_t* sa = smem + size_t(s) * C::STAGE;
+            constexpr int boxes = C::STAGE / 8192;  // A's two, then B's
+            for (int j = lane; j < boxes * count * 8; j += 32) {
+              const int box = j / (count * 8), r = j - box * count * 8;
+              *reinterpret_cast<uint4*>(sa + box * 8192 + (z0 + (r >> 3)) * 128 + (r & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) arrive_leader(leader_addr(&full[s]));
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue ----------------
+    const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; half of the columns
+    float* tile = epi + (warp - 4) * 32 * kEpiLd;
+    constexpr int kCols = BN / 2, kChunks = kCols / 32;
+    const int r8 = lane >> 2, c8 = (lane & 3) * 8;
+    uint32_t round = 0;
+    for (int t = pair; t < total; t += pairs) {
+      walk.at(t, w);
+      const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
+      const int row_base = w.tm * kTileM + int(rank) * 128 + q * 32;  // within the matrix or group
+      const int col0 = w.tn * BN + half * kCols;
+      const bool mirror = EPI == kPlanes && g.symmetric && w.tm * kTileM > w.tn * BN + BN - 1;
+
+      // one 32 x 32 piece: v = this lane's row of accumulators
+      auto piece = [&](const float (&v)[32], int cc) {
+        const int gc0 = col0 + cc * 32;
+        if (gc0 >= g.n || row_base >= w.rows) return;
+        float* trow = tile + lane * kEpiLd;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(trow + 4 * j) =
+              make_float4(g.alpha * v[4 * j], g.alpha * v[4 * j + 1], g.alpha * v[4 * j + 2],
+                          g.alpha * v[4 * j + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tr = i * 8 + r8, row = row_base + tr, col = gc0 + c8;
+          if (row < w.rows && col < g.n) {
+            const int count = g.n - col < 8 ? g.n - col : 8;
+            float x[8];
+            float4* src = reinterpret_cast<float4*>(tile + tr * kEpiLd + c8);
+            const float4 lo = src[0], hi = src[1];
+            x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+            x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+            if (EPI != kStore16 && g.beta != 0.f) {
+              constexpr int P = SPLIT ? 2 : 1;
+              const __half* cp = g.c + int64_t(w.index) * P * g.c_plane + int64_t(row) * g.ldc + col;
+              float y[8];
+              load8(cp, y, count, g.c_vec);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = fmaf(g.beta, y[j], x[j]);
+              if (SPLIT) {
+                load8(cp + g.c_plane, y, count, g.c_vec);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = fmaf(g.beta, y[j], x[j]);
+              }
+              if (mirror) {
+                src[0] = make_float4(x[0], x[1], x[2], x[3]);
+                src[1] = make_float4(x[4], x[5], x[6], x[7]);
+              }
+            }
+            emit<EPI, SPLIT>(g, MODE == kRaggedM ? 0 : w.index, int64_t(w.row0) + row, col, x, count);
+          }
+        }
+        if (mirror) {  // the transposed piece (never on the diagonal; rows and columns < m = n)
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tc = i * 8 + r8, row = gc0 + tc, col = row_base + c8;
+            if (row < g.n && col < w.rows) {
+              const int count = w.rows - col < 8 ? w.rows - col : 8;
+              float x[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = tile[(c8 + j) * kEpiLd + tc];
+              emit<EPI, SPLIT>(g, w.index, row, col, x, count);
+            }
+          }
+        }
+        __syncwarp();
+      };
+
+      if (num_k == 0) {  // nothing to sum: zeros (rows of no group, a group without rows)
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+#pragma unroll 1
+        for (int cc = 0; cc < kChunks; ++cc) piece(v, cc);
+        continue;
+      }
+      bool ok = true;
+      if (SPLIT) {
+        float sum[kChunks][32];
+        const int chunks = (num_k + kChunk - 1) / kChunk;
+        for (int ch = 0; ch < chunks; ++ch, ++round) {
+          const uint32_t buf = round & 1u;
+          ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +
+                               (uint32_t(q * 32) << 16);
+#pragma unroll
+          for (int cc = 0; cc < kChunks; ++cc) {
+            float v[32];
+            tmem_ld32(acc + uint32_t(cc * 32), v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[cc][j] = ch ? sum[cc][j] + v[j] : v[j];
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int cc = 0; cc < kChunks; ++cc) piece(sum[cc], cc);
+      } else {
+        const uint32_t buf = round & 1u;
+        if (!wait_bar(&tfull[buf], (round >> 1) & 1u, status)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +
+                             (uint32_t(q * 32) << 16);
+#pragma unroll 1
+        for (int cc = 0; cc < kChunks; ++cc) {
+          float v[32];
+          tmem_ld32(acc + uint32_t(cc * 32), v);
+          piece(v, cc);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
+        ++round;
+      }
+    }
+  }
+  // The other CTA's barriers and shared memory are used until both are done.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(uint32_t(C::TMEM_COLS))
+                 : "memory");
+  }
+}
+
+// ------------------------------- host side --------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+bool resolve_encode() {
+  std::call_once(g_encode_once, []() {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  return g_encode != nullptr;
+}
+
+bool make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows) {
+  if ((reinterpret_cast<uintptr_t>(o.base) & 15) || o.ld % 8 || (o.count > 1 && o.stride % 8))
+    return false;
+  cuuint64_t dims[3] = {cuuint64_t(o.cols), cuuint64_t(o.rows), cuuint64_t(o.count)};
+  cuuint64_t strides[2] = {cuuint64_t(o.ld) * 2,
+                           cuuint64_t(o.count > 1 ? o.stride : o.ld * o.rows) * 2};
+  cuuint32_t box[3] = {cuuint32_t(kBlockK), cuuint32_t(o.mn_major ? kBlockK : box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return g_encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(o.base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int g_sms = 148;
+
+template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
+cudaError_t set_smem() {
+  return cudaFuncSetAttribute(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<BN>::SMEM));
+}
+
+template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
+int launch(const Product& p, cudaStream_t q) {
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, p.a, p.bf16, 128) || !make_map(&mb, p.b, p.bf16, BN / 2))
+    return CHOL_ERR_UNSUPPORTED;
+  Args g{};
+  g.m = int(p.m), g.n = int(p.n), g.k = int(p.k), g.batch = int(p.batch);
+  g.tiles_m = int((p.m + kTileM - 1) / kTileM);
+  g.tiles_n = int((p.n + BN - 1) / BN);
+  int64_t per = int64_t(g.tiles_m) * g.tiles_n;
+  if (p.symmetric) {
+    const int ratio = kTileM / BN;
+    g.symmetric = ratio;
+    per = 0;
+    for (int tm = 0; tm < g.tiles_m; ++tm)
+      per += ratio * (tm + 1) < g.tiles_n ? ratio * (tm + 1) : g.tiles_n;
+  }
+  int64_t total = per * p.batch;
+  if (MODE == kRaggedM)  // an upper bound: every group may end in a partial tile
+    total = ((p.total_rows + kTileM - 1) / kTileM + p.batch + 2) * g.tiles_n;
+  if (per > 0x7fffffffLL || total > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;
+  if (total == 0) return CHOL_OK;
+  g.per_matrix = int(per);
+  g.alpha = p.alpha, g.beta = p.beta;
+  g.c = static_cast<const __half*>(p.c);
+  g.ldc = p.ldc, g.c_plane = p.c_plane;
+  g.c_vec = p.c != nullptr && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % 8 == 0 &&
+            p.c_plane % 8 == 0;
+  g.out = p.out;
+  g.ldo = p.ldo, g.out_stride = p.out_stride, g.out_type = p.out_type;
+  const int per16 = p.out_type == LINALG_FP32 ? 4 : 8;
+  g.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldo % per16 == 0 &&
+              p.out_stride % per16 == 0;
+  g.decay = p.decay, g.rate = p.rate;
+  g.offsets = p.offsets, g.offsets64 = p.offsets64;
+  g.total_rows = int(p.total_rows), g.fill = p.fill;
+  const uint32_t type = p.bf16 ? 1u : 0u;
+  g.idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(AMN) << 15) |
+            (uint32_t(BMN) << 16) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+  int64_t pairs = g_sms / 2;
+  if (pairs > total) pairs = total;
+  return chol::status_from(chol::launch_pdl(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
+                                            dim3(unsigned(2 * pairs)), dim3(kThreads),
+                                            Cfg<BN>::SMEM, q, true, ma, mb, g,
+                                            chol::device_status_ptr()));
+}
+
+// BN = 256 wherever the tiles still fill the GPU: the wider tile moves a third less shared
+// memory per product; narrower ones spread a small problem over more pairs.
+bool narrow(const Product& p) {
+  if (p.n <= 128) return true;
+  const int64_t tm = p.mode == kRaggedM ? (p.total_rows + kTileM - 1) / kTileM + p.batch / 2
+                                        : ((p.m + kTileM - 1) / kTileM) * p.batch;
+  return tm * ((p.n + 255) / 256) < g_sms / 2;
+}
+
+}  // namespace
+
+#define LIN_FOR_EACH(F)                              \
+  F(false, false, kBatch, kPlanes, false)            \
+  F(true, true, kBatch, kPlanes, false)              \
+  F(false, true, kBatch, kPlanes, false)             \
+  F(false, false, kBatch, kFinal, false)             \
+  F(false, true, kBatch, kFinal, false)              \
+  F(false, false, kBatch, kMuon, false)              \
+  F(false, true, kBatch, kMuon, false)               \
+  F(false, false, kRaggedM, kStore16, false)         \
+  F(false, true, kRaggedM, kStore16, false)          \
+  F(true, true, kRaggedK, kStore16, false)
+#define LIN_FOR_EACH_SPLIT(F)                        \
+  F(false, false, kBatch, kPlanes, true)             \
+  F(true, true, kBatch, kPlanes, true)               \
+  F(false, true, kBatch, kPlanes, true)              \
+  F(false, false, kBatch, kFinal, true)              \
+  F(false, true, kBatch, kFinal, true)               \
+  F(false, false, kBatch, kMuon, true)               \
+  F(false, true, kBatch, kMuon, true)
+
+int launch_product(const Product& p, cudaStream_t q) {
+  if (!resolve_encode()) return CHOL_ERR_DEVICE;
+  const int64_t lim = 0x7fffffffLL - 512;
+  if (p.m > lim || p.n > lim || p.k > lim || p.batch > lim || p.total_rows > lim)
+    return CHOL_ERR_UNSUPPORTED;
+  const bool small = narrow(p);
+#define LIN_CASE(AMN, BMN, MODE, EPI, SPLIT)                                                \
+  if (p.a.mn_major == AMN && p.b.mn_major == BMN && p.mode == MODE && p.epilogue == EPI &&  \
+      p.split == SPLIT) {                                                                   \
+    if (SPLIT || small) return launch<128, AMN, BMN, MODE, EPI, SPLIT>(p, q);               \
+    return launch<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>(p, q);                     \
+  }
+  LIN_FOR_EACH(LIN_CASE)
+  LIN_FOR_EACH_SPLIT(LIN_CASE)
+#undef LIN_CASE
+  return CHOL_ERR_UNSUPPORTED;
+}
+
+cudaError_t prepare_products() {
+  cudaError_t e;
+  int dev = 0;
+  if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+  if ((e = cudaDeviceGetAttribute(&g_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+    return e;
+#define LIN_SET(AMN, BMN, MODE, EPI, SPLIT)                                                   \
+  if ((e = set_smem<128, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;             \
+  if ((e = set_smem<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;
+  LIN_FOR_EACH(LIN_SET)
+  LIN_FOR_EACH_SPLIT(LIN_SET)
+#undef LIN_SET
+  return resolve_encode() ? cudaSuccess : cudaErrorNotSupported;
+}
+
+int sm_count() { return g_sms; }
+
+}  // namespace lin

@@ -1,0 +1,464 @@
+// lin_ortho.cu — Newton-Schulz orthogonalisation of a batch of matrices, alone and inside the
+// optimiser step around it.
+//
+//   X = u / (||u||_F + eps);  per step  G = X X^T,  B = b G + c G G,  X <- a X + B X
+//
+// (from the right, G = X^T X, X <- a X + X B, when the matrices are taller than wide, so G is
+// always the smaller square). One step is three products of lin_gemm.cu: G and B are
+// symmetric, so only the tiles on and below the diagonal are computed and each is written twice.
+// Per step 3 m^2 n + m^3 multiply-adds (m the smaller side) instead of the full products'
+// 4 m^2 n + 2 m^3.
+//
+// Number format: X, G and B are fp16, scaled by a power of two, and not bf16: |X|, |G| <= ~1.3
+// and |B| <= ~3, so fp16's range is enough, and its 11 bits make each rounding 8 times smaller
+// than bf16's at the same tensor rate. With bf16 results the error is then the last rounding
+// to bf16 (the iteration adds ~6e-4 of the norm against that rounding's 1.7e-3). The scale keeps
+// the small entries of a large matrix (~1 / sqrt(m n) at the start, ~1 / (m sqrt n) in
+// G) out of fp16's subnormals. Full precision (fp16 and fp32 results) keeps two planes,
+// x = hi + lo.
+//
+// The norm is summed in FP64 per block and then over the blocks in a fixed order: the same
+// input gives the same bits, whatever runs beside it.
+#include <math.h>
+
+#include <mutex>
+
+#include "lin_common.cuh"
+
+namespace lin {
+
+namespace {
+
+constexpr int kPrepThreads = 256;
+constexpr int kMaxParts = 256;
+
+struct Matrix {
+  void* data;
+  int64_t ld, stride;
+  int type;
+  int vec;  // rows of 8 elements can be accessed 16 bytes at a time
+};
+
+template <typename T>
+__device__ __forceinline__ void load8t(const T* p, float (&v)[8], int count, bool vec) {
+  if (vec && count == 8) {
+    alignas(16) T h[8];
+#pragma unroll
+    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+      reinterpret_cast<uint4*>(h)[j] = reinterpret_cast<const uint4*>(p)[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8t(T* p, float (&v)[8], int count, bool vec) {
+  alignas(16) T h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    h[j] = from_float<T>(v[j]);
+    v[j] = to_float(h[j]);  // what the array now holds
+  }
+  if (vec && count == 8) {
+#pragma unroll
+    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+      reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(h)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = h[j];
+  }
+}
+__device__ __forceinline__ void load_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
+  if (x.type == LINALG_BF16)
+    load8t(static_cast<const __nv_bfloat16*>(x.data) + at, v, count, x.vec);
+  else if (x.type == LINALG_FP16)
+    load8t(static_cast<const __half*>(x.data) + at, v, count, x.vec);
+  else
+    load8t(static_cast<const float*>(x.data) + at, v, count, x.vec);
+}
+__device__ __forceinline__ void store_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
+  if (x.type == LINALG_BF16)
+    store8t(static_cast<__nv_bfloat16*>(x.data) + at, v, count, x.vec);
+  else if (x.type == LINALG_FP16)
+    store8t(static_cast<__half*>(x.data) + at, v, count, x.vec);
+  else
+    store8t(static_cast<float*>(x.data) + at, v, count, x.vec);
+}
+
+struct Prep {
+  Matrix x, momentum;  // x: the input, or the gradient
+  float beta, gain;  // gain: 1 - beta, rounded once
+  int nesterov;
+  int64_t rows;
+  int n, chunks_row;  // chunks of 8 columns per row
+  int64_t chunks;     // per matrix
+  int parts;          // blocks per matrix
+  double* sums;       // [batch][parts]
+  __half* planes;     // X: [batch][P][rows][ldx]
+  int64_t ldx;
+  float scale, eps;
+};
+
+// The iteration's start value u of one chunk: the input itself, or the momentum average.
+template <bool MUON, bool UPDATE>
+__device__ __forceinline__ void start_value(const Prep& p, int64_t i, int64_t r, int c, int count,
+                                            float (&u)[8]) {
+  load_any(p.x, i * p.x.stride + r * p.x.ld + c, u, count);
+  if (MUON) {
+    float mo[8];
+    const int64_t at = i * p.momentum.stride + r * p.momentum.ld + c;
+    load_any(p.momentum, at, mo, count);
+    if (UPDATE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mo[j] = fmaf(p.beta, mo[j], p.gain * u[j]);
+      store_any(p.momentum, at, mo, count);  // mo: as stored
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = p.nesterov ? fmaf(p.beta, mo[j], p.gain * u[j]) : mo[j];
+  }
+}
+
+// Sum of squares of each block's share, with the momentum updated on the way. Bound by HBM:
+// reads the input (and reads and writes the momentum) once.
+template <bool MUON>
+__global__ void __launch_bounds__(kPrepThreads) sum_kernel(const Prep p) {
+  griddep_wait();
+  griddep_launch();
+  const int64_t i = blockIdx.x / p.parts;
+  const int part = int(blockIdx.x - i * p.parts);
+  double sum = 0.0;
+  for (int64_t t = int64_t(part) * kPrepThreads + threadIdx.x; t < p.chunks;
+       t += int64_t(p.parts) * kPrepThreads) {
+    const int64_t r = t / p.chunks_row;
+    const int c = int(t - r * p.chunks_row) * 8;
+    const int count = p.n - c < 8 ? p.n - c : 8;
+    float u[8];
+    start_value<MUON, true>(p, i, r, c, count, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) sum += double(u[j]) * double(u[j]);
+  }
+  __shared__ double warp_sum[kPrepThreads / 32];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int w = 0; w < kPrepThreads / 32; ++w) s += warp_sum[w];
+    p.sums[blockIdx.x] = s;
+  }
+}
+
+// X = scale * u / (||u||_F + eps) as fp16, or as hi + lo.
+template <bool MUON, bool SPLIT>
+__global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
+  griddep_wait();
+  griddep_launch();
+  const int64_t i = blockIdx.x / p.parts;
+  const int part = int(blockIdx.x - i * p.parts);
+  __shared__ float factor;
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int k = threadIdx.x; k < p.parts; k += 32) s += p.sums[i * p.parts + k];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (threadIdx.x == 0) factor = float(double(p.scale) / (sqrt(s) + double(p.eps)));
+  }
+  __syncthreads();
+  const float f = factor;
+  constexpr int P = SPLIT ? 2 : 1;
+  for (int64_t t = int64_t(part) * kPrepThreads + threadIdx.x; t < p.chunks;
+       t += int64_t(p.parts) * kPrepThreads) {
+    const int64_t r = t / p.chunks_row;
+    const int c = int(t - r * p.chunks_row) * 8;
+    const int count = p.n - c < 8 ? p.n - c : 8;
+    float u[8];
+    start_value<MUON, false>(p, i, r, c, count, u);
+    alignas(16) __half hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = j < count ? u[j] * f : 0.f;
+      hi[j] = __float2half_rn(v);
+      if (SPLIT) lo[j] = __float2half_rn(v - __half2float(hi[j]));
+    }
+    // rows of the workspace hold a multiple of 8 elements: whole chunks are written
+    __half* o = p.planes + (i * P * p.rows + r) * p.ldx + c;
+    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+    if (SPLIT)
+      *reinterpret_cast<uint4*>(o + p.rows * p.ldx) = *reinterpret_cast<const uint4*>(lo);
+  }
+}
+
+int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
+size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
+
+struct Layout {
+  int64_t planes, ldx, lds, side, x_plane, s_plane;
+  size_t x_bytes, s_bytes, sums_bytes, total;
+};
+
+Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
+  Layout l{};
+  l.planes = split ? 2 : 1;
+  l.side = m < n ? m : n;
+  l.ldx = round8(n);
+  l.lds = round8(l.side);
+  l.x_plane = m * l.ldx;
+  l.s_plane = l.side * l.lds;
+  l.x_bytes = round256(size_t(batch) * l.planes * l.x_plane * 2);
+  l.s_bytes = round256(size_t(batch) * l.planes * l.s_plane * 2);
+  l.sums_bytes = round256(size_t(batch) * kMaxParts * sizeof(double));
+  l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
+  return l;
+}
+
+bool valid_type(int t) { return t == LINALG_BF16 || t == LINALG_FP16 || t == LINALG_FP32; }
+int type_bytes(int t) { return t == LINALG_FP32 ? 4 : 2; }
+
+bool valid_matrix(const linalg_matrix* x, int64_t batch, int64_t m, int64_t n) {
+  if (x == nullptr || x->data == nullptr || !valid_type(x->type)) return false;
+  if (reinterpret_cast<uintptr_t>(x->data) % type_bytes(x->type)) return false;
+  if (x->ld < n || (batch > 1 && x->stride < 0)) return false;
+  // rows and matrices of one array must not overlap (the arrays are written)
+  if (batch > 1 && x->stride < (m - 1) * x->ld + n && x->stride != 0) return false;
+  return true;
+}
+
+Matrix device_matrix(const linalg_matrix* x) {
+  Matrix d{x->data, x->ld, x->stride, x->type, 0};
+  const int per16 = 16 / type_bytes(x->type);
+  d.vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->ld % per16 == 0 &&
+          x->stride % per16 == 0;
+  return d;
+}
+
+// Bytes from the first to one past the last element.
+void extent(const linalg_matrix* x, int64_t batch, int64_t m, int64_t n, uintptr_t* lo,
+            uintptr_t* hi) {
+  *lo = reinterpret_cast<uintptr_t>(x->data);
+  *hi = *lo + uintptr_t((batch - 1) * x->stride + (m - 1) * x->ld + n) * type_bytes(x->type);
+}
+bool overlap(const linalg_matrix* x, const linalg_matrix* y, int64_t batch, int64_t m, int64_t n) {
+  uintptr_t a, b, c, d;
+  extent(x, batch, m, n, &a, &b);
+  extent(y, batch, m, n, &c, &d);
+  return a < d && c < b;
+}
+
+// Shared part of both entry points; momentum == nullptr: plain orthogonalisation.
+int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_matrix* out,
+            int64_t batch, int64_t m, int64_t n, double beta, int nesterov, float decay, float rate,
+            int steps, const float* coefficients, float eps, bool split, void* workspace,
+            cudaStream_t q) {
+  const Layout l = layout(batch, m, n, split);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  __half* xs[2] = {reinterpret_cast<__half*>(w), reinterpret_cast<__half*>(w + l.x_bytes)};
+  __half* gram = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
+  __half* poly = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
+  const bool muon = momentum != nullptr;
+  // the largest entries, ~3 in B, stay a factor 5 (full) to 20 (half) under fp16's largest
+  const float scale = split ? 4096.f : 1024.f;
+
+  Prep p{};
+  p.x = device_matrix(x);
+  if (muon) p.momentum = device_matrix(momentum);
+  p.beta = float(beta), p.gain = float(1.0 - beta), p.nesterov = nesterov;
+  p.rows = m, p.n = int(n);
+  p.chunks_row = int((n + 7) / 8);
+  p.chunks = m * p.chunks_row;
+  // about 4 chunks a thread, at most ~16 blocks per SM over the batch
+  int64_t parts = (p.chunks + kPrepThreads * 4 - 1) / (kPrepThreads * 4);
+  const int64_t cap = (int64_t(sm_count()) * 16 + batch - 1) / batch;
+  if (parts > cap) parts = cap;
+  if (parts > kMaxParts) parts = kMaxParts;
+  p.parts = int(parts < 1 ? 1 : parts);
+  p.sums = reinterpret_cast<double*>(w + 2 * l.x_bytes + 2 * l.s_bytes);
+  p.planes = xs[0];
+  p.ldx = l.ldx;
+  p.scale = scale, p.eps = eps;
+  const dim3 grid(unsigned(p.parts * batch)), block(kPrepThreads);
+  cudaError_t e;
+  e = muon ? chol::launch_pdl(sum_kernel<true>, grid, block, 0, q, true, p)
+           : chol::launch_pdl(sum_kernel<false>, grid, block, 0, q, true, p);
+  if (e != cudaSuccess) return CHOL_ERR_LAUNCH;
+  if (muon)
+    e = split ? chol::launch_pdl(scale_kernel<true, true>, grid, block, 0, q, true, p)
+              : chol::launch_pdl(scale_kernel<true, false>, grid, block, 0, q, true, p);
+  else
+    e = split ? chol::launch_pdl(scale_kernel<false, true>, grid, block, 0, q, true, p)
+              : chol::launch_pdl(scale_kernel<false, false>, grid, block, 0, q, true, p);
+  if (e != cudaSuccess) return CHOL_ERR_LAUNCH;
+
+  const bool tall = m > n;
+  const int64_t s = l.side, matrices = batch * l.planes;
+  const Operand sq_gram{gram, s, s, l.lds, matrices, l.s_plane, false};
+  const Operand sq_poly{poly, s, s, l.lds, matrices, l.s_plane, false};
+  for (int k = 0; k < steps; ++k) {
+    const float a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+    const __half* cur = xs[k & 1];
+    const Operand rows_x{cur, m, n, l.ldx, matrices, l.x_plane, false};
+    const Operand cols_x{cur, m, n, l.ldx, matrices, l.x_plane, true};
+    Product g;  // G = X X^T or X^T X
+    g.a = g.b = tall ? cols_x : rows_x;
+    g.epilogue = kPlanes;
+    g.split = split;
+    g.symmetric = true;
+    g.m = g.n = s, g.k = tall ? m : n, g.batch = batch;
+    g.alpha = 1.f / scale;
+    g.out = gram, g.ldo = l.lds, g.out_stride = l.s_plane;
+    int st = launch_product(g, q);
+    if (st != CHOL_OK) return st;
+    Product f;  // B = b G + c G G
+    f.a = f.b = sq_gram;
+    f.epilogue = kPlanes;
+    f.split = split;
+    f.symmetric = true;
+    f.m = f.n = f.k = s, f.batch = batch;
+    f.alpha = c / scale, f.beta = b;
+    f.c = gram, f.ldc = l.lds, f.c_plane = l.s_plane;
+    f.out = poly, f.ldo = l.lds, f.out_stride = l.s_plane;
+    if ((st = launch_product(f, q)) != CHOL_OK) return st;
+    Product u;  // X <- a X + B X or a X + X B
+    u.a = tall ? rows_x : sq_poly;
+    u.b = tall ? sq_poly : cols_x;
+    u.split = split;
+    u.m = m, u.n = n, u.k = s, u.batch = batch;
+    u.alpha = 1.f / scale, u.beta = a;
+    u.c = cur, u.ldc = l.ldx, u.c_plane = l.x_plane;
+    if (k + 1 < steps) {
+      u.epilogue = kPlanes;
+      u.out = xs[(k + 1) & 1], u.ldo = l.ldx, u.out_stride = l.x_plane;
+    } else {
+      u.epilogue = muon ? kMuon : kFinal;
+      u.alpha /= scale, u.beta /= scale;
+      u.out = out->data, u.ldo = out->ld, u.out_stride = out->stride, u.out_type = out->type;
+      u.decay = decay, u.rate = rate;
+    }
+    if ((st = launch_product(u, q)) != CHOL_OK) return st;
+  }
+  return CHOL_OK;
+}
+
+int check_iteration(int64_t batch, int64_t m, int64_t n, int steps, const float* coefficients,
+                    float eps, int precision) {
+  if (batch < 0 || m < 0 || n < 0) return CHOL_ERR_INVALID_ARG;
+  if (steps < 1 || steps > LINALG_MAX_STEPS || coefficients == nullptr) return CHOL_ERR_INVALID_ARG;
+  if (precision < LINALG_PRECISION_AUTO || precision > LINALG_PRECISION_FULL)
+    return CHOL_ERR_INVALID_ARG;
+  for (int i = 0; i < 3 * steps; ++i)
+    if (!isfinite(coefficients[i])) return CHOL_ERR_INVALID_ARG;
+  if (!(eps >= 0.f) || !isfinite(eps)) return CHOL_ERR_INVALID_ARG;
+  return CHOL_OK;
+}
+
+bool too_large(int64_t batch, int64_t m, int64_t n) {
+  const int64_t lim = 1 << 24;  // planes * batch and tile counts stay within 32 bits
+  return batch > lim || m > lim || n > lim;
+}
+
+bool wants_split(int precision, int type) {
+  if (precision == LINALG_PRECISION_AUTO) return type != LINALG_BF16;
+  return precision == LINALG_PRECISION_FULL;
+}
+
+int check_workspace(int64_t batch, int64_t m, int64_t n, bool split, const void* ws, size_t bytes) {
+  if (ws == nullptr || reinterpret_cast<uintptr_t>(ws) % 256) return CHOL_ERR_WORKSPACE;
+  return bytes < layout(batch, m, n, split).total ? CHOL_ERR_WORKSPACE : CHOL_OK;
+}
+
+}  // namespace
+
+int prepare_device(int dev) {
+  static struct {
+    std::once_flag once;
+    int status;
+  } states[64];
+  if (dev < 0 || dev >= 64) return CHOL_ERR_DEVICE;
+  std::call_once(states[dev].once, [dev]() {
+    states[dev].status = chol::prepare_device_checked(dev);
+    int prev = 0;
+    if (states[dev].status != CHOL_OK) return;
+    if (cudaGetDevice(&prev) != cudaSuccess || (prev != dev && cudaSetDevice(dev) != cudaSuccess)) {
+      states[dev].status = CHOL_ERR_DEVICE;
+      return;
+    }
+    if (prepare_products() != cudaSuccess) states[dev].status = CHOL_ERR_DEVICE;
+    if (prev != dev) cudaSetDevice(prev);
+  });
+  return states[dev].status;
+}
+
+int prepare_current() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CHOL_ERR_DEVICE;
+  // A thread that has made no CUDA call yet (torch runs backward passes on threads of its own)
+  // has no current context, and encoding a tensor map needs one: bind it once per thread.
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return CHOL_ERR_DEVICE;
+    bound = dev;
+  }
+  return prepare_device(dev);
+}
+
+}  // namespace lin
+
+using namespace lin;
+
+extern "C" {
+
+int linalg_prepare(int device) { return prepare_device(device); }
+
+size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int precision) {
+  if (batch <= 0 || m <= 0 || n <= 0 || too_large(batch, m, n)) return 0;
+  return layout(batch, m, n, precision != LINALG_PRECISION_HALF).total;
+}
+
+int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64_t batch,
+                         int64_t m, int64_t n, int steps, const float* coefficients, float eps,
+                         int precision, void* workspace, size_t workspace_bytes, void* queue) {
+  int st = check_iteration(batch, m, n, steps, coefficients, eps, precision);
+  if (st != CHOL_OK) return st;
+  if (batch == 0 || m == 0 || n == 0) return CHOL_OK;
+  if (!valid_matrix(x, batch, m, n) || !valid_matrix(out, batch, m, n)) return CHOL_ERR_INVALID_ARG;
+  if (batch > 1 && out->stride == 0) return CHOL_ERR_INVALID_ARG;
+  if (too_large(batch, m, n)) return CHOL_ERR_UNSUPPORTED;
+  const bool same = x->data == out->data && x->ld == out->ld && x->type == out->type &&
+                    (batch == 1 || x->stride == out->stride);
+  if (!same && overlap(x, out, batch, m, n)) return CHOL_ERR_INVALID_ARG;
+  const bool split = wants_split(precision, out->type);
+  if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
+  if ((st = prepare_current()) != CHOL_OK) return st;
+  return iterate(x, nullptr, out, batch, m, n, 0.f, 0, 1.f, 0.f, steps, coefficients, eps, split,
+                 workspace, static_cast<cudaStream_t>(queue));
+}
+
+int linalg_muon_update(const linalg_matrix* param, const linalg_matrix* grad,
+                       const linalg_matrix* momentum, int64_t batch, int64_t m, int64_t n,
+                       double beta, int nesterov, float decay, float rate, int steps,
+                       const float* coefficients, float eps, int precision, void* workspace,
+                       size_t workspace_bytes, void* queue) {
+  int st = check_iteration(batch, m, n, steps, coefficients, eps, precision);
+  if (st != CHOL_OK) return st;
+  if (!isfinite(beta) || !isfinite(decay) || !isfinite(rate)) return CHOL_ERR_INVALID_ARG;
+  if (batch == 0 || m == 0 || n == 0) return CHOL_OK;
+  if (!valid_matrix(param, batch, m, n) || !valid_matrix(grad, batch, m, n) ||
+      !valid_matrix(momentum, batch, m, n))
+    return CHOL_ERR_INVALID_ARG;
+  if (batch > 1 && (param->stride == 0 || momentum->stride == 0)) return CHOL_ERR_INVALID_ARG;
+  if (too_large(batch, m, n)) return CHOL_ERR_UNSUPPORTED;
+  if (overlap(param, grad, batch, m, n) || overlap(param, momentum, batch, m, n) ||
+      overlap(grad, momentum, batch, m, n))
+    return CHOL_ERR_INVALID_ARG;
+  const bool split = wants_split(precision, param->type);
+  if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
+  if ((st = prepare_current()) != CHOL_OK) return st;
+  return iterate(grad, momentum, param, batch, m, n, beta, nesterov, decay, rate, steps,
+                 coefficients, eps, split, workspace, static_cast<cudaStream_t>(queue));
+}
+
+}  // extern "C"

@@ -1,0 +1,223 @@
+"""Products of rows grouped by an index, each group with its own matrix: the expert products of
+a routed layer, with their gradients.
+
+    y[r]  = x[r] @ w[e]                       for offsets[e] <= r < offsets[e + 1]
+    dx[r] = dy[r] @ w[e]^T
+    dw[e] = sum of outer(x[r], dy[r]) over the group
+
+``grouped_matmul`` is differentiable in x and w; ``grouped_outer`` is its weight gradient alone.
+The offsets stay on the device: no call waits for the GPU, and calls can be captured into a CUDA
+graph whose replays see other group sizes. The kernels are the tensor-core products of
+``libchol_b200.so`` (include/linalg_b200.h); CPU tensors raise ``TypeError``, as everywhere in
+this package. The reference project has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+__all__ = ["grouped_matmul", "grouped_outer"]
+
+_TYPES = {torch.bfloat16: _lib.LINALG_BF16, torch.float16: _lib.LINALG_FP16}
+
+
+def _check(t, name: str, dim: int, like: torch.Tensor | None = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be on a CUDA device (this build has no CPU fallback)")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    if t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the other operand's type and device")
+
+
+def _check_offsets(offsets, like: torch.Tensor, groups: int | None = None) -> int:
+    if not isinstance(offsets, torch.Tensor) or offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError("offsets must be an int32 or int64 tensor")
+    if offsets.device != like.device:
+        raise ValueError("offsets must be on the operands' device")
+    if offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+        raise ValueError("offsets must be contiguous, (groups + 1,)")
+    n = offsets.numel() - 1
+    if groups is not None and n != groups:
+        raise ValueError(f"offsets must have {groups + 1} entries, one more than w has matrices")
+    if n > _lib.LINALG_MAX_GROUPS:
+        raise ValueError(f"at most {_lib.LINALG_MAX_GROUPS} groups, got {n}")
+    return n
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with contiguous rows that start on 16-byte boundaries (as the bulk copies need), a
+    copy with padded rows where it has not."""
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and t.stride(-2) % 8 == 0 and
+            t.stride(-2) >= t.shape[-1] and
+            (t.dim() < 3 or (t.stride(0) % 8 == 0 and
+                             t.stride(0) >= t.shape[-1] + (t.shape[-2] - 1) * t.stride(-2)))):
+        return t
+    cols = t.shape[-1]
+    padded = t.new_empty(*t.shape[:-1], (cols + 7) // 8 * 8)[..., :cols]
+    return padded.copy_(t)
+
+
+def _matrix(t: torch.Tensor) -> tuple[int, int, int, int]:
+    return t.data_ptr(), t.stride(-2), (t.stride(0) if t.dim() == 3 else 0), _TYPES[t.dtype]
+
+
+def _on_device(t: torch.Tensor, call):
+    if t.device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(t.device):
+        return call()
+
+
+def _matmul(x, w, offsets, out=None):
+    rows, k = x.shape
+    groups, _, n = w.shape
+    fill = out is None
+    if out is None:
+        out = x.new_empty(rows, n)
+    if rows == 0 or n == 0:
+        return out
+    if k == 0 or groups == 0:
+        if groups and not fill:
+            raise ValueError("out needs k > 0")
+        return out.zero_() if fill else out
+    w_rows_k = not (w.stride(1) == 1 and w.stride(2) != 1)
+
+    def call():
+        a = _aligned(x)
+        b = _aligned(w if w_rows_k else w.transpose(1, 2))
+        return _lib.linalg().grouped_matmul(
+            *_matrix(a), *_matrix(b), *_matrix(out), int(w_rows_k), offsets.data_ptr(),
+            int(offsets.dtype == torch.int64), groups, rows, k, n, int(fill),
+            _lib.current_queue(x.device))
+
+    _lib.check(_on_device(x, call), "linalg_grouped_matmul")
+    return out
+
+
+def _outer(a, b, offsets, groups, out=None):
+    rows, k = a.shape
+    n = b.shape[1]
+    if out is None:
+        out = a.new_empty(groups, k, n)
+    if out.numel() == 0:
+        return out
+    if rows == 0:
+        return out.zero_()
+
+    def call():
+        p, q = _aligned(a), _aligned(b)
+        return _lib.linalg().grouped_outer(
+            *_matrix(p), *_matrix(q), *_matrix(out), offsets.data_ptr(),
+            int(offsets.dtype == torch.int64), groups, rows, k, n, _lib.current_queue(a.device))
+
+    _lib.check(_on_device(a, call), "linalg_grouped_outer")
+    return out
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets):
+        ctx.save_for_backward(x, w, offsets)
+        return _matmul(x, w, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = _matmul(dy, w.transpose(1, 2), offsets)
+        if ctx.needs_input_grad[1]:
+            if w.stride(1) == 1 and w.stride(2) != 1:  # stored (groups, n, k): so is its gradient
+                dw = _outer(dy, x, offsets, w.shape[0]).transpose(1, 2)
+            else:
+                dw = _outer(x, dy, offsets, w.shape[0])
+        return dx, dw, None
+
+
+def _check_out(out, shape, like, name, others):
+    _check(out, name, len(shape), like)
+    if tuple(out.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(out.shape)}")
+    if out.numel() == 0:
+        return
+    rows, cols = shape[-2:]
+    ld = out.stride(-2)
+    if out.stride(-1) != 1 or ld < cols or (
+            len(shape) == 3 and out.stride(0) < (rows - 1) * ld + cols):
+        raise ValueError(f"{name} must have contiguous, separate rows")
+    if torch.is_grad_enabled() and (out.requires_grad or any(o.requires_grad for o in others)):
+        raise RuntimeError(f"{name}= is not differentiable: call it under torch.no_grad()")
+
+    def ends(t):
+        last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    o0, o1 = ends(out)
+    for t in others:
+        if t.numel():
+            t0, t1 = ends(t)
+            if o0 < t1 and t0 < o1:
+                raise ValueError(f"{name} must not overlap the operands")
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[r] = x[r] @ w[e]`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of each group.
+
+    x: ``(rows, k)``, w: ``(groups, k, n)``, bfloat16 or float16 CUDA tensors of one type; sums in
+    FP32, rounded once. w may be the transposed view of ``(groups, n, k)`` weights, read as it
+    lies. Rows that do not start on 16-byte boundaries (k or n not a multiple of 8) and other
+    layouts are copied first. offsets: ``(groups + 1,)`` int32 or int64 on the device,
+    non-decreasing within ``[0, rows]`` (values that are not are clamped: no row outside x is
+    touched); groups may be empty. Rows of no group (padding in front of offsets[0] or behind
+    offsets[-1]) are zero in the result; with ``out`` given they stay as they were. At most
+    1024 groups.
+
+    Differentiable in x and w (without ``out``): the gradient of a group without rows, and of rows
+    of no group, is zero; dy's rows of no group are not read. Runs on the current queue of x's
+    device.
+    """
+    _check(x, "x", 2)
+    _check(w, "w", 3, x)
+    if w.shape[1] != x.shape[1]:
+        raise ValueError(f"w must be (groups, {x.shape[1]}, n), got {tuple(w.shape)}")
+    _check_offsets(offsets, x, w.shape[0])
+    if out is not None:
+        _check_out(out, (x.shape[0], w.shape[2]), x, "out", (x, w))
+        _matmul(x, w, offsets, out)
+        torch.autograd.graph.increment_version(out)
+        return out
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _GroupedMatmul.apply(x, w, offsets)
+    return _matmul(x, w, offsets)
+
+
+def grouped_outer(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, *,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """``dw[e] = a[i:j].T @ b[i:j]`` with ``i, j = offsets[e], offsets[e + 1]``: the weight gradient
+    of ``grouped_matmul``, ``(groups, k, n)`` for a ``(rows, k)`` and b ``(rows, n)``.
+
+    Types, layouts and offsets as in ``grouped_matmul``. A group without rows gives zeros. Rows
+    of no group are never read into a result, whatever they hold. Not differentiable.
+    """
+    _check(a, "a", 2)
+    _check(b, "b", 2, a)
+    if a.shape[0] != b.shape[0]:
+        raise ValueError(f"a and b must have the same rows, got {a.shape[0]} and {b.shape[0]}")
+    groups = _check_offsets(offsets, a)
+    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad):
+        raise RuntimeError("grouped_outer has no derivative: call it under torch.no_grad()")
+    if out is not None:
+        _check_out(out, (groups, a.shape[1], b.shape[1]), a, "out", (a, b))
+    result = _outer(a, b, offsets, groups, out)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return result
