@@ -19,8 +19,11 @@
 //   warp 2       TMEM allocation; with a ragged K: waits for each landed stage of its own CTA, zeroes
 //                the rows of a group's last block that belong to the next group (they may
 //                hold anything, NaN included), and reports to the first CTA.
-//   warps 4..11  epilogue: TMEM -> registers -> a 32 x 32 staging tile -> rows of 16-byte
-//                stores, overlapped with the next tile (two accumulators).
+//   warps 4..11  epilogue, overlapped with the next tile (two accumulators): a lane holds 32
+//                columns of one row and reads C and writes the result in 32-byte accesses
+//                straight from registers. (Staging the tile through shared memory for coalesced
+//                rows took the bandwidth the operands need, and C loaded where it is used left
+//                each piece waiting for L2: b640n512 4.80 ms, against XXX ms.)
 //
 // The grid is persistent: one pair per two SMs, tiles round-robin. Groups' sizes are read from
 // device memory by every CTA, so the host needs no synchronisation.
@@ -53,7 +56,7 @@ constexpr int kBlockK = 64;     // 16-bit elements of K per stage: one 128-byte 
 constexpr int kTileM = 256;     // rows of a pair's tile
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
-constexpr int kEpiLd = 36;      // staging row stride in floats: conflict-free 16-byte access
+constexpr int kEpiLd = 33;      // staging row stride in floats: conflict-free by row and by column
 constexpr int kChunk = 4;       // split: K blocks per drained accumulator
 
 template <int BN>
@@ -78,7 +81,7 @@ struct Args {
   void* out;
   int64_t ldo, out_stride;
   int out_type;
-  int c_vec, out_vec;  // 16-byte access possible
+  int out_vec;  // rows of the output start on 32-byte sectors
   float decay, rate;
   const void* offsets;
   int offsets64;
@@ -229,86 +232,76 @@ struct Walker {
   }
 };
 
-// Eight consecutive results of one row to 16-bit or 32-bit memory, `count` of them valid.
+// 32-byte accesses: a lane holds 32 columns of one row, so each access is one whole sector.
+__device__ __forceinline__ void ldg32(const void* p, uint32_t* r) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void stg32(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], int count, bool vec) {
-  if (vec && count == 8) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      alignas(16) T h[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = from_float<T>(v[j]);
-      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-    }
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  if constexpr (sizeof(T) == 4) {
+    return 0;
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) p[j] = from_float<T>(v[j]);
+    alignas(4) T h[2] = {from_float<T>(a), from_float<T>(b)};
+    return *reinterpret_cast<const uint32_t*>(h);
   }
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8], int count, bool vec) {
-  if (vec && count == 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      alignas(16) T h[8];
-      *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
-  }
+__device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
+  const T* h = reinterpret_cast<const T*>(&w);
+  a = to_float(h[0]);
+  b = to_float(h[1]);
 }
 
+// 32 columns of a row in 32-byte accesses.
 template <typename T>
-__device__ __forceinline__ void write_weights(T* p, const float (&v)[8], int count, bool vec,
-                                              float decay, float rate) {
-  float w[8];
-  load8(p, w, count, vec);
+__device__ __forceinline__ void store_row(T* p, const float (&v)[32]) {
+  constexpr int N = 32 * int(sizeof(T)) / 4;  // words
+  uint32_t r[N];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = fmaf(-rate, v[j], decay * w[j]);
-  store8(p, w, count, vec);
+  for (int j = 0; j < N; ++j)
+    r[j] = sizeof(T) == 4 ? __float_as_uint(v[j]) : pack<T>(v[(2 * j) & 31], v[(2 * j + 1) & 31]);
+#pragma unroll
+  for (int j = 0; j < N; j += 8) stg32(reinterpret_cast<uint32_t*>(p) + j, r + j);
 }
-
-// Results v of output row r, columns c.. of matrix i.
-template <int EPI, bool SPLIT>
-__device__ __forceinline__ void emit(const Args& g, int i, int64_t r, int c, const float (&v)[8],
-                                     int count) {
-  if (EPI == kPlanes) {
-    constexpr int P = SPLIT ? 2 : 1;
-    __half* o = static_cast<__half*>(g.out) + int64_t(i) * P * g.out_stride + r * g.ldo + c;
-    store8(o, v, count, g.out_vec);
-    if (SPLIT) {
-      float lo[8];
+template <typename T>
+__device__ __forceinline__ void load_row(const T* p, float (&v)[32]) {
+  constexpr int N = 32 * int(sizeof(T)) / 4;
+  uint32_t r[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
-      store8(o + g.out_stride, lo, count, g.out_vec);
-    }
-    return;
-  }
-  const int64_t at = int64_t(i) * g.out_stride + r * g.ldo + c;
-  if (EPI == kMuon) {
-    if (g.out_type == LINALG_BF16)
-      write_weights(static_cast<__nv_bfloat16*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
-    else if (g.out_type == LINALG_FP16)
-      write_weights(static_cast<__half*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
+  for (int j = 0; j < N; j += 8) ldg32(reinterpret_cast<const uint32_t*>(p) + j, r + j);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if constexpr (sizeof(T) == 4)
+      v[j] = __uint_as_float(r[j]);
     else
-      write_weights(static_cast<float*>(g.out) + at, v, count, g.out_vec, g.decay, g.rate);
-    return;
+      unpack<T>(r[j], v[2 * j], v[2 * j + 1]);
   }
-  if (g.out_type == LINALG_BF16)
-    store8(static_cast<__nv_bfloat16*>(g.out) + at, v, count, g.out_vec);
-  else if (g.out_type == LINALG_FP16)
-    store8(static_cast<__half*>(g.out) + at, v, count, g.out_vec);
-  else
-    store8(static_cast<float*>(g.out) + at, v, count, g.out_vec);
+}
+template <typename T>
+__device__ __forceinline__ void write_row(T* p, float (&v)[32], bool weights, float decay,
+                                          float rate) {
+  if (weights) {
+    float w[32];
+    load_row(p, w);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = fmaf(-rate, v[j], decay * w[j]);
+  }
+  store_row(p, v);
+}
+// One column of a 32 x 32 piece's row (any alignment, any number of columns).
+template <typename T>
+__device__ __forceinline__ void write_one(T* p, float v, bool weights, float decay, float rate) {
+  if (weights) v = fmaf(-rate, v, decay * to_float(*p));
+  *p = from_float<T>(v);
 }
 
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
@@ -554,7 +547,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; half of the columns
     float* tile = epi + (warp - 4) * 32 * kEpiLd;
     constexpr int kCols = BN / 2, kChunks = kCols / 32;
-    const int r8 = lane >> 2, c8 = (lane & 3) * 8;
     uint32_t round = 0;
     for (int t = pair; t < total; t += pairs) {
       walk.at(t, w);
@@ -563,70 +555,138 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       const int col0 = w.tn * BN + half * kCols;
       const bool mirror = EPI == kPlanes && g.symmetric && w.tm * kTileM > w.tn * BN + BN - 1;
 
+      // C of one 32 x 32 piece, this lane's row (whole pieces only; loaded ahead of their use)
+      constexpr bool kHasC = EPI != kStore16;
+      constexpr int P = SPLIT ? 2 : 1;
+      const int row = row_base + lane;
+      auto load_c = [&](int cc, uint32_t (&cw)[P][16]) {
+        const int gc0 = col0 + cc * 32;
+        if (!kHasC || g.beta == 0.f || row >= w.rows || gc0 + 32 > g.n) return;
+        const __half* cp = g.c + int64_t(w.index) * P * g.c_plane + int64_t(row) * g.ldc + gc0;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          ldg32(cp + p * g.c_plane, cw[p]);
+          ldg32(cp + p * g.c_plane + 16, cw[p] + 8);
+        }
+      };
       // one 32 x 32 piece: v = this lane's row of accumulators
-      auto piece = [&](const float (&v)[32], int cc) {
+      auto piece = [&](float (&v)[32], int cc, const uint32_t (&cw)[P][16]) {
         const int gc0 = col0 + cc * 32;
         if (gc0 >= g.n || row_base >= w.rows) return;
-        float* trow = tile + lane * kEpiLd;
+        const int cols = g.n - gc0 < 32 ? g.n - gc0 : 32;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<float4*>(trow + 4 * j) =
-              make_float4(g.alpha * v[4 * j], g.alpha * v[4 * j + 1], g.alpha * v[4 * j + 2],
-                          g.alpha * v[4 * j + 3]);
-        __syncwarp();
+        for (int j = 0; j < 32; ++j) v[j] *= g.alpha;
+        if (kHasC && g.beta != 0.f) {
+          if (cols == 32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tr = i * 8 + r8, row = row_base + tr, col = gc0 + c8;
-          if (row < w.rows && col < g.n) {
-            const int count = g.n - col < 8 ? g.n - col : 8;
-            float x[8];
-            float4* src = reinterpret_cast<float4*>(tile + tr * kEpiLd + c8);
-            const float4 lo = src[0], hi = src[1];
-            x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-            x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-            if (EPI != kStore16 && g.beta != 0.f) {
-              constexpr int P = SPLIT ? 2 : 1;
-              const __half* cp = g.c + int64_t(w.index) * P * g.c_plane + int64_t(row) * g.ldc + col;
-              float y[8];
-              load8(cp, y, count, g.c_vec);
+            for (int p = 0; p < P; ++p)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = fmaf(g.beta, y[j], x[j]);
-              if (SPLIT) {
-                load8(cp + g.c_plane, y, count, g.c_vec);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = fmaf(g.beta, y[j], x[j]);
+              for (int j = 0; j < 16; ++j) {
+                float c0, c1;
+                unpack<__half>(cw[p][j], c0, c1);
+                v[2 * j] = fmaf(g.beta, c0, v[2 * j]);
+                v[2 * j + 1] = fmaf(g.beta, c1, v[2 * j + 1]);
               }
-              if (mirror) {
-                src[0] = make_float4(x[0], x[1], x[2], x[3]);
-                src[1] = make_float4(x[4], x[5], x[6], x[7]);
-              }
-            }
-            emit<EPI, SPLIT>(g, MODE == kRaggedM ? 0 : w.index, int64_t(w.row0) + row, col, x, count);
+          } else if (row < w.rows) {
+            const __half* cp = g.c + int64_t(w.index) * P * g.c_plane + int64_t(row) * g.ldc + gc0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < cols)
+                for (int p = 0; p < P; ++p)
+                  v[j] = fmaf(g.beta, __half2float(cp[p * g.c_plane + j]), v[j]);
           }
         }
-        if (mirror) {  // the transposed piece (never on the diagonal; rows and columns < m = n)
-          __syncwarp();
+        if (EPI == kPlanes) {
+          // rows of the workspace are padded to whole 32-byte sectors
+          __half* o = static_cast<__half*>(g.out) + int64_t(w.index) * P * g.out_stride;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tc = i * 8 + r8, row = gc0 + tc, col = row_base + c8;
-            if (row < g.n && col < w.rows) {
-              const int count = w.rows - col < 8 ? w.rows - col : 8;
-              float x[8];
+          for (int p = 0; p < P; ++p, o += g.out_stride) {
+            uint32_t h[16];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = tile[(c8 + j) * kEpiLd + tc];
-              emit<EPI, SPLIT>(g, w.index, row, col, x, count);
+            for (int j = 0; j < 16; ++j) h[j] = pack<__half>(v[2 * j], v[2 * j + 1]);
+            if (row < w.rows) {
+              __half* q0 = o + int64_t(row) * g.ldo + gc0;
+              if (cols == 32) {
+                stg32(q0, h);
+                stg32(q0 + 16, h + 8);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)  // the pad after an odd last column exists
+                  if (2 * j < cols) reinterpret_cast<uint32_t*>(q0)[j] = h[j];
+              }
             }
+            if (mirror) {
+              // the transposed piece (its columns all exist): neighbouring lanes exchange halves,
+              // so that an even lane writes column 2j and an odd one column 2j + 1 of two rows
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, h[j], 1);
+                const uint32_t two = (lane & 1) ? __byte_perm(other, h[j], 0x7632)
+                                                : __byte_perm(h[j], other, 0x5410);
+                const int r = row & ~1;
+                if (r < w.rows)
+                  *reinterpret_cast<uint32_t*>(o + int64_t(gc0 + 2 * j + (lane & 1)) * g.ldo + r) =
+                      two;
+              }
+            }
+            if (SPLIT && p == 0) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float c0, c1;
+                unpack<__half>(h[j], c0, c1);
+                v[2 * j] -= c0;
+                v[2 * j + 1] -= c1;
+              }
+            }
+          }
+          return;
+        }
+        constexpr bool kWeights = EPI == kMuon;
+        const int64_t base = int64_t(MODE == kRaggedM ? 0 : w.index) * g.out_stride +
+                             int64_t(w.row0) * g.ldo + gc0;
+        if (cols == 32 && g.out_vec) {
+          if (row < w.rows) {
+            const int64_t at = base + int64_t(row) * g.ldo;
+            if (g.out_type == LINALG_BF16)
+              write_row(static_cast<__nv_bfloat16*>(g.out) + at, v, kWeights, g.decay, g.rate);
+            else if (g.out_type == LINALG_FP16)
+              write_row(static_cast<__half*>(g.out) + at, v, kWeights, g.decay, g.rate);
+            else if (EPI != kStore16)
+              write_row(static_cast<float*>(g.out) + at, v, kWeights, g.decay, g.rate);
+          }
+          return;
+        }
+        // rows that do not start on sectors, or the last columns: through shared memory, so that
+        // a warp writes along a row
+#pragma unroll
+        for (int j = 0; j < 32; ++j) tile[lane * kEpiLd + j] = v[j];
+        __syncwarp();
+        const int rows = w.rows - row_base < 32 ? w.rows - row_base : 32;
+        if (lane < cols) {
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r) {
+            const float x = tile[r * kEpiLd + lane];
+            const int64_t at = base + int64_t(row_base + r) * g.ldo + lane;
+            if (g.out_type == LINALG_BF16)
+              write_one(static_cast<__nv_bfloat16*>(g.out) + at, x, kWeights, g.decay, g.rate);
+            else if (g.out_type == LINALG_FP16)
+              write_one(static_cast<__half*>(g.out) + at, x, kWeights, g.decay, g.rate);
+            else if (EPI != kStore16)
+              write_one(static_cast<float*>(g.out) + at, x, kWeights, g.decay, g.rate);
           }
         }
         __syncwarp();
       };
 
       if (num_k == 0) {  // nothing to sum: zeros (rows of no group, a group without rows)
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+        const uint32_t none[P][16] = {};
 #pragma unroll 1
-        for (int cc = 0; cc < kChunks; ++cc) piece(v, cc);
+        for (int cc = 0; cc < kChunks; ++cc) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
+          piece(v, cc, none);
+        }
         continue;
       }
       bool ok = true;
@@ -653,18 +713,25 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc) piece(sum[cc], cc);
+        for (int cc = 0; cc < kChunks; ++cc) {
+          uint32_t cw[P][16];
+          load_c(cc, cw);
+          piece(sum[cc], cc, cw);
+        }
       } else {
         const uint32_t buf = round & 1u;
+        uint32_t cw[2][P][16];
+        load_c(0, cw[0]);
         if (!wait_bar(&tfull[buf], (round >> 1) & 1u, status)) break;
         tc_fence_after();
         const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +
                              (uint32_t(q * 32) << 16);
-#pragma unroll 1
+#pragma unroll
         for (int cc = 0; cc < kChunks; ++cc) {
+          if (cc + 1 < kChunks) load_c(cc + 1, cw[(cc + 1) & 1]);
           float v[32];
           tmem_ld32(acc + uint32_t(cc * 32), v);
-          piece(v, cc);
+          piece(v, cc, cw[cc & 1]);
         }
         tc_fence_before();
         __syncwarp();
@@ -750,13 +817,11 @@ int launch(const Product& p, cudaStream_t q) {
   g.alpha = p.alpha, g.beta = p.beta;
   g.c = static_cast<const __half*>(p.c);
   g.ldc = p.ldc, g.c_plane = p.c_plane;
-  g.c_vec = p.c != nullptr && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % 8 == 0 &&
-            p.c_plane % 8 == 0;
   g.out = p.out;
   g.ldo = p.ldo, g.out_stride = p.out_stride, g.out_type = p.out_type;
-  const int per16 = p.out_type == LINALG_FP32 ? 4 : 8;
-  g.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldo % per16 == 0 &&
-              p.out_stride % per16 == 0;
+  const int sector = p.out_type == LINALG_FP32 ? 8 : 16;
+  g.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % sector == 0 &&
+              p.out_stride % sector == 0;
   g.decay = p.decay, g.rate = p.rate;
   g.offsets = p.offsets, g.offsets64 = p.offsets64;
   g.total_rows = int(p.total_rows), g.fill = p.fill;

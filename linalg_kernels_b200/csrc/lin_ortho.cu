@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
   }
 }
 
-int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
+// rows of the workspace start on 32-byte sectors
+int64_t round16(int64_t v) { return (v + 15) & ~int64_t(15); }
 size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
 
 struct Layout {
@@ -205,8 +206,8 @@ Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   Layout l{};
   l.planes = split ? 2 : 1;
   l.side = m < n ? m : n;
-  l.ldx = round8(n);
-  l.lds = round8(l.side);
+  l.ldx = round16(n);
+  l.lds = round16(l.side);
   l.x_plane = m * l.ldx;
   l.s_plane = l.side * l.lds;
   l.x_bytes = round256(size_t(batch) * l.planes * l.x_plane * 2);
