@@ -16,9 +16,10 @@
 //                copies report to the full barrier of the pair's first CTA.
 //   warp 1       the first CTA's lane 0 issues tcgen05.mma (M256 x BN x K16); the commits free the
 //                stage in both CTAs.
-//   warp 2       TMEM allocation; with a ragged K: waits for each landed stage of its own CTA, zeroes
-//                the rows of a group's last block that belong to the next group (they may
-//                hold anything, NaN included), and reports to the first CTA.
+//   warp 2       TMEM allocation; with a ragged K, where a group ends inside a 16-wide slab: once its
+//                CTA's part of the last block has landed, zeroes the slab's rows that belong to
+//                the next group (they may hold anything, NaN included). (Passing every stage
+//                through this warp cost the weight gradient of 16384 rows 398 us, against XXX.)
 //   warps 4..11  epilogue, overlapped with the next tile (two accumulators): a lane holds 32
 //                columns of one row and reads C and writes the result in 32-byte accesses
 //                straight from registers. (Staging the tile through shared memory for coalesced
@@ -58,14 +59,15 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kEpiLd = 33;      // staging row stride in floats: conflict-free by row and by column
 constexpr int kChunk = 4;       // split: K blocks per drained accumulator
+constexpr int kBand = 8;        // row tiles per band of the tile order
 
 template <int BN>
 struct Cfg {
-  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr int STAGES = BN == 256 ? 6 : 8;
   static constexpr int A_BYTES = 128 * kBlockK * 2;
   static constexpr int B_BYTES = BN / 2 * kBlockK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int EPI = kEpiWarps * 32 * kEpiLd * 4;
+  static constexpr int EPI = kEpiWarps * 16 * kEpiLd * 4;  // half a piece per warp
   static constexpr int TABLE = 2 * (kMaxGroups + 4) * 4;
   static constexpr size_t SMEM = size_t(STAGES) * STAGE + EPI + 512 + TABLE + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
@@ -201,10 +203,7 @@ struct Walker {
       w.index = e;
       w.k0 = 0;
       w.k_len = e < g.batch ? g.k : 0;
-      const int tms = (w.rows + kTileM - 1) / kTileM;
-      const int r = t - first[e];
-      w.tn = r / tms;
-      w.tm = r - w.tn * tms;
+      band(t - first[e], (w.rows + kTileM - 1) / kTileM, w);
       return;
     }
     w.index = t / g.per_matrix;
@@ -226,9 +225,17 @@ struct Walker {
       w.tm = tm;
       w.tn = r - ratio * (tm * (tm + 1) / 2);
     } else {
-      w.tn = r / g.tiles_m;
-      w.tm = r - w.tn * g.tiles_m;
+      band(r, g.tiles_m, w);
     }
+  }
+  // Bands of 8 row tiles, down each column of a band: the tiles in flight at a time then read
+  // about as many rows of A as of B (8192^3 by offsets: 882 -> 842 us, 840 -> 777 with B MN-major).
+  __device__ __forceinline__ void band(int r, int tiles_m, Tile& w) const {
+    const int b = r / (kBand * g.tiles_n);
+    r -= b * kBand * g.tiles_n;
+    const int h = tiles_m - b * kBand < kBand ? tiles_m - b * kBand : kBand;
+    w.tn = r / h;
+    w.tm = b * kBand + r - w.tn * h;
   }
 };
 
@@ -316,11 +323,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   float* epi = reinterpret_cast<float*>(smem + size_t(S) * C::STAGE);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(S) * C::STAGE + C::EPI);
   uint64_t* full = bars;             // [S] first CTA: a stage of both CTAs has landed
-  uint64_t* landed = bars + S;       // [S] kRaggedK: this CTA's part of the stage has landed
+  uint64_t* landed = bars + S;       // [S] kRaggedK: this CTA's part of a group's last block landed
   uint64_t* empty = bars + 2 * S;    // [S] the MMAs have read the stage
   uint64_t* tfull = bars + 3 * S;    // [2] accumulator ready
   uint64_t* tempty = tfull + 2;      // [2] first CTA: accumulator drained by both CTAs
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* clean = tempty + 2;      // [S] kRaggedK, first CTA: the other CTA's part is clean
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(clean + S);
   int* start = reinterpret_cast<int*>(smem + size_t(S) * C::STAGE + C::EPI + 512);
   int* first = start + kMaxGroups + 4;
 
@@ -328,8 +336,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t rank = cta_rank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], MODE == kRaggedK ? 2 : 1);
+      mbar_init(&full[s], 1);
       mbar_init(&landed[s], 1);
+      mbar_init(&clean[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -407,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     // ---------------- TMA producer ----------------
     if (lane == 0) {
       uint32_t kt = 0;
+      uint32_t tails = 0;  // stages whose last copy reports to landed
       bool ok = true;
       for (int t = pair; t < total && ok; t += pairs) {
         walk.at(t, w);
@@ -436,12 +446,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           uint8_t* sa = smem + size_t(s) * C::STAGE;
           uint8_t* sb = sa + C::A_BYTES;
           uint32_t bar;
-          if (MODE == kRaggedK) {
-            mbar_expect_tx(&landed[s], C::STAGE);
+          if (MODE == kRaggedK && kb == num_k - 1 && (w.k_len & 15)) {
+            mbar_expect_tx(&landed[s], C::STAGE);  // warp 2 reports the stage
             bar = smem_u32(&landed[s]);
+            tails |= 1u << s;
           } else {
             if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
             bar = leader_addr(&full[s]);
+            tails &= ~(1u << s);
           }
           const int kx = w.k0 + kb * kBlockK;
           if (AMN) {
@@ -459,9 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
       }
       if (!ok && rank == 0) {
-        // copies still in flight write this pair's shared memory: give them time to land
+        // copies still in flight write this pair's shared memory: give them time to land (those of
+        // a last block are waited for by warp 2)
         for (uint32_t j = kt < uint32_t(S) ? 0 : kt - S; j < kt; ++j)
-          wait_bar(MODE == kRaggedK ? &landed[j % S] : &full[j % S], (j / S) & 1u, status);
+          if (!(tails >> (j % S) & 1u)) wait_bar(&full[j % S], (j / S) & 1u, status);
       }
     }
   } else if (warp == 1) {
@@ -512,40 +525,46 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       }
     }
   } else if (warp == 2) {
-    // ---------------- kRaggedK: end of a group's last block ----------------
+    // ---------------- kRaggedK: the last block of a group that ends inside a 16-wide slab --------
     if (MODE == kRaggedK) {
-      uint32_t kt = 0;
+      uint32_t kt = 0, landed_phase = 0, clean_phase = 0;  // bit s: parity of the next wait
       bool ok = true;
       for (int t = pair; t < total && ok; t += pairs) {
         walk.at(t, w);
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
-        for (int i = 0; i < num_k; ++i, ++kt) {
-          const int s = int(kt % S);
-          ok = wait_bar(&landed[s], (kt / S) & 1u, status);
+        kt += uint32_t(num_k);
+        if ((w.k_len & 15) == 0) continue;
+        const int s = int((kt - 1) % S);
+        ok = wait_bar(&landed[s], landed_phase >> s & 1u, status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        landed_phase ^= 1u << s;
+        // the K rows from the group's end to the end of their slab are read by the MMA: zero them
+        const int left = w.k_len - (num_k - 1) * kBlockK;
+        const int count = ((left + 15) & ~15) - left;
+        uint8_t* sa = smem + size_t(s) * C::STAGE;
+        constexpr int boxes = C::STAGE / 8192;  // A's two, then B's
+        for (int j = lane; j < boxes * count * 8; j += 32) {
+          const int box = j / (count * 8), r = j - box * count * 8;
+          *reinterpret_cast<uint4*>(sa + box * 8192 + (left + (r >> 3)) * 128 + (r & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (rank != 0) {
+          if (lane == 0) arrive_leader(leader_addr(&clean[s]));
+        } else {
+          ok = wait_bar(&clean[s], clean_phase >> s & 1u, status);
           ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int left = w.k_len - i * kBlockK;
-          if (left < kBlockK && (left & 15)) {
-            // K rows left .. the end of their 16-wide slab are read by the MMA: zero them
-            const int z0 = left, count = ((left + 15) & ~15) - left;
-            uint8_t* sa = smem + size_t(s) * C::STAGE;
-            constexpr int boxes = C::STAGE / 8192;  // A's two, then B's
-            for (int j = lane; j < boxes * count * 8; j += 32) {
-              const int box = j / (count * 8), r = j - box * count * 8;
-              *reinterpret_cast<uint4*>(sa + box * 8192 + (z0 + (r >> 3)) * 128 + (r & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
-          __syncwarp();
-          if (lane == 0) arrive_leader(leader_addr(&full[s]));
+          clean_phase ^= 1u << s;
+          if (lane == 0 && ok) arrive_leader(leader_addr(&full[s]));
         }
       }
     }
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; half of the columns
-    float* tile = epi + (warp - 4) * 32 * kEpiLd;
+    float* tile = epi + (warp - 4) * 16 * kEpiLd;
     constexpr int kCols = BN / 2, kChunks = kCols / 32;
     uint32_t round = 0;
     for (int t = pair; t < total; t += pairs) {
@@ -656,26 +675,31 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
           return;
         }
-        // rows that do not start on sectors, or the last columns: through shared memory, so that
-        // a warp writes along a row
+        // rows that do not start on sectors, or the last columns: through shared memory, half a
+        // piece at a time, so that a warp writes along a row
+#pragma unroll 1
+        for (int h = 0; h < 32; h += 16) {
+          if ((lane & 16) == h) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) tile[lane * kEpiLd + j] = v[j];
-        __syncwarp();
-        const int rows = w.rows - row_base < 32 ? w.rows - row_base : 32;
-        if (lane < cols) {
-#pragma unroll 4
-          for (int r = 0; r < rows; ++r) {
-            const float x = tile[r * kEpiLd + lane];
-            const int64_t at = base + int64_t(row_base + r) * g.ldo + lane;
-            if (g.out_type == LINALG_BF16)
-              write_one(static_cast<__nv_bfloat16*>(g.out) + at, x, kWeights, g.decay, g.rate);
-            else if (g.out_type == LINALG_FP16)
-              write_one(static_cast<__half*>(g.out) + at, x, kWeights, g.decay, g.rate);
-            else if (EPI != kStore16)
-              write_one(static_cast<float*>(g.out) + at, x, kWeights, g.decay, g.rate);
+            for (int j = 0; j < 32; ++j) tile[(lane & 15) * kEpiLd + j] = v[j];
           }
+          __syncwarp();
+          const int left = w.rows - row_base - h, rows = left < 16 ? left : 16;
+          if (lane < cols) {
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+              const float x = tile[r * kEpiLd + lane];
+              const int64_t at = base + int64_t(row_base + h + r) * g.ldo + lane;
+              if (g.out_type == LINALG_BF16)
+                write_one(static_cast<__nv_bfloat16*>(g.out) + at, x, kWeights, g.decay, g.rate);
+              else if (g.out_type == LINALG_FP16)
+                write_one(static_cast<__half*>(g.out) + at, x, kWeights, g.decay, g.rate);
+              else if (EPI != kStore16)
+                write_one(static_cast<float*>(g.out) + at, x, kWeights, g.decay, g.rate);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
       };
 
       if (num_k == 0) {  // nothing to sum: zeros (rows of no group, a group without rows)

@@ -30,7 +30,7 @@ namespace lin {
 namespace {
 
 constexpr int kPrepThreads = 256;
-constexpr int kMaxParts = 256;
+constexpr int kMaxParts = 2048;
 
 struct Matrix {
   void* data;
