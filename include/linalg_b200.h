@@ -46,7 +46,9 @@ typedef struct {
 } linalg_matrix;
 
 /* Bytes of device workspace (256-byte aligned) of linalg_orthogonalize and linalg_muon_update
-   for `batch` m x n matrices at a working precision (HALF or FULL; AUTO counts as FULL). */
+   for `batch` m x n matrices at a working precision (HALF or FULL; AUTO counts as FULL). 0 where
+   the iteration runs on chip (smaller side <= 128 and the other within a cluster's shared
+   memory). */
 CHOL_API size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n,
                                                int precision);
 

@@ -1,0 +1,80 @@
+// lin_elem.cuh — element access of the orthogonalisation's first and last passes: caller matrices
+// of any supported type and alignment, eight columns at a time.
+#pragma once
+
+#include "lin_common.cuh"
+
+namespace lin {
+
+struct Matrix {
+  void* data;
+  int64_t ld, stride;
+  int type;
+  int vec;  // rows of 8 elements can be accessed 16 bytes at a time
+};
+
+template <typename T>
+__device__ __forceinline__ void load8t(const T* p, float (&v)[8], int count, bool vec) {
+  if (vec && count == 8) {
+    alignas(16) T h[8];
+#pragma unroll
+    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+      reinterpret_cast<uint4*>(h)[j] = reinterpret_cast<const uint4*>(p)[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8t(T* p, float (&v)[8], int count, bool vec) {
+  alignas(16) T h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    h[j] = from_float<T>(v[j]);
+    v[j] = to_float(h[j]);  // what the array now holds
+  }
+  if (vec && count == 8) {
+#pragma unroll
+    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+      reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(h)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = h[j];
+  }
+}
+__device__ __forceinline__ void load_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
+  if (x.type == LINALG_BF16)
+    load8t(static_cast<const __nv_bfloat16*>(x.data) + at, v, count, x.vec);
+  else if (x.type == LINALG_FP16)
+    load8t(static_cast<const __half*>(x.data) + at, v, count, x.vec);
+  else
+    load8t(static_cast<const float*>(x.data) + at, v, count, x.vec);
+}
+__device__ __forceinline__ void store_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
+  if (x.type == LINALG_BF16)
+    store8t(static_cast<__nv_bfloat16*>(x.data) + at, v, count, x.vec);
+  else if (x.type == LINALG_FP16)
+    store8t(static_cast<__half*>(x.data) + at, v, count, x.vec);
+  else
+    store8t(static_cast<float*>(x.data) + at, v, count, x.vec);
+}
+
+// The factor F of X = F * u, F = scale / (norm + eps), as a power of two near its square root (x)
+// times the rest (y): F alone passes FP32's range for norms of subnormals and for the largest
+// ones, (u * x) * y does not. Not finite: the matrix holds a NaN or an infinity (or norm + eps
+// is zero).
+__device__ __forceinline__ float2 start_factor(double squares, float scale, float eps) {
+  const double f = double(scale) / (sqrt(squares) + double(eps));
+  if (!isfinite(f) || !isfinite(squares)) {
+    const float nan = __int_as_float(0x7fc00000);
+    return make_float2(nan, nan);
+  }
+  const int k = ilogb(f) / 2;
+  return make_float2(float(ldexp(1.0, k)), float(ldexp(f, -k)));
+}
+__device__ __forceinline__ float start_scaled(float u, float2 f) { return (u * f.x) * f.y; }
+
+}  // namespace lin

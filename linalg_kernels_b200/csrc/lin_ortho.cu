@@ -23,7 +23,8 @@
 
 #include <mutex>
 
-#include "lin_common.cuh"
+#include "lin_elem.cuh"
+#include "lin_small.cuh"
 
 namespace lin {
 
@@ -31,62 +32,6 @@ namespace {
 
 constexpr int kPrepThreads = 256;
 constexpr int kMaxParts = 2048;
-
-struct Matrix {
-  void* data;
-  int64_t ld, stride;
-  int type;
-  int vec;  // rows of 8 elements can be accessed 16 bytes at a time
-};
-
-template <typename T>
-__device__ __forceinline__ void load8t(const T* p, float (&v)[8], int count, bool vec) {
-  if (vec && count == 8) {
-    alignas(16) T h[8];
-#pragma unroll
-    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-      reinterpret_cast<uint4*>(h)[j] = reinterpret_cast<const uint4*>(p)[j];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8t(T* p, float (&v)[8], int count, bool vec) {
-  alignas(16) T h[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    h[j] = from_float<T>(v[j]);
-    v[j] = to_float(h[j]);  // what the array now holds
-  }
-  if (vec && count == 8) {
-#pragma unroll
-    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-      reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(h)[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) p[j] = h[j];
-  }
-}
-__device__ __forceinline__ void load_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
-  if (x.type == LINALG_BF16)
-    load8t(static_cast<const __nv_bfloat16*>(x.data) + at, v, count, x.vec);
-  else if (x.type == LINALG_FP16)
-    load8t(static_cast<const __half*>(x.data) + at, v, count, x.vec);
-  else
-    load8t(static_cast<const float*>(x.data) + at, v, count, x.vec);
-}
-__device__ __forceinline__ void store_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
-  if (x.type == LINALG_BF16)
-    store8t(static_cast<__nv_bfloat16*>(x.data) + at, v, count, x.vec);
-  else if (x.type == LINALG_FP16)
-    store8t(static_cast<__half*>(x.data) + at, v, count, x.vec);
-  else
-    store8t(static_cast<float*>(x.data) + at, v, count, x.vec);
-}
 
 struct Prep {
   Matrix x, momentum;  // x: the input, or the gradient
@@ -160,16 +105,16 @@ __global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
   griddep_launch();
   const int64_t i = blockIdx.x / p.parts;
   const int part = int(blockIdx.x - i * p.parts);
-  __shared__ float factor;
+  __shared__ float2 factor;
   if (threadIdx.x < 32) {
     double s = 0.0;
     for (int k = threadIdx.x; k < p.parts; k += 32) s += p.sums[i * p.parts + k];
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (threadIdx.x == 0) factor = float(double(p.scale) / (sqrt(s) + double(p.eps)));
+    if (threadIdx.x == 0) factor = start_factor(s, p.scale, p.eps);
   }
   __syncthreads();
-  const float f = factor;
+  const float2 f = factor;
   constexpr int P = SPLIT ? 2 : 1;
   for (int64_t t = int64_t(part) * kPrepThreads + threadIdx.x; t < p.chunks;
        t += int64_t(p.parts) * kPrepThreads) {
@@ -181,7 +126,7 @@ __global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
     alignas(16) __half hi[8], lo[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = j < count ? u[j] * f : 0.f;
+      const float v = j < count ? start_scaled(u[j], f) : 0.f;
       hi[j] = __float2half_rn(v);
       if (SPLIT) lo[j] = __float2half_rn(v - __half2float(hi[j]));
     }
@@ -204,6 +149,7 @@ struct Layout {
 
 Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   Layout l{};
+  if (small_supported(m, n, split)) return l;  // on chip: no workspace
   l.planes = split ? 2 : 1;
   l.side = m < n ? m : n;
   l.ldx = round16(n);
@@ -255,6 +201,9 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
             int64_t batch, int64_t m, int64_t n, double beta, int nesterov, float decay, float rate,
             int steps, const float* coefficients, float eps, bool split, void* workspace,
             cudaStream_t q) {
+  if (small_supported(m, n, split))
+    return launch_small(x, momentum, out, batch, m, n, beta, nesterov, decay, rate, steps,
+                        coefficients, eps, split, q);
   const Layout l = layout(batch, m, n, split);
   uint8_t* w = static_cast<uint8_t*>(workspace);
   __half* xs[2] = {reinterpret_cast<__half*>(w), reinterpret_cast<__half*>(w + l.x_bytes)};
@@ -367,8 +316,10 @@ bool wants_split(int precision, int type) {
 }
 
 int check_workspace(int64_t batch, int64_t m, int64_t n, bool split, const void* ws, size_t bytes) {
+  const size_t need = layout(batch, m, n, split).total;
+  if (need == 0) return CHOL_OK;
   if (ws == nullptr || reinterpret_cast<uintptr_t>(ws) % 256) return CHOL_ERR_WORKSPACE;
-  return bytes < layout(batch, m, n, split).total ? CHOL_ERR_WORKSPACE : CHOL_OK;
+  return bytes < need ? CHOL_ERR_WORKSPACE : CHOL_OK;
 }
 
 }  // namespace
@@ -387,7 +338,8 @@ int prepare_device(int dev) {
       states[dev].status = CHOL_ERR_DEVICE;
       return;
     }
-    if (prepare_products() != cudaSuccess) states[dev].status = CHOL_ERR_DEVICE;
+    if (prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess)
+      states[dev].status = CHOL_ERR_DEVICE;
     if (prev != dev) cudaSetDevice(prev);
   });
   return states[dev].status;

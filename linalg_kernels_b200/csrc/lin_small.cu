@@ -1,0 +1,615 @@
+// lin_small.cu — the whole Newton-Schulz iteration of small matrices (smaller side <= 128) in one
+// launch, on chip.
+//
+// A matrix is held as s x L, s its smaller side (a tall matrix is transposed on the way in and
+// out). p = floor(128 / s) matrices (s rounded up to 16) are stacked to the 128 rows of one tile: with the entries of
+// G = X X^T between different matrices set to zero, G, G G and B = b G + c G G stay block
+// diagonal and B X acts on each matrix alone, so one set of M = 128 MMAs serves all of them.
+//
+// X lives in shared memory as 128-byte-swizzled K-major blocks of 64 columns; the same bytes are
+// the MN-major B operand of B X (the summed index is then X's row). G and B share one buffer: an
+// epilogue thread overwrites the elements it has read. Accumulators in TMEM, one thread per row
+// and half of the columns.
+//
+//   per step:  G = X X^T -> mask, fp16   |   B = b G + c G G -> fp16   |   X <- a X + B X
+//
+// A long matrix is split over a cluster of 2, 4 or 8 CTAs by columns. Only G needs all columns:
+// each CTA puts its FP32 partial into shared memory, sums one slice of G over the CTAs in rank
+// order (the same bits every time) and writes the rounded slice to all of them.
+//
+// `SPLIT`: two fp16 planes per operand and three products, as in lin_gemm.cu. One accumulator
+// covers at most 192 columns of K, so it needs no drain.
+//
+// Bound by latency: per step three dependent chains MMA -> TMEM read -> convert -> shared memory,
+// MEASURED_SMALL
+#include <cuda.h>
+
+#include "chol_tc_ptx.cuh"
+#include "lin_elem.cuh"
+#include "lin_small.cuh"
+
+namespace lin {
+
+namespace {
+
+using namespace chol::tcx;
+using chol::fence_proxy_async_smem;
+using chol::smem_u32;
+
+constexpr int kThreads = 256;
+constexpr int kBlockBytes = 128 * 128;  // 128 rows x 64 fp16 columns
+
+struct SmallArgs {
+  Matrix x, momentum, out;
+  int s, len;        // smaller side, other side
+  int pitch;         // rows of the tile per matrix: s rounded up to the MMA's 16-wide K slabs, so
+                     // that a matrix's sums do not depend on its place in the tile
+  int tall;
+  int per_cta;       // matrices stacked in one tile
+  int64_t batch;
+  int cta_cols;      // columns per CTA of a cluster (multiple of 64)
+  int ranks;         // CTAs per cluster
+  int steps;
+  int nesterov;
+  float beta, gain, decay, rate;
+  float scale, eps;
+  float coef[3 * LINALG_MAX_STEPS];
+};
+
+__device__ __forceinline__ uint32_t rank_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void sync_cluster() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_remote4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_remote_f64(uint32_t addr) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_remote16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void mma_half(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// X as B operand of B X: N = its columns (contiguous), K = its rows. The next 64 columns are one
+// block further, the next 8 rows 1024 bytes.
+__device__ __forceinline__ uint64_t desc_cols(const void* tile) {
+  const uint32_t addr = smem_u32(tile);
+  uint64_t d = 0;
+  d |= uint64_t((addr >> 4) & 0x3FFF);
+  d |= uint64_t(kBlockBytes >> 4) << 16;
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;
+  return d;
+}
+// fp16 operands, FP32 sums, M = 128.
+__device__ __forceinline__ uint32_t idesc_half(int n, int b_mn_major) {
+  return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (8u << 24);
+}
+// Byte offset of the 16-byte chunk holding columns c .. c + 7 of row r.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return uint32_t(c >> 6) * kBlockBytes + uint32_t(r) * 128 + ((uint32_t(c >> 3) & 7) ^ (r & 7)) * 16;
+}
+
+// Elements (row r of the tile, columns c .. c + 7) of a caller's matrix; the tile's row of matrix i
+// is `r`, in the caller's orientation a column when tall.
+__device__ __forceinline__ void load_tile8(const SmallArgs& g, const Matrix& x, int64_t i, int r,
+                                           int c, int count, float (&v)[8]) {
+  if (!g.tall) {
+    load_any(x, i * x.stride + int64_t(r) * x.ld + c, v, count);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float one[8];
+      v[j] = 0.f;
+      if (j < count) {
+        load_any(x, i * x.stride + int64_t(c + j) * x.ld + r, one, 1);
+        v[j] = one[0];
+      }
+    }
+  }
+}
+__device__ __forceinline__ void store_tile8(const SmallArgs& g, const Matrix& x, int64_t i, int r,
+                                            int c, int count, float (&v)[8]) {
+  if (!g.tall) {
+    store_any(x, i * x.stride + int64_t(r) * x.ld + c, v, count);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) {
+        float one[8] = {v[j]};
+        store_any(x, i * x.stride + int64_t(c + j) * x.ld + r, one, 1);
+        v[j] = one[0];
+      }
+  }
+}
+
+template <bool MUON>
+__device__ __forceinline__ void start8(const SmallArgs& g, int64_t i, int r, int c, int count,
+                                       bool update, float (&u)[8]) {
+  load_tile8(g, g.x, i, r, c, count, u);
+  if (MUON) {
+    float mo[8];
+    load_tile8(g, g.momentum, i, r, c, count, mo);
+    if (update) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mo[j] = fmaf(g.beta, mo[j], g.gain * u[j]);
+      store_tile8(g, g.momentum, i, r, c, count, mo);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = g.nesterov ? fmaf(g.beta, mo[j], g.gain * u[j]) : mo[j];
+  }
+}
+
+// Eight values to fp16 (and the remainder plane): shared-memory chunks of 16 bytes. Saturating: an
+// infinity in one matrix would reach the others of its tile as 0 * inf in B X. (Only
+// coefficients with which the iteration diverges get there: 65504 is 16 times the
+// largest singular value's bound in full precision, 64 times in half.)
+__device__ __forceinline__ uint32_t half2_sat(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <bool SPLIT>
+__device__ __forceinline__ void round8v(const float (&v)[8], uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = half2_sat(v[2 * j], v[2 * j + 1]);
+    if (SPLIT) {
+      const __half2 x = *reinterpret_cast<const __half2*>(&h[j]);
+      l[j] = half2_sat(v[2 * j] - __low2float(x), v[2 * j + 1] - __high2float(x));
+    }
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  if (SPLIT) lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void add8(float (&v)[8], uint4 w, float f) {
+  const __half* h = reinterpret_cast<const __half*>(&w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = fmaf(f, __half2float(h[j]), v[j]);
+}
+
+template <bool SPLIT, bool MUON, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int* status) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  constexpr int P = SPLIT ? 2 : 1;
+  const int blocks = g.cta_cols / 64;
+  const uint32_t x_plane = uint32_t(blocks) * kBlockBytes;
+  uint8_t* xs = smem;                            // [P] X: blocks of 64 columns
+  uint8_t* gs = xs + P * x_plane;                // [P] G, then B: two blocks
+  constexpr uint32_t g_plane = 2 * kBlockBytes;
+  uint8_t* es = gs + P * g_plane;                // CLUSTER: FP32 partial of G, [column / 4][row] x 4
+  double* row_sum = reinterpret_cast<double*>(es);  // [2][128] (CLUSTER: before es is used)
+  double* mat_sum = reinterpret_cast<double*>(es + (CLUSTER ? 65536 : 2048));  // [128] per matrix
+  float2* factor = reinterpret_cast<float2*>(mat_sum + 128);  // [128]
+  uint64_t* bar = reinterpret_cast<uint64_t*>(factor + 128);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = tid & 127, half = tid >> 7;  // this thread's TMEM lane and half of the columns
+  const uint32_t rank = CLUSTER ? rank_in_cluster() : 0;
+  const int64_t tile = CLUSTER ? blockIdx.x / g.ranks : blockIdx.x;
+  const int in_tile = row / g.pitch, r = row - in_tile * g.pitch;  // matrix of the tile, row within it
+  const int64_t i = tile * g.per_cta + in_tile;
+  const bool live = in_tile < g.per_cta && r < g.s && i < g.batch;
+  const int c_first = int(rank) * g.cta_cols;     // first column of this CTA
+  const int cols = g.len - c_first < g.cta_cols ? (g.len - c_first > 0 ? g.len - c_first : 0)
+                                                : g.cta_cols;
+  const int tmem_cols = g.cta_cols <= 128 ? 128 : (g.cta_cols <= 256 ? 256 : 512);
+
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(uint32_t(tmem_cols))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  griddep_wait();
+  griddep_launch();
+
+  // ---- the norms: each thread sums half a row, a warp the rows of a matrix ----
+  const int my_cols = g.cta_cols / 2, c_begin = half * my_cols;
+  {
+    double sum = 0.0;
+    if (live)
+      for (int c = c_begin; c < c_begin + my_cols && c < cols; c += 8) {
+        float u[8];
+        const int count = cols - c < 8 ? cols - c : 8;
+        start8<MUON>(g, i, r, c_first + c, count, true, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < count) sum += double(u[j]) * double(u[j]);
+      }
+    row_sum[tid] = sum;
+  }
+  __syncthreads();
+  for (int m = warp; m < g.per_cta; m += kThreads / 32) {
+    double sum = 0.0;
+    for (int k = lane; k < g.s; k += 32) sum += row_sum[m * g.pitch + k] + row_sum[128 + m * g.pitch + k];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) mat_sum[m] = sum;
+  }
+  __syncthreads();
+  if (CLUSTER) sync_cluster();
+  if (tid < g.per_cta) {
+    double sum = 0.0;
+    if (CLUSTER)
+      for (int k = 0; k < g.ranks; ++k) sum += ld_remote_f64(remote(smem_u32(mat_sum + tid), k));
+    else
+      sum = mat_sum[tid];
+    // a matrix with a NaN or an infinity is worked on as zeros (its entries would reach the
+    // others of the tile) and written as NaN: marked by a factor that is not finite
+    factor[tid] = start_factor(sum, g.scale, g.eps);
+  }
+  __syncthreads();
+
+  // ---- X = scale * u / (norm + eps); zeros outside the matrices ----
+  {
+    float2 f = make_float2(0.f, 0.f);
+    if (live && isfinite(factor[in_tile].x)) f = factor[in_tile];
+    for (int c = c_begin; c < c_begin + my_cols; c += 8) {
+      float u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = 0.f;
+      if (f.x != 0.f && c < cols) {
+        const int count = cols - c < 8 ? cols - c : 8;
+        start8<MUON>(g, i, r, c_first + c, count, false, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = j < count ? start_scaled(u[j], f) : 0.f;
+      }
+      uint4 hi, lo;
+      round8v<SPLIT>(u, hi, lo);
+      const uint32_t at = chunk_at(row, c);
+      *reinterpret_cast<uint4*>(xs + at) = hi;
+      if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+  uint32_t phase = 0;
+  bool ok = true;
+  auto wait = [&]() {  // for the MMAs committed last
+    if (ok) ok = mbar_wait(bar, phase, status);
+    phase ^= 1;
+    tc_fence_after();
+  };
+  auto publish = [&]() {  // shared-memory writes before the next MMAs
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  const int k16 = (cols + 15) / 16;  // X's columns beyond `cols` are zero
+  const float inv = 1.f / g.scale;
+
+  for (int step = 0; step < g.steps; ++step) {
+    const float ca = g.coef[3 * step], cb = g.coef[3 * step + 1], cc = g.coef[3 * step + 2];
+    // ---- G = X X^T ----
+    if (tid == 0 && ok) {
+      const uint32_t id = idesc_half(128, 0);
+      uint32_t any = 0;
+#pragma unroll
+      for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // lo hi, hi lo, hi hi
+        const uint8_t* pa = xs + (t == 0 ? x_plane : 0);
+        const uint8_t* pb = xs + (t == 1 ? x_plane : 0);
+        for (int k = 0; k < k16; ++k) {
+          const uint64_t off = uint64_t((k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
+          mma_half(tmem, sw128_desc(pa) + off, sw128_desc(pb) + off, id, any);
+          any = 1;
+        }
+      }
+      if (!any)  // no columns here (a cluster longer than the matrix): zeros from zero columns
+        mma_half(tmem, sw128_desc(xs), sw128_desc(xs), id, 0);
+      mma_commit(bar);
+    }
+    wait();
+    // columns 64 * half .. + 63 of this thread's row; entries between matrices are dropped
+    if (!CLUSTER) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float v[32];
+        const int c0 = half * 64 + q * 32;
+        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = c0 + j + e;
+            y[e] = (c >= in_tile * g.pitch && c < (in_tile + 1) * g.pitch) ? v[j + e] * inv : 0.f;
+          }
+          uint4 hi, lo;
+          round8v<SPLIT>(y, hi, lo);
+          const uint32_t at = chunk_at(row, c0 + j);
+          *reinterpret_cast<uint4*>(gs + at) = hi;
+          if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float v[32];
+        const int c0 = half * 64 + q * 32;
+        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(es + (uint32_t((c0 + j) >> 2) * 128 + row) * 16) =
+              make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+      sync_cluster();
+      // this CTA's slice: 128 / ranks columns of every row; a thread sums 8 columns at a time
+      const int width = 128 / g.ranks;
+      for (int k = tid; k < 128 * (width / 8); k += kThreads) {
+        const int rr = k & 127, c0 = int(rank) * width + (k >> 7) * 8;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        for (int o = 0; o < g.ranks; ++o) {
+          const uint32_t at = remote(smem_u32(es + (uint32_t(c0 >> 2) * 128 + rr) * 16), o);
+          const float4 a = ld_remote4(at), b = ld_remote4(at + 2048);
+          y[0] += a.x, y[1] += a.y, y[2] += a.z, y[3] += a.w;
+          y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
+        }
+        const int mt = rr / g.pitch;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = c0 + e;
+          y[e] = (c >= mt * g.pitch && c < (mt + 1) * g.pitch) ? y[e] * inv : 0.f;
+        }
+        uint4 hi, lo;
+        round8v<SPLIT>(y, hi, lo);
+        const uint32_t at = smem_u32(gs) + chunk_at(rr, c0);
+        for (int o = 0; o < g.ranks; ++o) {
+          st_remote16(remote(at, o), hi);
+          if (SPLIT) st_remote16(remote(at + g_plane, o), lo);
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      sync_cluster();
+    }
+    publish();
+    // ---- B = b G + c G G ----
+    if (tid == 0 && ok) {
+      const uint32_t id = idesc_half(128, 0);
+#pragma unroll
+      for (int t = SPLIT ? 0 : 2; t < 3; ++t) {
+        const uint8_t* pa = gs + (t == 0 ? g_plane : 0);
+        const uint8_t* pb = gs + (t == 1 ? g_plane : 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t off = uint64_t((k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
+          mma_half(tmem, sw128_desc(pa) + off, sw128_desc(pb) + off, id,
+                   (k || t > (SPLIT ? 0 : 2)) ? 1u : 0u);
+        }
+      }
+      mma_commit(bar);
+    }
+    wait();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      float v[32];
+      const int c0 = half * 64 + q * 32;
+      tmem_ld32(tmem + lane_base + uint32_t(c0), v);
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = v[j + e] * (cc * inv);
+        const uint32_t at = chunk_at(row, c0 + j);
+        add8(y, *reinterpret_cast<const uint4*>(gs + at), cb);
+        if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), cb);
+        uint4 hi, lo;
+        round8v<SPLIT>(y, hi, lo);
+        *reinterpret_cast<uint4*>(gs + at) = hi;
+        if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+      }
+    }
+    publish();
+    // ---- X <- a X + B X ----
+    if (tid == 0 && ok) {
+      for (int n0 = 0; n0 < g.cta_cols; n0 += 256) {
+        const int n = g.cta_cols - n0 < 256 ? g.cta_cols - n0 : 256;
+        const uint32_t id = idesc_half(n, 1);
+#pragma unroll
+        for (int t = SPLIT ? 0 : 2; t < 3; ++t) {
+          const uint8_t* pa = gs + (t == 0 ? g_plane : 0);
+          const uint8_t* pb = xs + (t == 1 ? x_plane : 0) + (n0 >> 6) * kBlockBytes;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_half(tmem + uint32_t(n0),
+                     sw128_desc(pa) + (uint64_t((k >> 2) * kBlockBytes + (k & 3) * 32) >> 4),
+                     desc_cols(pb) + (uint64_t(k * 2048) >> 4), id,
+                     (k || t > (SPLIT ? 0 : 2)) ? 1u : 0u);
+        }
+      }
+      mma_commit(bar);
+    }
+    wait();
+    const bool last = step + 1 == g.steps;
+    const float f = last ? inv * inv : inv, fa = last ? ca * inv : ca;
+    for (int c0 = c_begin; c0 < c_begin + my_cols; c0 += 32) {
+      float v[32];
+      tmem_ld32(tmem + lane_base + uint32_t(c0), v);
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
+        const int c = c0 + j;
+        const uint32_t at = chunk_at(row, c);
+        add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
+        if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
+        if (!last) {
+          uint4 hi, lo;
+          round8v<SPLIT>(y, hi, lo);
+          *reinterpret_cast<uint4*>(xs + at) = hi;
+          if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
+        } else if (live && c < cols) {
+          const int count = cols - c < 8 ? cols - c : 8;
+          if (!isfinite(factor[in_tile].x)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fc00000);
+          }
+          if (MUON) {
+            float w[8];
+            load_tile8(g, g.out, i, r, c_first + c, count, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(-g.rate, y[e], g.decay * w[e]);
+          }
+          store_tile8(g, g.out, i, r, c_first + c, count, y);
+        }
+      }
+    }
+    publish();
+  }
+  if (CLUSTER) sync_cluster();  // no CTA leaves while another may read its shared memory
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(uint32_t(tmem_cols))
+                 : "memory");
+}
+
+// Columns one CTA can hold: X and G (both planes) and, in a cluster, the FP32 partial of G fit
+// the 227 KB of shared memory, and an accumulator of X the 512 columns of TMEM.
+constexpr int kMaxCols = 512, kMaxColsSplit = 192;
+constexpr int kMaxRanks = 8;
+constexpr int kMaxSmem = 227 * 1024;
+
+size_t smem_bytes(bool split, int ranks, int cta_cols) {
+  size_t b = size_t(split ? 2 : 1) * (size_t(cta_cols / 64) + 2) * kBlockBytes;
+  b += ranks > 1 ? 65536 : 256 * 8;
+  b += 128 * 8 + 128 * 8 + 16 + 1008;  // 1008: to a 1024-byte boundary from a 16-byte one
+  // CTAs of different clusters on one SM could wait for each other's TMEM: one CTA per SM
+  if (ranks > 1 && b < 118 * 1024) b = 118 * 1024;
+  return b;
+}
+
+template <bool SPLIT, bool MUON, bool CLUSTER>
+int launch(const SmallArgs& g, int64_t tiles, size_t smem, cudaStream_t q) {
+  chol::note_launch(q);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles * g.ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = q;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(g.ranks);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
+  return chol::status_from(
+      cudaLaunchKernelEx(&cfg, small_kernel<SPLIT, MUON, CLUSTER>, g, chol::device_status_ptr()));
+}
+
+Matrix device_side(const linalg_matrix* x) {
+  Matrix d{x->data, x->ld, x->stride, x->type, 0};
+  const int per16 = x->type == LINALG_FP32 ? 4 : 8;
+  d.vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->ld % per16 == 0 &&
+          x->stride % per16 == 0;
+  return d;
+}
+
+}  // namespace
+
+bool small_supported(int64_t m, int64_t n, bool split) {
+  const int64_t s = m < n ? m : n, len = m < n ? n : m;
+  return s <= 128 && len <= int64_t(kMaxRanks) * (split ? kMaxColsSplit : kMaxCols);
+}
+
+int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_matrix* out,
+                 int64_t batch, int64_t m, int64_t n, double beta, int nesterov, float decay,
+                 float rate, int steps, const float* coefficients, float eps, bool split,
+                 cudaStream_t q) {
+  SmallArgs g{};
+  g.x = device_side(x);
+  if (momentum != nullptr) g.momentum = device_side(momentum);
+  g.out = device_side(out);
+  g.tall = m > n;
+  g.s = int(g.tall ? n : m), g.len = int(g.tall ? m : n);
+  g.pitch = (g.s + 15) / 16 * 16;
+  g.per_cta = 128 / g.pitch;
+  if (g.per_cta > batch) g.per_cta = int(batch);
+  g.batch = batch;
+  const int most = split ? kMaxColsSplit : kMaxCols;
+  g.ranks = 1;
+  while (int64_t(g.ranks) * most < g.len) g.ranks *= 2;
+  const int64_t tiles = (batch + g.per_cta - 1) / g.per_cta;
+  const int chunk = (g.len + g.ranks - 1) / g.ranks;
+  g.cta_cols = (chunk + 63) / 64 * 64;
+  g.steps = steps;
+  g.beta = float(beta), g.gain = float(1.0 - beta), g.nesterov = nesterov;
+  g.decay = decay, g.rate = rate;
+  g.scale = split ? 4096.f : 1024.f, g.eps = eps;
+  for (int k = 0; k < 3 * steps; ++k) g.coef[k] = coefficients[k];
+  const size_t smem = smem_bytes(split, g.ranks, g.cta_cols);
+  if (tiles * g.ranks > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;
+  const bool muon = momentum != nullptr, cluster = g.ranks > 1;
+  if (split) {
+    if (muon) return cluster ? launch<true, true, true>(g, tiles, smem, q) : launch<true, true, false>(g, tiles, smem, q);
+    return cluster ? launch<true, false, true>(g, tiles, smem, q) : launch<true, false, false>(g, tiles, smem, q);
+  }
+  if (muon) return cluster ? launch<false, true, true>(g, tiles, smem, q) : launch<false, true, false>(g, tiles, smem, q);
+  return cluster ? launch<false, false, true>(g, tiles, smem, q) : launch<false, false, false>(g, tiles, smem, q);
+}
+
+template <bool SPLIT, bool MUON, bool CLUSTER>
+cudaError_t set_small() {
+  return cudaFuncSetAttribute(small_kernel<SPLIT, MUON, CLUSTER>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+}
+
+cudaError_t prepare_small_ortho() {
+  cudaError_t e;
+  if ((e = set_small<false, false, false>()) != cudaSuccess) return e;
+  if ((e = set_small<false, false, true>()) != cudaSuccess) return e;
+  if ((e = set_small<false, true, false>()) != cudaSuccess) return e;
+  if ((e = set_small<false, true, true>()) != cudaSuccess) return e;
+  if ((e = set_small<true, false, false>()) != cudaSuccess) return e;
+  if ((e = set_small<true, false, true>()) != cudaSuccess) return e;
+  if ((e = set_small<true, true, false>()) != cudaSuccess) return e;
+  return set_small<true, true, true>();
+}
+
+}  // namespace lin

@@ -30,6 +30,8 @@ def test_library_exports_and_binding():
 def test_workspace():
     f = _lib.load().linalg_orthogonalize_workspace
     assert f(0, 5, 5, 1) == 0 and f(2, 0, 5, 1) == 0 and f(2, 5, 0, 1) == 0
+    assert f(5, 128, 4096, 1) == 0 and f(5, 4096, 100, 1) == 0 and f(5, 129, 130, 1) > 0
+    assert f(5, 128, 1536, 2) == 0 and f(5, 128, 1537, 2) > 0
     # two X and two squares of fp16, twice that for full precision
     assert f(3, 512, 1024, 1) >= 3 * 2 * 2 * (512 * 1024 + 512 * 512)
     assert f(3, 512, 1024, 2) >= 2 * 3 * 2 * 2 * (512 * 1024 + 512 * 512)
@@ -66,14 +68,16 @@ def test_orthogonalize_refusals_of_the_c_entry():
     assert _orth(x=_m(stride=100), batch=2) == BAD
     assert _orth(out=_m(1 << 20, stride=0), batch=2) == BAD
     assert _orth(out=_m(4096 + 128)) == BAD  # overlaps x by all but a row
-    assert _orth(ws=0) == SPACE and _orth(ws=4096 + 16) == SPACE and _orth(size=100) == SPACE
+    big = dict(x=_m(ld=300), out=_m(1 << 20, ld=300), m=200, n=300)  # needs a workspace
+    assert _orth(**big, ws=0) == SPACE and _orth(**big, ws=4096 + 16) == SPACE
+    assert _orth(**big, size=100) == SPACE
     assert _orth(x=_m(ld=1 << 25), out=_m(1 << 40, ld=1 << 25), n=1 << 25) == TOO_BIG
 
 
-def _muon(param=None, grad=None, momentum=None, beta=0.9, decay=1.0, rate=0.1, batch=1, steps=1):
+def _muon(param=None, grad=None, momentum=None, beta=0.9, decay=1.0, rate=0.1, batch=1, steps=1, m=64):
     return _lib.load().linalg_muon_update(
         ctypes.byref(param or _m(1 << 20)), ctypes.byref(grad or _m(1 << 22)),
-        ctypes.byref(momentum or _m(1 << 24, kind=2)), batch, 64, 64, beta, 1, decay, rate, steps,
+        ctypes.byref(momentum or _m(1 << 24, kind=2)), batch, m, m, beta, 1, decay, rate, steps,
         _floats(3.0, -3.0, 1.0), 0.0, 1, ctypes.c_void_p(4096), 100, None)
 
 
@@ -85,7 +89,8 @@ def test_muon_refusals_of_the_c_entry():
     assert _muon(grad=_m(1 << 20)) == BAD  # the parameter's own memory
     assert _muon(momentum=_m((1 << 22) + 64)) == BAD
     assert _muon(param=_m(1 << 20, stride=0), batch=2) == BAD
-    assert _muon() == SPACE
+    wide = [_m(1 << k, ld=200) for k in (20, 22)]
+    assert _muon(wide[0], wide[1], _m(1 << 24, ld=200, kind=2), m=200) == SPACE
 
 
 def _mul(x=None, w=None, y=None, off=4096, off64=0, groups=2, rows=10, k=64, n=64, fill=1):
@@ -126,9 +131,9 @@ def test_binding_checks_its_arguments():
         lib.orthogonalize(*range(16), 0.0, 5)  # not a buffer
     # a coefficient buffer shorter than the steps is refused, not read past its end
     short = bytes(4 * 3)
-    x, out = (4096, 64, 4096, 0), (1 << 20, 64, 4096, 0)
-    assert lib.orthogonalize(*x, *out, 1, 64, 64, 2, 1, 4096, 0, 0, 0.0, short) == BAD
-    assert lib.orthogonalize(*x, *out, 1, 64, 64, 1, 1, 4096, 0, 0, 0.0, short) == SPACE
+    x, out = (4096, 200, 4096, 0), (1 << 20, 200, 4096, 0)
+    assert lib.orthogonalize(*x, *out, 1, 200, 200, 2, 1, 4096, 0, 0, 0.0, short) == BAD
+    assert lib.orthogonalize(*x, *out, 1, 200, 200, 1, 1, 4096, 0, 0, 0.0, short) == SPACE
 
 
 def test_wrappers_refuse_what_has_no_gpu_path():

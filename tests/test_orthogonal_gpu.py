@@ -65,7 +65,11 @@ def _tolerance(x, dtype, half, **kw):
 
 SHAPES = [(1, 128, 128), (3, 64, 64), (2, 256, 256), (1, 512, 512), (2, 200, 328), (2, 328, 200),
           (1, 1000, 601), (1, 601, 1000), (5, 33, 17), (5, 17, 33), (2, 1, 40), (2, 40, 1),
-          (3, 1, 1), (1, 2048, 130), (1, 130, 2048), (4, 65, 1025), (300, 16, 24), (1, 768, 1536)]
+          (3, 1, 1), (1, 2048, 130), (1, 130, 2048), (4, 65, 1025), (300, 16, 24), (1, 768, 1536),
+          # on chip: one matrix or several per tile, split over 2, 4 and 8 CTAs, odd sizes
+          (1, 128, 512), (2, 128, 513), (1, 100, 700), (2, 700, 100), (1, 90, 1537), (1, 4096, 128),
+          (1, 127, 4096), (5, 1, 3000), (6, 43, 64), (9, 31, 1), (7, 64, 129), (130, 1, 5),
+          (3, 1536, 20)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -118,9 +122,10 @@ def test_magnitudes(magnitude):
     assert _far(got, exact) <= tol
 
 
-@pytest.mark.parametrize("m,n", [(48, 80), (128, 128), (300, 260)])
+@pytest.mark.parametrize("m,n", [(48, 80), (10, 30), (30, 10), (128, 128), (60, 900), (300, 260)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_zero_and_non_finite_matrices(m, n, dtype):
+    """(Matrices of 48 x 80 and 10 x 30 share a tile.)"""
     x = _input(3, (5, m, n), dtype)
     x[1] = 0
     x[2, 5, 7] = float("nan")
@@ -207,6 +212,19 @@ def test_muon_update(shape, types, nesterov):
     allowed = (torch.finfo(pt).eps / 2 + 3 * 2.0 ** -24) * want.square().sum((-2, -1)).sqrt() + \
         lr * scale * tol * o.square().sum((-2, -1)).sqrt()
     assert (off <= allowed).all(), (off, allowed)
+
+
+@pytest.mark.parametrize("m,n", [(6, 8), (40, 30), (150, 140)])
+def test_smallest_and_largest_norms(m, n):
+    """FP32 subnormals and values whose squares pass FP32's range."""
+    base = _input(6, (3, m, n))
+    want = orthogonalize(base, eps=0.0)
+    for power in (-146 if m < 100 else -140, 120):
+        x = torch.ldexp(base.double(), torch.tensor(float(power), device=DEV)).float()
+        exact, tol = _tolerance(x.double() * 2.0 ** -power, torch.float32, False, eps=0.0)
+        assert _far(orthogonalize(x, eps=0.0), exact) <= tol
+    assert want.isfinite().all()
+    assert orthogonalize(torch.zeros_like(base)).eq(0).all()
 
 
 def test_muon_layouts_and_scale():
