@@ -8,8 +8,8 @@
 //
 // X lives in shared memory as 128-byte-swizzled K-major blocks of 64 columns; the same bytes are
 // the MN-major B operand of B X (the summed index is then X's row). G and B share one buffer: an
-// epilogue thread overwrites the elements it has read. Accumulators in TMEM, one thread per row
-// and half of the columns.
+// epilogue thread overwrites the elements it has read. Accumulators in TMEM, a thread per row
+// and share of the columns.
 //
 //   per step:  G = X X^T -> mask, fp16   |   B = b G + c G G -> fp16   |   X <- a X + B X
 //
@@ -36,7 +36,6 @@ using namespace chol::tcx;
 using chol::fence_proxy_async_smem;
 using chol::smem_u32;
 
-constexpr int kThreads = 256;
 constexpr int kBlockBytes = 128 * 128;  // 128 rows x 64 fp16 columns
 
 struct SmallArgs {
@@ -117,56 +116,6 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return uint32_t(c >> 6) * kBlockBytes + uint32_t(r) * 128 + ((uint32_t(c >> 3) & 7) ^ (r & 7)) * 16;
 }
 
-// Elements (row r of the tile, columns c .. c + 7) of a caller's matrix; the tile's row of matrix i
-// is `r`, in the caller's orientation a column when tall.
-__device__ __forceinline__ void load_tile8(const SmallArgs& g, const Matrix& x, int64_t i, int r,
-                                           int c, int count, float (&v)[8]) {
-  if (!g.tall) {
-    load_any(x, i * x.stride + int64_t(r) * x.ld + c, v, count);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float one[8];
-      v[j] = 0.f;
-      if (j < count) {
-        load_any(x, i * x.stride + int64_t(c + j) * x.ld + r, one, 1);
-        v[j] = one[0];
-      }
-    }
-  }
-}
-__device__ __forceinline__ void store_tile8(const SmallArgs& g, const Matrix& x, int64_t i, int r,
-                                            int c, int count, float (&v)[8]) {
-  if (!g.tall) {
-    store_any(x, i * x.stride + int64_t(r) * x.ld + c, v, count);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) {
-        float one[8] = {v[j]};
-        store_any(x, i * x.stride + int64_t(c + j) * x.ld + r, one, 1);
-        v[j] = one[0];
-      }
-  }
-}
-
-template <bool MUON>
-__device__ __forceinline__ void start8(const SmallArgs& g, int64_t i, int r, int c, int count,
-                                       bool update, float (&u)[8]) {
-  load_tile8(g, g.x, i, r, c, count, u);
-  if (MUON) {
-    float mo[8];
-    load_tile8(g, g.momentum, i, r, c, count, mo);
-    if (update) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mo[j] = fmaf(g.beta, mo[j], g.gain * u[j]);
-      store_tile8(g, g.momentum, i, r, c, count, mo);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = g.nesterov ? fmaf(g.beta, mo[j], g.gain * u[j]) : mo[j];
-  }
-}
-
 // Eight values to fp16 (and the remainder plane): shared-memory chunks of 16 bytes. Saturating: an
 // infinity in one matrix would reach the others of its tile as 0 * inf in B X. (Only
 // coefficients with which the iteration diverges get there: 65504 is 16 times the
@@ -196,29 +145,96 @@ __device__ __forceinline__ void add8(float (&v)[8], uint4 w, float f) {
   for (int j = 0; j < 8; ++j) v[j] = fmaf(f, __half2float(h[j]), v[j]);
 }
 
-template <bool SPLIT, bool MUON, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int* status) {
+// The input (and momentum) of one matrix's share of this CTA, in the caller's order: `WARPS`
+// warps walk chunks of eight of its columns, four in flight per thread. body(row, column, count,
+// u) gets the iteration's start value; row and column count from the share's first element.
+template <bool MUON, bool UPDATE, typename Body>
+__device__ __forceinline__ void walk_input(const SmallArgs& g, int64_t i, int c_first, int cols,
+                                           int worker, int workers, const Body& body) {
+  const int rows = g.tall ? cols : g.s, width = g.tall ? g.s : cols;
+  const int row0 = g.tall ? c_first : 0, col0 = g.tall ? 0 : c_first;
+  // a wide matrix's row goes to one row of X: consecutive lanes take consecutive chunks. A tall
+  // one's row is scattered over X's rows (two bytes each): 8 rows x 4 chunks per warp, which
+  // trades 64-byte reads for 4-way instead of 16-way bank conflicts
+  const int per_row = (width + 7) / 8;
+  const int cw = g.tall ? 4 : 1;
+  const int strips = (per_row + cw - 1) / cw;
+  const int total = g.tall ? (rows + 7) / 8 * strips * 32 : rows * per_row;
+  constexpr int U = 4;
+  for (int k0 = worker; k0 < total; k0 += U * workers) {
+    Raw8 x[U], mo[U];
+    int rr[U], cc[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int k = k0 + q * workers;
+      if (g.tall) {
+        const int t = k >> 5, l = k & 31;
+        rr[q] = (t / strips) * 8 + (l & 7);
+        cc[q] = ((t % strips) * 4 + (l >> 3)) * 8;
+      } else {
+        rr[q] = k / per_row;
+        cc[q] = (k - rr[q] * per_row) * 8;
+      }
+      if (k >= total || rr[q] >= rows || cc[q] >= width) rr[q] = -1;
+      if (rr[q] >= 0) {
+        const int count = width - cc[q] < 8 ? width - cc[q] : 8;
+        load_raw(g.x, i * g.x.stride + int64_t(row0 + rr[q]) * g.x.ld + col0 + cc[q], count, x[q]);
+        if (MUON)
+          load_raw(g.momentum,
+                   i * g.momentum.stride + int64_t(row0 + rr[q]) * g.momentum.ld + col0 + cc[q],
+                   count, mo[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      if (rr[q] < 0) continue;
+      const int count = width - cc[q] < 8 ? width - cc[q] : 8;
+      float u[8];
+      convert_raw(x[q], g.x.type, u);
+      if (MUON) {
+        float m[8];
+        convert_raw(mo[q], g.momentum.type, m);
+        if (UPDATE) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m[j] = fmaf(g.beta, m[j], g.gain * u[j]);
+          store_any(g.momentum,
+                    i * g.momentum.stride + int64_t(row0 + rr[q]) * g.momentum.ld + col0 + cc[q],
+                    m, count);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = g.nesterov ? fmaf(g.beta, m[j], g.gain * u[j]) : m[j];
+      }
+      body(rr[q], cc[q], count, u);
+    }
+  }
+}
+
+template <int T, bool SPLIT, bool MUON, bool CLUSTER>
+__global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
+    small_kernel(const SmallArgs g, int* status) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   constexpr int P = SPLIT ? 2 : 1;
+  constexpr int PARTS = T / 128;       // threads per row of the tile
+  constexpr int GCOLS = 128 / PARTS;   // columns of G per thread
   const int blocks = g.cta_cols / 64;
   const uint32_t x_plane = uint32_t(blocks) * kBlockBytes;
   uint8_t* xs = smem;                            // [P] X: blocks of 64 columns
   uint8_t* gs = xs + P * x_plane;                // [P] G, then B: two blocks
   constexpr uint32_t g_plane = 2 * kBlockBytes;
   uint8_t* es = gs + P * g_plane;                // CLUSTER: FP32 partial of G, [column / 4][row] x 4
-  double* row_sum = reinterpret_cast<double*>(es);  // [2][128] (CLUSTER: before es is used)
-  double* mat_sum = reinterpret_cast<double*>(es + (CLUSTER ? 65536 : 2048));  // [128] per matrix
-  float2* factor = reinterpret_cast<float2*>(mat_sum + 128);  // [128]
-  uint64_t* bar = reinterpret_cast<uint64_t*>(factor + 128);
+  double* warp_sum = reinterpret_cast<double*>(es);  // [T / 32] (CLUSTER: before es is used)
+  double* mat_sum = reinterpret_cast<double*>(es + (CLUSTER ? 65536 : 128));  // [8] per matrix
+  float2* factor = reinterpret_cast<float2*>(mat_sum + 8);  // [8]
+  uint64_t* bar = reinterpret_cast<uint64_t*>(factor + 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = tid & 127, half = tid >> 7;  // this thread's TMEM lane and half of the columns
+  const int row = tid & 127, part = tid >> 7;  // this thread's TMEM lane and share of the columns
   const uint32_t rank = CLUSTER ? rank_in_cluster() : 0;
   const int64_t tile = CLUSTER ? blockIdx.x / g.ranks : blockIdx.x;
-  const int in_tile = row / g.pitch, r = row - in_tile * g.pitch;  // matrix of the tile, row within it
+  const int in_tile = row / g.pitch, r = row - in_tile * g.pitch;  // matrix, row within it
   const int64_t i = tile * g.per_cta + in_tile;
   const bool live = in_tile < g.per_cta && r < g.s && i < g.batch;
   const int c_first = int(rank) * g.cta_cols;     // first column of this CTA
@@ -237,66 +253,78 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // zeros in X's padding: rows between and behind the matrices, columns behind the last
+  if (g.per_cta * g.pitch < 128 || g.s < g.pitch || cols < g.cta_cols ||
+      (tile + 1) * g.per_cta > g.batch)
+    for (uint32_t k = tid * 16; k < P * x_plane; k += T * 16)
+      *reinterpret_cast<uint4*>(xs + k) = make_uint4(0, 0, 0, 0);
   griddep_wait();
   griddep_launch();
 
-  // ---- the norms: each thread sums half a row, a warp the rows of a matrix ----
-  const int my_cols = g.cta_cols / 2, c_begin = half * my_cols;
-  {
-    double sum = 0.0;
-    if (live)
-      for (int c = c_begin; c < c_begin + my_cols && c < cols; c += 8) {
-        float u[8];
-        const int count = cols - c < 8 ? cols - c : 8;
-        start8<MUON>(g, i, r, c_first + c, count, true, u);
+  // ---- the norms. Each matrix of the tile has its own warps. ----
+  const int team = (T / 32) / g.per_cta;  // warps per matrix (per_cta <= 8)
+  const int mine = warp / team;           // matrix of the tile this warp reads
+  const int64_t im = tile * g.per_cta + mine;
+  const bool reads = mine < g.per_cta && im < g.batch;
+  const int worker = tid - mine * team * 32, workers = team * 32;
+  double sum = 0.0;
+  if (reads)
+    walk_input<MUON, true>(g, im, c_first, cols, worker, workers,
+                           [&](int, int, int count, const float (&u)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < count) sum += double(u[j]) * double(u[j]);
-      }
-    row_sum[tid] = sum;
-  }
-  __syncthreads();
-  for (int m = warp; m < g.per_cta; m += kThreads / 32) {
-    double sum = 0.0;
-    for (int k = lane; k < g.s; k += 32) sum += row_sum[m * g.pitch + k] + row_sum[128 + m * g.pitch + k];
+                             for (int j = 0; j < 8; ++j)
+                               if (j < count) sum += double(u[j]) * double(u[j]);
+                           });
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) mat_sum[m] = sum;
-  }
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) warp_sum[warp] = sum;
   __syncthreads();
+  if (tid < g.per_cta) {
+    double total = 0.0;
+    for (int k = 0; k < team; ++k) total += warp_sum[tid * team + k];
+    mat_sum[tid] = total;
+  }
   if (CLUSTER) sync_cluster();
   if (tid < g.per_cta) {
-    double sum = 0.0;
-    if (CLUSTER)
-      for (int k = 0; k < g.ranks; ++k) sum += ld_remote_f64(remote(smem_u32(mat_sum + tid), k));
-    else
-      sum = mat_sum[tid];
+    double total = mat_sum[tid];
+    if (CLUSTER) {
+      total = 0.0;
+      for (int k = 0; k < g.ranks; ++k) total += ld_remote_f64(remote(smem_u32(mat_sum + tid), k));
+    }
     // a matrix with a NaN or an infinity is worked on as zeros (its entries would reach the
     // others of the tile) and written as NaN: marked by a factor that is not finite
-    factor[tid] = start_factor(sum, g.scale, g.eps);
+    factor[tid] = start_factor(total, g.scale, g.eps);
   }
   __syncthreads();
 
-  // ---- X = scale * u / (norm + eps); zeros outside the matrices ----
-  {
-    float2 f = make_float2(0.f, 0.f);
-    if (live && isfinite(factor[in_tile].x)) f = factor[in_tile];
-    for (int c = c_begin; c < c_begin + my_cols; c += 8) {
-      float u[8];
+  // ---- X = scale * u / (norm + eps) ----
+  if (reads) {
+    const float2 f = factor[mine];
+    const bool finite = isfinite(f.x);
+    const int base = mine * g.pitch;
+    walk_input<MUON, false>(g, im, c_first, cols, worker, workers,
+                            [&](int rr, int cc, int count, const float (&u)[8]) {
+      float y[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = 0.f;
-      if (f.x != 0.f && c < cols) {
-        const int count = cols - c < 8 ? cols - c : 8;
-        start8<MUON>(g, i, r, c_first + c, count, false, u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = j < count ? start_scaled(u[j], f) : 0.f;
-      }
+      for (int j = 0; j < 8; ++j) y[j] = finite && j < count ? start_scaled(u[j], f) : 0.f;
       uint4 hi, lo;
-      round8v<SPLIT>(u, hi, lo);
-      const uint32_t at = chunk_at(row, c);
-      *reinterpret_cast<uint4*>(xs + at) = hi;
-      if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
-    }
+      round8v<SPLIT>(y, hi, lo);
+      if (!g.tall) {
+        const uint32_t at = chunk_at(base + rr, cc);
+        *reinterpret_cast<uint4*>(xs + at) = hi;
+        if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
+      } else {
+        const __half* h = reinterpret_cast<const __half*>(&hi);
+        const __half* l = reinterpret_cast<const __half*>(&lo);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= count) break;
+          const uint32_t at = chunk_at(base + cc + j, rr) + (rr & 7) * 2;
+          *reinterpret_cast<__half*>(xs + at) = h[j];
+          if (SPLIT) *reinterpret_cast<__half*>(xs + x_plane + at) = l[j];
+        }
+      }
+    });
   }
   fence_proxy_async_smem();
   tc_fence_before();
@@ -344,18 +372,17 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
     // columns 64 * half .. + 63 of this thread's row; entries between matrices are dropped
     if (!CLUSTER) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < GCOLS / 32; ++q) {
         float v[32];
-        const int c0 = half * 64 + q * 32;
+        const int c0 = part * GCOLS + q * 32;
         tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
+          // 8 columns are of one matrix: the pitch is a multiple of 16
+          const float f = uint32_t(c0 + j - in_tile * g.pitch) < uint32_t(g.pitch) ? inv : 0.f;
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = c0 + j + e;
-            y[e] = (c >= in_tile * g.pitch && c < (in_tile + 1) * g.pitch) ? v[j + e] * inv : 0.f;
-          }
+          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
           uint4 hi, lo;
           round8v<SPLIT>(y, hi, lo);
           const uint32_t at = chunk_at(row, c0 + j);
@@ -365,9 +392,9 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
       }
     } else {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < GCOLS / 32; ++q) {
         float v[32];
-        const int c0 = half * 64 + q * 32;
+        const int c0 = part * GCOLS + q * 32;
         tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
         for (int j = 0; j < 32; j += 4)
@@ -377,7 +404,7 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
       sync_cluster();
       // this CTA's slice: 128 / ranks columns of every row; a thread sums 8 columns at a time
       const int width = 128 / g.ranks;
-      for (int k = tid; k < 128 * (width / 8); k += kThreads) {
+      for (int k = tid; k < 128 * (width / 8); k += T) {
         const int rr = k & 127, c0 = int(rank) * width + (k >> 7) * 8;
         float y[8];
 #pragma unroll
@@ -389,11 +416,9 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
           y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
         }
         const int mt = rr / g.pitch;
+        const float f = uint32_t(c0 - mt * g.pitch) < uint32_t(g.pitch) ? inv : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int c = c0 + e;
-          y[e] = (c >= mt * g.pitch && c < (mt + 1) * g.pitch) ? y[e] * inv : 0.f;
-        }
+        for (int e = 0; e < 8; ++e) y[e] *= f;
         uint4 hi, lo;
         round8v<SPLIT>(y, hi, lo);
         const uint32_t at = smem_u32(gs) + chunk_at(rr, c0);
@@ -424,9 +449,9 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
     }
     wait();
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < GCOLS / 32; ++q) {
       float v[32];
-      const int c0 = half * 64 + q * 32;
+      const int c0 = part * GCOLS + q * 32;
       tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
       for (int j = 0; j < 32; j += 8) {
@@ -465,7 +490,26 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
     wait();
     const bool last = step + 1 == g.steps;
     const float f = last ? inv * inv : inv, fa = last ? ca * inv : ca;
-    for (int c0 = c_begin; c0 < c_begin + my_cols; c0 += 32) {
+    for (int c0 = part * 32; c0 < g.cta_cols; c0 += PARTS * 32) {
+      // the weights of the last step, ahead of their use
+      Raw8 w[MUON ? 4 : 1];
+      uint32_t wt[MUON ? 32 : 1];
+      const int64_t at_row = g.tall ? i * g.out.stride + int64_t(c_first) * g.out.ld + r
+                                    : i * g.out.stride + int64_t(r) * g.out.ld + c_first;
+      if (MUON && last && live) {
+        if (g.tall) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < cols) wt[MUON ? j : 0] = load_one(g.out, at_row + int64_t(c0 + j) * g.out.ld);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 8 * j;
+            if (c < cols)
+              load_raw(g.out, at_row + c, cols - c < 8 ? cols - c : 8, w[MUON ? j : 0]);
+          }
+        }
+      }
       float v[32];
       tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
@@ -489,12 +533,23 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const SmallArgs g, int*
             for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fc00000);
           }
           if (MUON) {
-            float w[8];
-            load_tile8(g, g.out, i, r, c_first + c, count, w);
+            float old[8];
+            if (g.tall) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = fmaf(-g.rate, y[e], g.decay * w[e]);
+              for (int e = 0; e < 8; ++e) old[e] = bits_to_float(wt[MUON ? j + e : 0], g.out.type);
+            } else {
+              convert_raw(w[MUON ? j / 8 : 0], g.out.type, old);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(-g.rate, y[e], g.decay * old[e]);
           }
-          store_tile8(g, g.out, i, r, c_first + c, count, y);
+          if (g.tall) {  // a warp's lanes are consecutive columns of the caller's row
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e < count) store_one(g.out, at_row + int64_t(c + e) * g.out.ld, y[e]);
+          } else {
+            store_any(g.out, at_row + c, y, count);
+          }
         }
       }
     }
@@ -515,19 +570,19 @@ constexpr int kMaxSmem = 227 * 1024;
 
 size_t smem_bytes(bool split, int ranks, int cta_cols) {
   size_t b = size_t(split ? 2 : 1) * (size_t(cta_cols / 64) + 2) * kBlockBytes;
-  b += ranks > 1 ? 65536 : 256 * 8;
-  b += 128 * 8 + 128 * 8 + 16 + 1008;  // 1008: to a 1024-byte boundary from a 16-byte one
+  b += ranks > 1 ? 65536 : 128;
+  b += 8 * 8 + 8 * 8 + 16 + 1008;  // 1008: to a 1024-byte boundary from a 16-byte one
   // CTAs of different clusters on one SM could wait for each other's TMEM: one CTA per SM
   if (ranks > 1 && b < 118 * 1024) b = 118 * 1024;
   return b;
 }
 
-template <bool SPLIT, bool MUON, bool CLUSTER>
+template <int T, bool SPLIT, bool MUON, bool CLUSTER>
 int launch(const SmallArgs& g, int64_t tiles, size_t smem, cudaStream_t q) {
   chol::note_launch(q);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles * g.ranks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(T);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = q;
   cudaLaunchAttribute attr[2];
@@ -540,7 +595,7 @@ int launch(const SmallArgs& g, int64_t tiles, size_t smem, cudaStream_t q) {
   cfg.attrs = attr;
   cfg.numAttrs = CLUSTER ? 2 : 1;
   return chol::status_from(
-      cudaLaunchKernelEx(&cfg, small_kernel<SPLIT, MUON, CLUSTER>, g, chol::device_status_ptr()));
+      cudaLaunchKernelEx(&cfg, small_kernel<T, SPLIT, MUON, CLUSTER>, g, chol::device_status_ptr()));
 }
 
 Matrix device_side(const linalg_matrix* x) {
@@ -552,6 +607,16 @@ Matrix device_side(const linalg_matrix* x) {
 }
 
 }  // namespace
+
+#define LIN_FOR_EACH_SMALL(F) \
+  F(false, false, false)      \
+  F(false, false, true)       \
+  F(false, true, false)       \
+  F(false, true, true)        \
+  F(true, false, false)       \
+  F(true, false, true)        \
+  F(true, true, false)        \
+  F(true, true, true)
 
 bool small_supported(int64_t m, int64_t n, bool split) {
   const int64_t s = m < n ? m : n, len = m < n ? n : m;
@@ -586,30 +651,32 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
   const size_t smem = smem_bytes(split, g.ranks, g.cta_cols);
   if (tiles * g.ranks > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;
   const bool muon = momentum != nullptr, cluster = g.ranks > 1;
-  if (split) {
-    if (muon) return cluster ? launch<true, true, true>(g, tiles, smem, q) : launch<true, true, false>(g, tiles, smem, q);
-    return cluster ? launch<true, false, true>(g, tiles, smem, q) : launch<true, false, false>(g, tiles, smem, q);
-  }
-  if (muon) return cluster ? launch<false, true, true>(g, tiles, smem, q) : launch<false, true, false>(g, tiles, smem, q);
-  return cluster ? launch<false, false, true>(g, tiles, smem, q) : launch<false, false, false>(g, tiles, smem, q);
+  // 512 threads shorten the epilogues of a lone tile per SM; 256 leave registers for four tiles
+  const bool wide = cluster || split || tiles <= sm_count();
+#define LIN_SMALL(SPLIT, MUON, CLUSTER)                                      \
+  if (split == SPLIT && muon == MUON && cluster == CLUSTER)                  \
+    return wide ? launch<512, SPLIT, MUON, CLUSTER>(g, tiles, smem, q)       \
+                : launch<SPLIT || CLUSTER ? 512 : 256, SPLIT, MUON, CLUSTER>(g, tiles, smem, q);
+  LIN_FOR_EACH_SMALL(LIN_SMALL)
+#undef LIN_SMALL
+  return CHOL_ERR_UNSUPPORTED;
 }
 
-template <bool SPLIT, bool MUON, bool CLUSTER>
+template <int T, bool SPLIT, bool MUON, bool CLUSTER>
 cudaError_t set_small() {
-  return cudaFuncSetAttribute(small_kernel<SPLIT, MUON, CLUSTER>,
+  return cudaFuncSetAttribute(small_kernel<T, SPLIT, MUON, CLUSTER>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
 }
 
 cudaError_t prepare_small_ortho() {
   cudaError_t e;
-  if ((e = set_small<false, false, false>()) != cudaSuccess) return e;
-  if ((e = set_small<false, false, true>()) != cudaSuccess) return e;
-  if ((e = set_small<false, true, false>()) != cudaSuccess) return e;
-  if ((e = set_small<false, true, true>()) != cudaSuccess) return e;
-  if ((e = set_small<true, false, false>()) != cudaSuccess) return e;
-  if ((e = set_small<true, false, true>()) != cudaSuccess) return e;
-  if ((e = set_small<true, true, false>()) != cudaSuccess) return e;
-  return set_small<true, true, true>();
+#define LIN_SMALL(SPLIT, MUON, CLUSTER)                                                    \
+  if ((e = set_small<512, SPLIT, MUON, CLUSTER>()) != cudaSuccess) return e;               \
+  if ((e = set_small<SPLIT || CLUSTER ? 512 : 256, SPLIT, MUON, CLUSTER>()) != cudaSuccess) \
+    return e;
+  LIN_FOR_EACH_SMALL(LIN_SMALL)
+#undef LIN_SMALL
+  return cudaSuccess;
 }
 
 }  // namespace lin
