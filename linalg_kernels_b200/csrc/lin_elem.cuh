@@ -62,71 +62,50 @@ __device__ __forceinline__ void store_any(const Matrix& x, int64_t at, float (&v
     store8t(static_cast<float*>(x.data) + at, v, count, x.vec);
 }
 
+__device__ __forceinline__ float load_one(const Matrix& x, int64_t at) {
+  if (x.type == LINALG_FP32) return static_cast<const float*>(x.data)[at];
+  if (x.type == LINALG_BF16) return to_float(static_cast<const __nv_bfloat16*>(x.data)[at]);
+  return to_float(static_cast<const __half*>(x.data)[at]);
+}
+
 // Eight columns as loaded: the conversion comes later, so that several loads are in flight at a
-// time (a load is waited for where its register is used).
-struct Raw8 {
-  uint32_t w[8];  // 16-bit types: four words
+// time. `T` an element type: whole aligned chunks; `Any`: a matrix of any type, alignment and
+// number of columns.
+struct Any {};
+template <typename T>
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const Matrix& x, int64_t at, int) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(x.data) + at);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = p[i];
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const T* h = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
+  }
+  // v: as rounded to the array's type on return
+  static __device__ __forceinline__ void put(const Matrix& x, int64_t at, float (&v)[8], int) {
+    store8t(static_cast<T*>(x.data) + at, v, 8, true);
+  }
 };
-__device__ __forceinline__ void load_raw(const Matrix& x, int64_t at, int count, Raw8& r) {
-  if (x.vec && count == 8) {
-    const uint4* p = x.type == LINALG_FP32
-                         ? reinterpret_cast<const uint4*>(static_cast<const float*>(x.data) + at)
-                         : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x.data) + at);
-    const uint4 a = p[0];
-    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
-    if (x.type == LINALG_FP32) {
-      const uint4 b = p[1];
-      r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
-    }
-  } else if (x.type == LINALG_FP32) {
+template <>
+struct Eight<Any> {
+  float w[8];
+  __device__ __forceinline__ void load(const Matrix& x, int64_t at, int count) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      r.w[j] = j < count ? static_cast<const uint32_t*>(x.data)[at + j] : 0u;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint16_t* p = static_cast<const uint16_t*>(x.data) + at + 2 * j;
-      const uint32_t lo = 2 * j < count ? p[0] : 0, hi = 2 * j + 1 < count ? p[1] : 0;
-      r.w[j] = lo | (hi << 16);
-    }
+    for (int j = 0; j < 8; ++j) w[j] = j < count ? load_one(x, at + j) : 0.f;
   }
-}
-__device__ __forceinline__ float bits_to_float(uint32_t w, int type) {  // one element, low bits
-  if (type == LINALG_FP32) return __uint_as_float(w);
-  if (type == LINALG_BF16) return __uint_as_float(w << 16);
-  return __half2float(__ushort_as_half(uint16_t(w)));
-}
-__device__ __forceinline__ void convert_raw(const Raw8& r, int type, float (&v)[8]) {
-  if (type == LINALG_FP32) {
+  __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r.w[j]);
-  } else if (type == LINALG_BF16) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(r.w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(r.w[j] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __half2 h = *reinterpret_cast<const __half2*>(&r.w[j]);
-      v[2 * j] = __low2float(h);
-      v[2 * j + 1] = __high2float(h);
-    }
+    for (int j = 0; j < 8; ++j) v[j] = w[j];
   }
-}
-__device__ __forceinline__ uint32_t load_one(const Matrix& x, int64_t at) {
-  return x.type == LINALG_FP32 ? static_cast<const uint32_t*>(x.data)[at]
-                               : uint32_t(static_cast<const uint16_t*>(x.data)[at]);
-}
-__device__ __forceinline__ void store_one(const Matrix& x, int64_t at, float v) {
-  if (x.type == LINALG_FP32)
-    static_cast<float*>(x.data)[at] = v;
-  else if (x.type == LINALG_BF16)
-    static_cast<__nv_bfloat16*>(x.data)[at] = __float2bfloat16_rn(v);
-  else
-    static_cast<__half*>(x.data)[at] = __float2half_rn(v);
-}
+  static __device__ __forceinline__ void put(const Matrix& x, int64_t at, float (&v)[8],
+                                             int count) {
+    store_any(x, at, v, count);
+  }
+};
 
 // The factor F of X = F * u, F = scale / (norm + eps), as a power of two near its square root (x)
 // times the rest (y): F alone passes FP32's range for norms of subnormals and for the largest

@@ -14,8 +14,8 @@
 //   per step:  G = X X^T -> mask, fp16   |   B = b G + c G G -> fp16   |   X <- a X + B X
 //
 // A long matrix is split over a cluster of 2, 4 or 8 CTAs by columns. Only G needs all columns:
-// each CTA puts its FP32 partial into shared memory, sums one slice of G over the CTAs in rank
-// order (the same bits every time) and writes the rounded slice to all of them.
+// each CTA writes its FP32 partials to the CTAs that own their columns, which sum them in rank
+// order (the same bits every time) and write the rounded slice to all.
 //
 // `SPLIT`: two fp16 planes per operand and three products, as in lin_gemm.cu. One accumulator
 // covers at most 192 columns of K, so it needs no drain.
@@ -50,6 +50,9 @@ struct SmallArgs {
   int ranks;         // CTAs per cluster
   int steps;
   int nesterov;
+  int in_path, out_path;  // 0: any types and alignment; else whole aligned chunks of these types:
+                          // in 1 bf16 (momentum fp32), 2 fp32 (fp32), 3 bf16 (bf16); out 1 bf16,
+                          // 2 fp32
   float beta, gain, decay, rate;
   float scale, eps;
   float coef[3 * LINALG_MAX_STEPS];
@@ -67,14 +70,6 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void sync_cluster() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ float4 ld_remote4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
 }
 __device__ __forceinline__ double ld_remote_f64(uint32_t addr) {
   double v;
@@ -145,67 +140,227 @@ __device__ __forceinline__ void add8(float (&v)[8], uint4 w, float f) {
   for (int j = 0; j < 8; ++j) v[j] = fmaf(f, __half2float(h[j]), v[j]);
 }
 
-// The input (and momentum) of one matrix's share of this CTA, in the caller's order: `WARPS`
-// warps walk chunks of eight of its columns, four in flight per thread. body(row, column, count,
-// u) gets the iteration's start value; row and column count from the share's first element.
-template <bool MUON, bool UPDATE, typename Body>
-__device__ __forceinline__ void walk_input(const SmallArgs& g, int64_t i, int c_first, int cols,
-                                           int worker, int workers, const Body& body) {
-  const int rows = g.tall ? cols : g.s, width = g.tall ? g.s : cols;
-  const int row0 = g.tall ? c_first : 0, col0 = g.tall ? 0 : c_first;
-  // a wide matrix's row goes to one row of X: consecutive lanes take consecutive chunks. A tall
-  // one's row is scattered over X's rows (two bytes each): 8 rows x 4 chunks per warp, which
-  // trades 64-byte reads for 4-way instead of 16-way bank conflicts
-  const int per_row = (width + 7) / 8;
-  const int cw = g.tall ? 4 : 1;
-  const int strips = (per_row + cw - 1) / cw;
-  const int total = g.tall ? (rows + 7) / 8 * strips * 32 : rows * per_row;
-  constexpr int U = 4;
-  for (int k0 = worker; k0 < total; k0 += U * workers) {
-    Raw8 x[U], mo[U];
-    int rr[U], cc[U];
+// k / d for the divisor whose rounded-up 2^32 / d is given; exact while k * d < 2^32.
+__device__ __forceinline__ int div_by(int k, uint32_t reciprocal, int d) {
+  return d == 1 ? k : int(__umulhi(uint32_t(k), reciprocal));
+}
+// Sum of squares of eight values, in FP32 (of scaled values where a square could leave its range)
+// and handed on in FP64: converting every element costs more than everything else here.
+__device__ __forceinline__ double squares8(const float (&u)[8], int count) {
+  float top = 0.f, s = 0.f;
 #pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int k = k0 + q * workers;
-      if (g.tall) {
-        const int t = k >> 5, l = k & 31;
-        rr[q] = (t / strips) * 8 + (l & 7);
-        cc[q] = ((t % strips) * 4 + (l >> 3)) * 8;
-      } else {
-        rr[q] = k / per_row;
-        cc[q] = (k - rr[q] * per_row) * 8;
+  for (int j = 0; j < 8; ++j)
+    if (j < count) {
+      top = fmaxf(top, fabsf(u[j]));
+      s = fmaf(u[j], u[j], s);
+    }
+  if (s != s || top == 0.f || (top > 0x1p-40f && top < 0x1p50f)) return double(s);
+  if (isinf(top)) return double(top);
+  const int k = ilogbf(top) / 2;
+  const float f = ldexpf(1.f, -k);
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < count) s = fmaf(u[j] * f * f, u[j] * f * f, s);
+  return ldexp(double(s), 4 * k);
+}
+
+struct Start {  // where read_start works
+  uint8_t* xs;
+  uint32_t x_plane;
+  double *warp_sum, *mat_sum;
+  float2* factor;
+  int64_t tile;
+  int c_first, cols;
+};
+
+// Norms, then X = scale * u / (norm + eps). Each matrix of the tile has its own warps, which walk
+// its share of this CTA in the caller's order in chunks of eight columns, U in flight per
+// thread. The last U stay in registers between the two passes: all of them up to 128 x 128.
+// One instance per pair of types, and rolled loops: what runs once waits for its own
+// instructions, so the path taken has to be short.
+template <int T, bool SPLIT, bool MUON, bool CLUSTER, typename TX, typename TM>
+__device__ __forceinline__ void read_start(const SmallArgs& g, const Start& st) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int team = (T / 32) / g.per_cta;  // warps per matrix (per_cta <= 8)
+  const int mine = warp / team;           // matrix of the tile this warp reads
+  const int64_t im = st.tile * g.per_cta + mine;
+  const bool reads = mine < g.per_cta && im < g.batch;
+  const int worker = tid - mine * team * 32, workers = team * 32;
+  const int rows = g.tall ? st.cols : g.s, width = g.tall ? g.s : st.cols;
+  // A wide matrix's row goes to one row of X: consecutive lanes take consecutive chunks. A tall
+  // one's is scattered over X's rows, two bytes each: 8 rows x 4 chunks per warp, which trades
+  // shorter reads for 4-way instead of 16-way bank conflicts.
+  const int per_row = (width + 7) / 8;
+  const int strips = g.tall ? (per_row + 3) / 4 : per_row;
+  const uint32_t reciprocal = uint32_t(0xffffffffu / uint32_t(strips > 0 ? strips : 1)) + 1u;
+  const int total = g.tall ? (rows + 7) / 8 * strips * 32 : rows * per_row;
+  constexpr int U = T == 512 && !MUON ? 4 : 2;  // registers: 16 (32) per chunk and array
+  const int batches = (total + U * workers - 1) / (U * workers);
+  const int64_t x0 = im * g.x.stride + (g.tall ? int64_t(st.c_first) * g.x.ld : st.c_first);
+  const int64_t m0 =
+      im * g.momentum.stride + (g.tall ? int64_t(st.c_first) * g.momentum.ld : st.c_first);
+  const int base = mine * g.pitch;
+  float u[U][8];
+  int rr[U], cc[U];
+  double sum = 0.0;
+  float2 f = make_float2(0.f, 0.f);
+  bool finite = false;
+#pragma unroll 1
+  for (int it = 0; it < 2 * batches || it == 0; ++it) {
+    const bool first = it < batches;
+    if (it == batches) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) st.warp_sum[warp] = sum;
+      __syncthreads();
+      if (tid < g.per_cta) {
+        double t = 0.0;
+        for (int k = 0; k < team; ++k) t += st.warp_sum[tid * team + k];
+        st.mat_sum[tid] = t;
       }
-      if (k >= total || rr[q] >= rows || cc[q] >= width) rr[q] = -1;
-      if (rr[q] >= 0) {
-        const int count = width - cc[q] < 8 ? width - cc[q] : 8;
-        load_raw(g.x, i * g.x.stride + int64_t(row0 + rr[q]) * g.x.ld + col0 + cc[q], count, x[q]);
-        if (MUON)
-          load_raw(g.momentum,
-                   i * g.momentum.stride + int64_t(row0 + rr[q]) * g.momentum.ld + col0 + cc[q],
-                   count, mo[q]);
+      if (CLUSTER) sync_cluster();
+      if (tid < g.per_cta) {
+        double t = st.mat_sum[tid];
+        if (CLUSTER) {
+          t = 0.0;
+          for (int k = 0; k < g.ranks; ++k)
+            t += ld_remote_f64(remote(smem_u32(st.mat_sum + tid), k));
+        }
+        // a matrix with a NaN or an infinity is worked on as zeros (its entries would reach the
+        // others of the tile) and written as NaN: marked by a factor that is not finite
+        st.factor[tid] = start_factor(t, g.scale, g.eps);
+      }
+      __syncthreads();
+      if (batches == 0) break;
+      if (reads) f = st.factor[mine];
+      finite = isfinite(f.x);
+    }
+    if (!reads) continue;
+    if (it != batches) {
+      const int k0 = (first ? it : 2 * batches - 1 - it) * U * workers + worker;
+      Eight<TX> x[U];
+      Eight<TM> mo[MUON ? U : 1];
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        const int k = k0 + q * workers;
+        if (g.tall) {
+          const int t = k >> 5, l = k & 31, block = div_by(t, reciprocal, strips);
+          rr[q] = block * 8 + (l & 7);
+          cc[q] = ((t - block * strips) * 4 + (l >> 3)) * 8;
+        } else {
+          rr[q] = div_by(k, reciprocal, strips);
+          cc[q] = (k - rr[q] * per_row) * 8;
+        }
+        if (k >= total || rr[q] >= rows || cc[q] >= width) rr[q] = -1;
+        if (rr[q] >= 0) {
+          const int count = width - cc[q] < 8 ? width - cc[q] : 8;
+          x[q].load(g.x, x0 + int64_t(rr[q]) * g.x.ld + cc[q], count);
+          if (MUON) mo[MUON ? q : 0].load(g.momentum, m0 + int64_t(rr[q]) * g.momentum.ld + cc[q], count);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        if (rr[q] < 0) continue;
+        x[q].get(u[q]);
+        if (MUON) {
+          float m[8];
+          mo[MUON ? q : 0].get(m);
+          if (first) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[j] = fmaf(g.beta, m[j], g.gain * u[q][j]);
+            Eight<TM>::put(g.momentum, m0 + int64_t(rr[q]) * g.momentum.ld + cc[q], m,
+                           width - cc[q] < 8 ? width - cc[q] : 8);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            u[q][j] = g.nesterov ? fmaf(g.beta, m[j], g.gain * u[q][j]) : m[j];
+        }
       }
     }
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       if (rr[q] < 0) continue;
       const int count = width - cc[q] < 8 ? width - cc[q] : 8;
-      float u[8];
-      convert_raw(x[q], g.x.type, u);
-      if (MUON) {
-        float m[8];
-        convert_raw(mo[q], g.momentum.type, m);
-        if (UPDATE) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) m[j] = fmaf(g.beta, m[j], g.gain * u[j]);
-          store_any(g.momentum,
-                    i * g.momentum.stride + int64_t(row0 + rr[q]) * g.momentum.ld + col0 + cc[q],
-                    m, count);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = g.nesterov ? fmaf(g.beta, m[j], g.gain * u[j]) : m[j];
+      if (first) {
+        sum += squares8(u[q], count);
+        continue;
       }
-      body(rr[q], cc[q], count, u);
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = finite && j < count ? start_scaled(u[q][j], f) : 0.f;
+      uint4 hi, lo;
+      round8v<SPLIT>(y, hi, lo);
+      if (!g.tall) {
+        const uint32_t at = chunk_at(base + rr[q], cc[q]);
+        *reinterpret_cast<uint4*>(st.xs + at) = hi;
+        if (SPLIT) *reinterpret_cast<uint4*>(st.xs + st.x_plane + at) = lo;
+      } else {
+        const __half* h = reinterpret_cast<const __half*>(&hi);
+        const __half* l = reinterpret_cast<const __half*>(&lo);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= count) break;
+          const uint32_t at = chunk_at(base + cc[q] + j, rr[q]) + (rr[q] & 7) * 2;
+          *reinterpret_cast<__half*>(st.xs + at) = h[j];
+          if (SPLIT) *reinterpret_cast<__half*>(st.xs + st.x_plane + at) = l[j];
+        }
+      }
     }
+  }
+}
+
+// Writes 64 columns of the result, staged as FP32, in the caller's order. Wide: [row][column],
+// the 16-byte units of a row permuted by it; tall: [column][row].
+template <int T, bool MUON, typename TO>
+__device__ __forceinline__ void write_result(const SmallArgs& g, const Start& st,
+                                             const float* stage, int n0) {
+  const int left = st.cols - n0 < 64 ? st.cols - n0 : 64;  // columns of X in this piece
+  const int per_row = g.tall ? g.pitch / 8 : 8;            // chunks of a caller's row
+  const int lines = g.tall ? 64 * g.per_cta : 128;         // caller's rows
+#pragma unroll 1
+  for (int k = threadIdx.x; k < lines * per_row; k += T) {
+    const int line = k / per_row, c = (k - line * per_row) * 8;
+    int mt, er, ec, count;  // matrix of the tile; the caller's row, first column, columns
+    const float* src;
+    int flip = 0;
+    if (g.tall) {
+      mt = line >> 6;
+      const int col = line & 63;
+      er = st.c_first + n0 + col, ec = c;
+      count = col < left ? g.s - c : 0;
+      src = stage + col * 128 + mt * g.pitch + c;
+    } else {
+      mt = line / g.pitch;
+      const int lr = line - mt * g.pitch;
+      er = lr, ec = st.c_first + n0 + c;
+      count = lr < g.s && mt < g.per_cta ? left - c : 0;
+      flip = line & 15;
+      src = stage + line * 64;
+    }
+    const int64_t im = st.tile * g.per_cta + mt;
+    if (count <= 0 || im >= g.batch) continue;
+    if (count > 8) count = 8;
+    const int64_t at = im * g.out.stride + int64_t(er) * g.out.ld + ec;
+    Eight<TO> w;
+    if (MUON) w.load(g.out, at, count);
+    float y[8];
+    const float4 a = *reinterpret_cast<const float4*>(g.tall ? src : src + ((c / 4) ^ flip) * 4);
+    const float4 b =
+        *reinterpret_cast<const float4*>(g.tall ? src + 4 : src + ((c / 4 + 1) ^ flip) * 4);
+    y[0] = a.x, y[1] = a.y, y[2] = a.z, y[3] = a.w;
+    y[4] = b.x, y[5] = b.y, y[6] = b.z, y[7] = b.w;
+    if (!isfinite(st.factor[mt].x)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fc00000);
+    }
+    if (MUON) {
+      float old[8];
+      w.get(old);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = fmaf(-g.rate, y[e], g.decay * old[e]);
+    }
+    Eight<TO>::put(g.out, at, y, count);
   }
 }
 
@@ -223,20 +378,18 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
   uint8_t* xs = smem;                            // [P] X: blocks of 64 columns
   uint8_t* gs = xs + P * x_plane;                // [P] G, then B: two blocks
   constexpr uint32_t g_plane = 2 * kBlockBytes;
-  uint8_t* es = gs + P * g_plane;                // CLUSTER: FP32 partial of G, [column / 4][row] x 4
+  uint8_t* es = gs + P * g_plane;                // CLUSTER: FP32 partials of this CTA's slice of G
   double* warp_sum = reinterpret_cast<double*>(es);  // [T / 32] (CLUSTER: before es is used)
   double* mat_sum = reinterpret_cast<double*>(es + (CLUSTER ? 65536 : 128));  // [8] per matrix
   float2* factor = reinterpret_cast<float2*>(mat_sum + 8);  // [8]
   uint64_t* bar = reinterpret_cast<uint64_t*>(factor + 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5;
   const int row = tid & 127, part = tid >> 7;  // this thread's TMEM lane and share of the columns
   const uint32_t rank = CLUSTER ? rank_in_cluster() : 0;
   const int64_t tile = CLUSTER ? blockIdx.x / g.ranks : blockIdx.x;
-  const int in_tile = row / g.pitch, r = row - in_tile * g.pitch;  // matrix, row within it
-  const int64_t i = tile * g.per_cta + in_tile;
-  const bool live = in_tile < g.per_cta && r < g.s && i < g.batch;
+  const int in_tile = row / g.pitch;  // matrix of this row
   const int c_first = int(rank) * g.cta_cols;     // first column of this CTA
   const int cols = g.len - c_first < g.cta_cols ? (g.len - c_first > 0 ? g.len - c_first : 0)
                                                 : g.cta_cols;
@@ -258,73 +411,26 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       (tile + 1) * g.per_cta > g.batch)
     for (uint32_t k = tid * 16; k < P * x_plane; k += T * 16)
       *reinterpret_cast<uint4*>(xs + k) = make_uint4(0, 0, 0, 0);
+  // and in G's: its entries between matrices stay as they are
+  if (g.per_cta > 1)
+    for (uint32_t k = tid * 16; k < P * g_plane; k += T * 16)
+      *reinterpret_cast<uint4*>(gs + k) = make_uint4(0, 0, 0, 0);
   griddep_wait();
   griddep_launch();
 
-  // ---- the norms. Each matrix of the tile has its own warps. ----
-  const int team = (T / 32) / g.per_cta;  // warps per matrix (per_cta <= 8)
-  const int mine = warp / team;           // matrix of the tile this warp reads
-  const int64_t im = tile * g.per_cta + mine;
-  const bool reads = mine < g.per_cta && im < g.batch;
-  const int worker = tid - mine * team * 32, workers = team * 32;
-  double sum = 0.0;
-  if (reads)
-    walk_input<MUON, true>(g, im, c_first, cols, worker, workers,
-                           [&](int, int, int count, const float (&u)[8]) {
-#pragma unroll
-                             for (int j = 0; j < 8; ++j)
-                               if (j < count) sum += double(u[j]) * double(u[j]);
-                           });
-#pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) warp_sum[warp] = sum;
-  __syncthreads();
-  if (tid < g.per_cta) {
-    double total = 0.0;
-    for (int k = 0; k < team; ++k) total += warp_sum[tid * team + k];
-    mat_sum[tid] = total;
-  }
-  if (CLUSTER) sync_cluster();
-  if (tid < g.per_cta) {
-    double total = mat_sum[tid];
-    if (CLUSTER) {
-      total = 0.0;
-      for (int k = 0; k < g.ranks; ++k) total += ld_remote_f64(remote(smem_u32(mat_sum + tid), k));
-    }
-    // a matrix with a NaN or an infinity is worked on as zeros (its entries would reach the
-    // others of the tile) and written as NaN: marked by a factor that is not finite
-    factor[tid] = start_factor(total, g.scale, g.eps);
-  }
-  __syncthreads();
-
-  // ---- X = scale * u / (norm + eps) ----
-  if (reads) {
-    const float2 f = factor[mine];
-    const bool finite = isfinite(f.x);
-    const int base = mine * g.pitch;
-    walk_input<MUON, false>(g, im, c_first, cols, worker, workers,
-                            [&](int rr, int cc, int count, const float (&u)[8]) {
-      float y[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = finite && j < count ? start_scaled(u[j], f) : 0.f;
-      uint4 hi, lo;
-      round8v<SPLIT>(y, hi, lo);
-      if (!g.tall) {
-        const uint32_t at = chunk_at(base + rr, cc);
-        *reinterpret_cast<uint4*>(xs + at) = hi;
-        if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
-      } else {
-        const __half* h = reinterpret_cast<const __half*>(&hi);
-        const __half* l = reinterpret_cast<const __half*>(&lo);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j >= count) break;
-          const uint32_t at = chunk_at(base + cc + j, rr) + (rr & 7) * 2;
-          *reinterpret_cast<__half*>(xs + at) = h[j];
-          if (SPLIT) *reinterpret_cast<__half*>(xs + x_plane + at) = l[j];
-        }
-      }
-    });
+  const Start st{xs, x_plane, warp_sum, mat_sum, factor, tile, c_first, cols};
+  switch (g.in_path) {
+    case 1:
+      read_start<T, SPLIT, MUON, CLUSTER, __nv_bfloat16, float>(g, st);
+      break;
+    case 2:
+      read_start<T, SPLIT, MUON, CLUSTER, float, float>(g, st);
+      break;
+    case 3:
+      read_start<T, SPLIT, MUON, CLUSTER, __nv_bfloat16, __nv_bfloat16>(g, st);
+      break;
+    default:
+      read_start<T, SPLIT, MUON, CLUSTER, Any, Any>(g, st);
   }
   fence_proxy_async_smem();
   tc_fence_before();
@@ -346,6 +452,11 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
     tc_fence_after();
   };
   const int k16 = (cols + 15) / 16;  // X's columns beyond `cols` are zero
+  // the 32-column groups of G that hold entries of this warp's rows (lanes 32 q .. + 31)
+  const int q32 = (warp & 3) * 32;
+  const int last_col = ((q32 + 31) / g.pitch + 1) * g.pitch;
+  const int win0 = g.per_cta == 1 ? 0 : q32 / g.pitch * g.pitch / 32;
+  const int win1 = g.per_cta == 1 || last_col > 128 ? 4 : (last_col + 31) / 32;
   const float inv = 1.f / g.scale;
 
   for (int step = 0; step < g.steps; ++step) {
@@ -371,10 +482,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
     wait();
     // columns 64 * half .. + 63 of this thread's row; entries between matrices are dropped
     if (!CLUSTER) {
-#pragma unroll
-      for (int q = 0; q < GCOLS / 32; ++q) {
+      for (int q = win0 + part; q < win1; q += PARTS) {
         float v[32];
-        const int c0 = part * GCOLS + q * 32;
+        const int c0 = q * 32;
         tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
@@ -391,27 +501,35 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
         }
       }
     } else {
+      // FP32 partials to the CTA that owns their columns: [from][column / 4][row] x 4 floats. Only
+      // writes cross the cluster, so nothing waits for a remote read.
+      const int width = 128 / g.ranks;  // columns per owner: 64, 32 or 16
+      const uint32_t slot = uint32_t(rank) * uint32_t(width) * 512;
 #pragma unroll
       for (int q = 0; q < GCOLS / 32; ++q) {
         float v[32];
         const int c0 = part * GCOLS + q * 32;
         tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(es + (uint32_t((c0 + j) >> 2) * 128 + row) * 16) =
-              make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < 32; j += 4) {
+          const int owner = (c0 + j) / width, c = (c0 + j) - owner * width;
+          const uint32_t at = smem_u32(es) + slot + (uint32_t(c >> 2) * 128 + row) * 16;
+          st_remote16(remote(at, owner),
+                      make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]),
+                                 __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])));
+        }
       }
       sync_cluster();
-      // this CTA's slice: 128 / ranks columns of every row; a thread sums 8 columns at a time
-      const int width = 128 / g.ranks;
+      // the slice this CTA owns: summed in rank order, rounded, written to every CTA
       for (int k = tid; k < 128 * (width / 8); k += T) {
-        const int rr = k & 127, c0 = int(rank) * width + (k >> 7) * 8;
+        const int rr = k & 127, c = (k >> 7) * 8, c0 = int(rank) * width + c;
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = 0.f;
-        for (int o = 0; o < g.ranks; ++o) {
-          const uint32_t at = remote(smem_u32(es + (uint32_t(c0 >> 2) * 128 + rr) * 16), o);
-          const float4 a = ld_remote4(at), b = ld_remote4(at + 2048);
+        const uint8_t* at = es + (uint32_t(c >> 2) * 128 + rr) * 16;
+        for (int o = 0; o < g.ranks; ++o, at += width * 512) {
+          const float4 a = *reinterpret_cast<const float4*>(at);
+          const float4 b = *reinterpret_cast<const float4*>(at + 2048);
           y[0] += a.x, y[1] += a.y, y[2] += a.z, y[3] += a.w;
           y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
         }
@@ -421,10 +539,10 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
         for (int e = 0; e < 8; ++e) y[e] *= f;
         uint4 hi, lo;
         round8v<SPLIT>(y, hi, lo);
-        const uint32_t at = smem_u32(gs) + chunk_at(rr, c0);
+        const uint32_t to = smem_u32(gs) + chunk_at(rr, c0);
         for (int o = 0; o < g.ranks; ++o) {
-          st_remote16(remote(at, o), hi);
-          if (SPLIT) st_remote16(remote(at + g_plane, o), lo);
+          st_remote16(remote(to, o), hi);
+          if (SPLIT) st_remote16(remote(to + g_plane, o), lo);
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");
@@ -448,10 +566,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-#pragma unroll
-    for (int q = 0; q < GCOLS / 32; ++q) {
+    for (int q = win0 + part; q < win1; q += PARTS) {
       float v[32];
-      const int c0 = part * GCOLS + q * 32;
+      const int c0 = q * 32;
       tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
       for (int j = 0; j < 32; j += 8) {
@@ -490,70 +607,68 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
     wait();
     const bool last = step + 1 == g.steps;
     const float f = last ? inv * inv : inv, fa = last ? ca * inv : ca;
-    for (int c0 = part * 32; c0 < g.cta_cols; c0 += PARTS * 32) {
-      // the weights of the last step, ahead of their use
-      Raw8 w[MUON ? 4 : 1];
-      uint32_t wt[MUON ? 32 : 1];
-      const int64_t at_row = g.tall ? i * g.out.stride + int64_t(c_first) * g.out.ld + r
-                                    : i * g.out.stride + int64_t(r) * g.out.ld + c_first;
-      if (MUON && last && live) {
-        if (g.tall) {
+    if (!last) {
+      for (int c0 = part * 32; c0 < g.cta_cols; c0 += PARTS * 32) {
+        float v[32];
+        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j < cols) wt[MUON ? j : 0] = load_one(g.out, at_row + int64_t(c0 + j) * g.out.ld);
-        } else {
+        for (int j = 0; j < 32; j += 8) {
+          float y[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 8 * j;
-            if (c < cols)
-              load_raw(g.out, at_row + c, cols - c < 8 ? cols - c : 8, w[MUON ? j : 0]);
-          }
-        }
-      }
-      float v[32];
-      tmem_ld32(tmem + lane_base + uint32_t(c0), v);
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
-        const int c = c0 + j;
-        const uint32_t at = chunk_at(row, c);
-        add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
-        if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
-        if (!last) {
+          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
+          const uint32_t at = chunk_at(row, c0 + j);
+          add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
+          if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
           uint4 hi, lo;
           round8v<SPLIT>(y, hi, lo);
           *reinterpret_cast<uint4*>(xs + at) = hi;
           if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
-        } else if (live && c < cols) {
-          const int count = cols - c < 8 ? cols - c : 8;
-          if (!isfinite(factor[in_tile].x)) {
+        }
+      }
+      publish();
+      continue;
+    }
+    // ---- the result, 64 columns at a time through G's buffer (no MMA reads it any more), so that
+    // the caller's rows are written in order ----
+    float* stage = reinterpret_cast<float*>(gs);
+#pragma unroll 1
+    for (int n0 = 0; n0 < g.cta_cols; n0 += 64) {
+      for (int h = part; h < 2; h += PARTS) {
+        const int c0 = n0 + h * 32;
+        float v[32];
+        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fc00000);
-          }
-          if (MUON) {
-            float old[8];
-            if (g.tall) {
+        for (int j = 0; j < 32; j += 8) {
+          float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) old[e] = bits_to_float(wt[MUON ? j + e : 0], g.out.type);
-            } else {
-              convert_raw(w[MUON ? j / 8 : 0], g.out.type, old);
-            }
+          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
+          const uint32_t at = chunk_at(row, c0 + j);
+          add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
+          if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
+          if (g.tall) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = fmaf(-g.rate, y[e], g.decay * old[e]);
-          }
-          if (g.tall) {  // a warp's lanes are consecutive columns of the caller's row
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e < count) store_one(g.out, at_row + int64_t(c + e) * g.out.ld, y[e]);
+            for (int e = 0; e < 8; ++e) stage[(h * 32 + j + e) * 128 + row] = y[e];
           } else {
-            store_any(g.out, at_row + c, y, count);
+            const int unit = (h * 32 + j) / 4;
+            *reinterpret_cast<float4*>(stage + row * 64 + ((unit ^ (row & 15)) * 4)) =
+                make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(stage + row * 64 + (((unit + 1) ^ (row & 15)) * 4)) =
+                make_float4(y[4], y[5], y[6], y[7]);
           }
         }
       }
+      __syncthreads();
+      if (g.out_path == 1)
+        write_result<T, MUON, __nv_bfloat16>(g, st, stage, n0);
+      else if (g.out_path == 2)
+        write_result<T, MUON, float>(g, st, stage, n0);
+      else
+        write_result<T, MUON, Any>(g, st, stage, n0);
+      __syncthreads();
     }
-    publish();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
   }
   if (CLUSTER) sync_cluster();  // no CTA leaves while another may read its shared memory
   if (warp == 0)
@@ -644,6 +759,14 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
   const int chunk = (g.len + g.ranks - 1) / g.ranks;
   g.cta_cols = (chunk + 63) / 64 * 64;
   g.steps = steps;
+  if (n % 8 == 0) {
+    const bool mo32 = momentum == nullptr || (momentum->type == LINALG_FP32 && g.momentum.vec);
+    const bool mo16 = momentum != nullptr && momentum->type == LINALG_BF16 && g.momentum.vec;
+    if (g.x.vec && x->type == LINALG_BF16) g.in_path = mo32 ? 1 : (mo16 ? 3 : 0);
+    if (g.x.vec && x->type == LINALG_FP32) g.in_path = mo32 ? 2 : 0;
+    if (g.out.vec && out->type == LINALG_BF16) g.out_path = 1;
+    if (g.out.vec && out->type == LINALG_FP32) g.out_path = 2;
+  }
   g.beta = float(beta), g.gain = float(1.0 - beta), g.nesterov = nesterov;
   g.decay = decay, g.rate = rate;
   g.scale = split ? 4096.f : 1024.f, g.eps = eps;
