@@ -4,14 +4,14 @@
 // A matrix is held as s x L, s its smaller side (a tall matrix is transposed on the way in and
 // out). p = floor(128 / s) matrices (s rounded up to 16) are stacked to the 128 rows of one tile: with the entries of
 // G = X X^T between different matrices set to zero, G, G G and B = b G + c G G stay block
-// diagonal and B X acts on each matrix alone, so one set of M = 128 MMAs serves all of them.
+// diagonal and (a I + B) X acts on each matrix alone, so one set of M = 128 MMAs serves all of them.
 //
 // X lives in shared memory as 128-byte-swizzled K-major blocks of 64 columns; the same bytes are
 // the MN-major B operand of B X (the summed index is then X's row). G and B share one buffer: an
 // epilogue thread overwrites the elements it has read. Accumulators in TMEM, a thread per row
 // and share of the columns.
 //
-//   per step:  G = X X^T -> mask, fp16   |   B = b G + c G G -> fp16   |   X <- a X + B X
+//   per step:  G = X X^T -> mask, fp16   |   B = a I + b G + c G G -> fp16   |   X <- B X
 //
 // A long matrix is split over a cluster of 2, 4 or 8 CTAs by columns. Only G needs all columns:
 // each CTA writes its FP32 partials to the CTAs that own their columns, which sum them in rank
@@ -54,7 +54,8 @@ struct SmallArgs {
                           // in 1 bf16 (momentum fp32), 2 fp32 (fp32), 3 bf16 (bf16); out 1 bf16,
                           // 2 fp32
   float beta, gain, decay, rate;
-  float scale, eps;
+  float scale, eps;       // of X; G has scale^2, B 1
+  float inv_gram, inv_x;  // their reciprocals
   float coef[3 * LINALG_MAX_STEPS];
 };
 
@@ -106,6 +107,19 @@ __device__ __forceinline__ uint64_t desc_cols(const void* tile) {
 __device__ __forceinline__ uint32_t idesc_half(int n, int b_mn_major) {
   return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (8u << 24);
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 // Byte offset of the 16-byte chunk holding columns c .. c + 7 of row r.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return uint32_t(c >> 6) * kBlockBytes + uint32_t(r) * 128 + ((uint32_t(c >> 3) & 7) ^ (r & 7)) * 16;
@@ -113,8 +127,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 
 // Eight values to fp16 (and the remainder plane): shared-memory chunks of 16 bytes. Saturating: an
 // infinity in one matrix would reach the others of its tile as 0 * inf in B X. (Only
-// coefficients with which the iteration diverges get there: 65504 is 16 times the
-// largest singular value's bound in full precision, 64 times in half.)
+// coefficients with which the iteration diverges get there: 65504 stands for
+// singular values of G of 16 in full precision and 64 in half.)
 __device__ __forceinline__ uint32_t half2_sat(float a, float b) {
   uint32_t r;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
@@ -134,10 +148,16 @@ __device__ __forceinline__ void round8v(const float (&v)[8], uint4& hi, uint4& l
   hi = make_uint4(h[0], h[1], h[2], h[3]);
   if (SPLIT) lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
+// v += f * (eight fp16 values)
 __device__ __forceinline__ void add8(float (&v)[8], uint4 w, float f) {
-  const __half* h = reinterpret_cast<const __half*>(&w);
+  const __half2* h = reinterpret_cast<const __half2*>(&w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = fmaf(f, __half2float(h[j]), v[j]);
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = __half22float2(h[j]);
+    const float2 r = chol::ffma2(make_float2(f, f), x, make_float2(v[2 * j], v[2 * j + 1]));
+    v[2 * j] = r.x;
+    v[2 * j + 1] = r.y;
+  }
 }
 
 // k / d for the divisor whose rounded-up 2^32 / d is given; exact while k * d < 2^32.
@@ -457,7 +477,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
   const int last_col = ((q32 + 31) / g.pitch + 1) * g.pitch;
   const int win0 = g.per_cta == 1 ? 0 : q32 / g.pitch * g.pitch / 32;
   const int win1 = g.per_cta == 1 || last_col > 128 ? 4 : (last_col + 31) / 32;
-  const float inv = 1.f / g.scale;
+  constexpr bool KEEP = T == 512 && !CLUSTER;  // G's FP32 values stay in registers until B
+  constexpr int GROUPS = 4 / PARTS;            // 32-column groups of G per thread
+  float gram[KEEP ? 32 : 1];
 
   for (int step = 0; step < g.steps; ++step) {
     const float ca = g.coef[3 * step], cb = g.coef[3 * step + 1], cc = g.coef[3 * step + 2];
@@ -469,10 +491,16 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // lo hi, hi lo, hi hi
         const uint8_t* pa = xs + (t == 0 ? x_plane : 0);
         const uint8_t* pb = xs + (t == 1 ? x_plane : 0);
-        for (int k = 0; k < k16; ++k) {
-          const uint64_t off = uint64_t((k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
-          mma_half(tmem, sw128_desc(pa) + off, sw128_desc(pb) + off, id, any);
-          any = 1;
+        const uint64_t da = sw128_desc(pa), db = sw128_desc(pb);
+#pragma unroll 1
+        for (int k = 0; k < k16; k += 4) {
+          const uint64_t off = uint64_t((k >> 2) * kBlockBytes) >> 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (k + e >= k16) break;
+            mma_half(tmem, da + off + e * 2, db + off + e * 2, id, any);
+            any = 1;
+          }
         }
       }
       if (!any)  // no columns here (a cluster longer than the matrix): zeros from zero columns
@@ -480,24 +508,34 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-    // columns 64 * half .. + 63 of this thread's row; entries between matrices are dropped
+    // (scale of G: X's squared, so the sums are stored as they are; entries between matrices are
+    // dropped)
     if (!CLUSTER) {
-      for (int q = win0 + part; q < win1; q += PARTS) {
-        float v[32];
-        const int c0 = q * 32;
-        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          // 8 columns are of one matrix: the pitch is a multiple of 16
-          const float f = uint32_t(c0 + j - in_tile * g.pitch) < uint32_t(g.pitch) ? inv : 0.f;
-          float y[8];
+      for (int n = 0; n < GROUPS; ++n) {
+        const int q = win0 + part + n * PARTS;
+        if (q >= win1) break;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
-          uint4 hi, lo;
-          round8v<SPLIT>(y, hi, lo);
-          const uint32_t at = chunk_at(row, c0 + j);
-          *reinterpret_cast<uint4*>(gs + at) = hi;
-          if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+        for (int h = 0; h < 2; ++h) {
+          float v[16];
+          const int c0 = q * 32 + h * 16;
+          tmem_ld16(tmem + lane_base + uint32_t(c0), v);
+          // 16 columns are of one matrix: the pitch is a multiple of 16
+          const bool own = uint32_t(c0 - in_tile * g.pitch) < uint32_t(g.pitch);
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              y[e] = own ? v[j + e] : 0.f;
+              if (KEEP) gram[KEEP ? h * 16 + j + e : 0] = y[e];
+            }
+            uint4 hi, lo;
+            round8v<SPLIT>(y, hi, lo);
+            const uint32_t at = chunk_at(row, c0 + j);
+            *reinterpret_cast<uint4*>(gs + at) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+          }
         }
       }
     } else {
@@ -534,9 +572,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
           y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
         }
         const int mt = rr / g.pitch;
-        const float f = uint32_t(c0 - mt * g.pitch) < uint32_t(g.pitch) ? inv : 0.f;
+        const bool own = uint32_t(c0 - mt * g.pitch) < uint32_t(g.pitch);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= f;
+        for (int e = 0; e < 8; ++e) y[e] = own ? y[e] : 0.f;
         uint4 hi, lo;
         round8v<SPLIT>(y, hi, lo);
         const uint32_t to = smem_u32(gs) + chunk_at(rr, c0);
@@ -566,26 +604,57 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-    for (int q = win0 + part; q < win1; q += PARTS) {
-      float v[32];
-      const int c0 = q * 32;
-      tmem_ld32(tmem + lane_base + uint32_t(c0), v);
+    // B takes a on its diagonal (its scale is 1), so that X <- B X needs no old X: one more rounding
+    // of 2^-12 per row, as X's own, for half of that epilogue's instructions
+    const float fb = cb * g.inv_gram, fc = cc * g.inv_gram * g.inv_gram;
 #pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        float y[8];
+    for (int n = 0; n < GROUPS; ++n) {
+      const int q = win0 + part + n * PARTS;
+      if (q >= win1) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = v[j + e] * (cc * inv);
-        const uint32_t at = chunk_at(row, c0 + j);
-        add8(y, *reinterpret_cast<const uint4*>(gs + at), cb);
-        if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), cb);
-        uint4 hi, lo;
-        round8v<SPLIT>(y, hi, lo);
-        *reinterpret_cast<uint4*>(gs + at) = hi;
-        if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+      for (int h = 0; h < 2; ++h) {
+        float v[16];
+        const int c0 = q * 32 + h * 16;
+        tmem_ld16(tmem + lane_base + uint32_t(c0), v);
+        const int diag = row - c0;  // this row's diagonal element, if in these columns
+        if (CLUSTER || !KEEP) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] *= fc;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j += 8) {
+          float y[8];
+          const uint32_t at = chunk_at(row, c0 + j);
+          if (!CLUSTER && KEEP) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float2 t = chol::ffma2(
+                  make_float2(gram[KEEP ? h * 16 + j + e : 0], gram[KEEP ? h * 16 + j + e + 1 : 0]),
+                  make_float2(fb, fb), make_float2(0.f, 0.f));
+              const float2 x = chol::ffma2(make_float2(v[j + e], v[j + e + 1]), make_float2(fc, fc), t);
+              y[e] = x.x;
+              y[e + 1] = x.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = v[j + e];
+            add8(y, *reinterpret_cast<const uint4*>(gs + at), fb);
+            if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), fb);
+          }
+          if (q * 32 == q32) {  // the same for the whole warp
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              y[e] += j + e == diag ? ca : 0.f;  // a select: branches would part the warp
+          }
+          uint4 hi, lo;
+          round8v<SPLIT>(y, hi, lo);
+          *reinterpret_cast<uint4*>(gs + at) = hi;
+          if (SPLIT) *reinterpret_cast<uint4*>(gs + g_plane + at) = lo;
+        }
       }
     }
     publish();
-    // ---- X <- a X + B X ----
+    // ---- X <- B X ----
     if (tid == 0 && ok) {
       for (int n0 = 0; n0 < g.cta_cols; n0 += 256) {
         const int n = g.cta_cols - n0 < 256 ? g.cta_cols - n0 : 256;
@@ -605,24 +674,23 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-    const bool last = step + 1 == g.steps;
-    const float f = last ? inv * inv : inv, fa = last ? ca * inv : ca;
-    if (!last) {
+    if (step + 1 < g.steps) {
       for (int c0 = part * 32; c0 < g.cta_cols; c0 += PARTS * 32) {
-        float v[32];
-        tmem_ld32(tmem + lane_base + uint32_t(c0), v);
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          float y[8];
+        for (int h = 0; h < 2; ++h) {
+          float v[16];
+          tmem_ld16(tmem + lane_base + uint32_t(c0 + h * 16), v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
-          const uint32_t at = chunk_at(row, c0 + j);
-          add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
-          if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
-          uint4 hi, lo;
-          round8v<SPLIT>(y, hi, lo);
-          *reinterpret_cast<uint4*>(xs + at) = hi;
-          if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
+          for (int j = 0; j < 16; j += 8) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = v[j + e];
+            uint4 hi, lo;
+            round8v<SPLIT>(y, hi, lo);
+            const uint32_t at = chunk_at(row, c0 + h * 16 + j);
+            *reinterpret_cast<uint4*>(xs + at) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
+          }
         }
       }
       publish();
@@ -641,10 +709,7 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
         for (int j = 0; j < 32; j += 8) {
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * f;
-          const uint32_t at = chunk_at(row, c0 + j);
-          add8(y, *reinterpret_cast<const uint4*>(xs + at), fa);
-          if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), fa);
+          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * g.inv_x;
           if (g.tall) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) stage[(h * 32 + j + e) * 128 + row] = y[e];
@@ -769,7 +834,8 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
   }
   g.beta = float(beta), g.gain = float(1.0 - beta), g.nesterov = nesterov;
   g.decay = decay, g.rate = rate;
-  g.scale = split ? 4096.f : 1024.f, g.eps = eps;
+  g.scale = split ? 64.f : 32.f, g.eps = eps;
+  g.inv_x = 1.f / g.scale, g.inv_gram = g.inv_x * g.inv_x;
   for (int k = 0; k < 3 * steps; ++k) g.coef[k] = coefficients[k];
   const size_t smem = smem_bytes(split, g.ranks, g.cta_cols);
   if (tiles * g.ranks > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;

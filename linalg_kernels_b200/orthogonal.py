@@ -66,6 +66,8 @@ def _batch_stride(t: torch.Tensor) -> int | None:
 
 def _is_rows(t: torch.Tensor, writable: bool) -> bool:
     """Whether the C ABI can address ``t``: contiguous rows, one row and one matrix stride."""
+    if t.is_contiguous():
+        return True
     m, n = t.shape[-2:]
     step = _batch_stride(t)
     if step is None or (n > 1 and t.stride(-1) != 1) or (m > 1 and t.stride(-2) < n):
@@ -83,6 +85,8 @@ def _is_transposed(t: torch.Tensor) -> bool:
 
 def _matrix(t: torch.Tensor) -> tuple[int, int, int, int]:
     m, n = t.shape[-2:]
+    if t.is_contiguous():
+        return t.data_ptr(), n, m * n, _TYPES[t.dtype]
     return t.data_ptr(), (t.stride(-2) if m > 1 else n), _batch_stride(t), _TYPES[t.dtype]
 
 
@@ -116,8 +120,8 @@ def _check_iteration(steps, coefficients, eps, precision):
 def _workspace(batch, m, n, precision, dtype, device):
     if precision is None:
         precision = "half" if dtype is torch.bfloat16 else "full"
-    need = int(_lib.load().linalg_orthogonalize_workspace(batch, m, n, _PRECISIONS[precision]))
-    return torch.empty(need, dtype=torch.uint8, device=device), need
+    need = _workspace_bytes(batch, m, n, _PRECISIONS[precision])
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
 def _same_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -125,6 +129,9 @@ def _same_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _ends(t: torch.Tensor) -> tuple[int, int]:
+    if t.is_contiguous():
+        start = t.data_ptr()
+        return start, start + t.numel() * t.element_size()
     last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
@@ -132,6 +139,45 @@ def _ends(t: torch.Tensor) -> tuple[int, int]:
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     (a0, a1), (b0, b1) = _ends(a), _ends(b)
     return a0 < b1 and b0 < a1
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, m: int, n: int, precision: int) -> int:
+    """A function of its arguments alone (no library option changes it)."""
+    return int(_lib.load().linalg_orthogonalize_workspace(batch, m, n, precision))
+
+
+_plain: dict = {}  # (steps, coefficients, eps, precision) of earlier calls -> checked arguments
+_call = None       # the binding, once loaded
+
+
+def _contiguous_call(x, steps, coefficients, eps, precision):
+    """The common call (contiguous input, fresh output, one GPU) with arguments that an earlier call
+    has checked: the host path paces calls of a few microseconds. None: not that case."""
+    if type(x) is not torch.Tensor or not x.is_cuda or not x.is_contiguous() or \
+            x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()):
+        return None
+    kind = _TYPES.get(x.dtype)
+    try:
+        plan = _plain.get((steps, coefficients, eps, precision))
+    except TypeError:  # coefficients as lists
+        return None
+    if kind is None or plan is None or _call is None:
+        return None
+    shape = x.shape
+    m, n = shape[-2], shape[-1]
+    batch = shape[0] if len(shape) == 3 else 1
+    size = m * n
+    if not size or not batch:
+        return None
+    coef, code = plan
+    out = torch.empty_like(x)
+    need = _workspace_bytes(batch, m, n, code or (1 if kind == 0 else 2))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device).data_ptr() if need else 0
+    _lib.check(_call(x.data_ptr(), n, size, kind, out.data_ptr(), n, size, kind, batch, m, n, steps,
+                     code, ws, need, _lib.current_queue(x.device.index), eps, coef),
+               "linalg_orthogonalize")
+    return out
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5, *,
@@ -151,8 +197,13 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     others of the batch alone. It has no derivative: call it under ``torch.no_grad()`` or on a
     detached tensor.
     """
+    if out is None and _one_device():
+        out = _contiguous_call(x, steps, coefficients, eps, precision)
+        if out is not None:
+            return out
     _check_tensor(x, "x")
     coef = _check_iteration(steps, coefficients, eps, precision)
+    _remember(steps, coefficients, eps, precision, coef)
     if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
         raise RuntimeError("orthogonalize has no derivative: call it under torch.no_grad()")
     if out is None:
@@ -181,11 +232,32 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
         ws, need = _workspace(batch, m, n, precision, x.dtype, x.device)
         return _lib.linalg().orthogonalize(
             *_matrix(source), *_matrix(target), batch, m, n, steps, _PRECISIONS[precision],
-            ws.data_ptr(), need, _lib.current_queue(x.device), eps, coef)
+            ws.data_ptr() if need else 0, need, _lib.current_queue(x.device), eps, coef)
 
     _lib.check(_on_device(x, call), "linalg_orthogonalize")
     torch.autograd.graph.increment_version(out)
     return out
+
+
+_single: bool | None = None
+
+
+def _one_device() -> bool:
+    """A single visible GPU: no call ever needs a device switch."""
+    global _single
+    if _single is None:
+        _single = torch.cuda.device_count() == 1
+    return _single
+
+
+def _remember(steps, coefficients, eps, precision, coef) -> None:
+    global _call
+    _call = _lib.linalg().orthogonalize
+    if isinstance(coefficients, tuple) and len(_plain) < 64:
+        try:
+            _plain[(steps, coefficients, eps, precision)] = coef, _PRECISIONS[precision]
+        except TypeError:
+            pass
 
 
 def _on_device(t: torch.Tensor, call):
@@ -235,7 +307,8 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
     if not _is_rows(p, True) or not _is_rows(mo, True):
         raise ValueError("param and momentum must both have contiguous rows, or both contiguous "
                          "columns, and one stride between matrices")
-    if _overlap(p, mo) or _overlap(p, g) or _overlap(mo, g):
+    (p0, p1), (g0, g1), (m0, m1) = _ends(p), _ends(g), _ends(mo)
+    if (p0 < m1 and m0 < p1) or (p0 < g1 and g0 < p1) or (m0 < g1 and g0 < m1):
         raise ValueError("param, grad and momentum must not overlap")
     if not _is_rows(g, False):
         g = g.contiguous()
@@ -246,7 +319,7 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
         ws, need = _workspace(batch, m, n, precision, param.dtype, param.device)
         return _lib.linalg().muon_update(
             *_matrix(p), *_matrix(g), *_matrix(mo), batch, m, n, int(bool(nesterov)), steps,
-            _PRECISIONS[precision], ws.data_ptr(), need, _lib.current_queue(param.device), beta,
+            _PRECISIONS[precision], ws.data_ptr() if need else 0, need, _lib.current_queue(param.device), beta,
             1.0 - lr * weight_decay, lr * scale, eps, coef)
 
     _lib.check(_on_device(param, call), "linalg_muon_update")
