@@ -1,0 +1,449 @@
+// lin_fused.cu — the Newton-Schulz iteration of a batch of middle-sized matrices (both sides > 128)
+// in one launch: a CTA pair takes a matrix through all its steps.
+//
+// Launched product by product (lin_gemm.cu), a batch whose X, G and B together exceed L2 streams
+// them through HBM three times a step (b640n512: 7 of 335 MB per step and array), and a small
+// batch pays a launch and an idle GPU's ramp per product. Here a pair owns one X (two buffers),
+// one G and one B, reused for each of its matrices, so they stay in L2, and the only work that
+// passes HBM is the start value and the result. The tiles, the operands' orders and the epilogue
+// are lin_gemm.cu's: 256 x 256 tiles, two accumulators, the epilogue of a tile beside the next
+// tile's MMAs.
+//
+// A tile needs parts of the phase before it (G of X, B of G, X of B). The pair's epilogue warps
+// count finished tiles in shared memory of both CTAs; the producers wait for the last tile that
+// theirs reads, not for the phase: with two row blocks (n = 512) every phase starts while the last
+// tile of the one before is in its epilogue. With one block (n = 256) the chain
+// MMA -> epilogue -> TMA is exposed, 15 times per matrix; it is still shorter than a launch.
+#include "lin_tile.cuh"
+#include "lin_fused.cuh"
+
+namespace lin {
+
+namespace {
+
+using namespace tile;
+
+using C = Cfg<256>;
+constexpr int S = C::STAGES;
+
+struct FusedArgs {
+  int m, n, s, batch;             // s: the smaller side
+  int tiles_m, tiles_n, tiles_s;  // 256-wide blocks of rows, columns, smaller side
+  int steps;
+  const __half* x0;  // [batch] start values
+  __half* x;         // [pair][2]
+  __half* sq;        // [pair][2]: G, B
+  int64_t ldx, lds, x_plane, s_plane;
+  float scale;
+  void* out;
+  int64_t ldo, out_stride;
+  int out_type, out_vec;
+  float decay, rate;
+  uint32_t idesc;  // K-major operands
+  float coef[3 * LINALG_MAX_STEPS];
+};
+
+// The tiles of one pair in order: per matrix and step G's lower tiles, B's, then X's.
+template <bool TALL>
+struct Sequence {
+  const FusedArgs& g;
+  int matrix, pairs, step, phase, index, count;  // count: tiles of the phase
+  int number;                                    // of this tile among all the pair's
+  int before;                                    // number of the first tile of the phase before
+  int tm, tn;
+  __device__ __forceinline__ Sequence(const FusedArgs& a, int pair, int p)
+      : g(a), matrix(pair), pairs(p), step(0), phase(0), index(0), number(0), before(0) {
+    count = lower();
+    place();
+  }
+  __device__ __forceinline__ int lower() const { return g.tiles_s * (g.tiles_s + 1) / 2; }
+  __device__ __forceinline__ bool valid() const { return matrix < g.batch; }
+  __device__ __forceinline__ void place() {
+    if (phase < 2) {
+      tm = int((sqrtf(8.f * float(index) + 1.f) - 1.f) * 0.5f);
+      while (tm * (tm + 1) / 2 > index) --tm;
+      while ((tm + 1) * (tm + 2) / 2 <= index) ++tm;
+      tn = index - tm * (tm + 1) / 2;
+    } else if (TALL) {  // by columns: the first need only B's first rows
+      tn = index / g.tiles_m;
+      tm = index - tn * g.tiles_m;
+    } else {
+      tm = index / g.tiles_n;
+      tn = index - tm * g.tiles_n;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    ++number;
+    if (++index == count) {
+      before = number - count;
+      index = 0;
+      if (++phase == 3) {
+        phase = 0;
+        if (++step == g.steps) {
+          step = 0;
+          matrix += pairs;
+        }
+      }
+      count = phase < 2 ? lower() : g.tiles_m * g.tiles_n;
+    }
+    place();
+  }
+  // Number of the last tile that this one reads from the phase before it; -1: none.
+  __device__ __forceinline__ int needs() const {
+    if (phase == 0) {
+      if (step == 0) return -1;
+      return TALL ? before + g.tiles_m * g.tiles_n - 1 : before + (tm + 1) * g.tiles_n - 1;
+    }
+    // rows r of a symmetric result: its lower tiles up to (last row, r) hold them or their mirror
+    const int r = phase == 1 || !TALL ? tm : tn;
+    return before + (g.tiles_s - 1) * g.tiles_s / 2 + r;
+  }
+  __device__ __forceinline__ int k_len() const {
+    return phase == 0 ? (TALL ? g.m : g.n) : g.s;
+  }
+  __device__ __forceinline__ bool a_mn() const { return TALL && phase == 0; }
+  __device__ __forceinline__ bool b_mn() const { return TALL ? phase == 0 : phase == 2; }
+};
+
+__device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.cluster.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void add_release(uint32_t cluster_addr) {
+  asm volatile("red.release.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_addr), "r"(1u)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t addr_in(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+
+template <bool TALL, int LAST>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    fused_kernel(const __grid_constant__ CUtensorMap x0_rows,
+                 const __grid_constant__ CUtensorMap x0_cols,
+                 const __grid_constant__ CUtensorMap x_rows,
+                 const __grid_constant__ CUtensorMap x_cols,
+                 const __grid_constant__ CUtensorMap squares, const FusedArgs g, int* status) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* epi = reinterpret_cast<float*>(smem + size_t(S) * C::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(S) * C::STAGE + C::EPI);
+  uint64_t* full = bars;           // [S] first CTA: a stage of both CTAs has landed
+  uint64_t* empty = bars + S;      // [S] the MMAs have read the stage
+  uint64_t* tfull = bars + 2 * S;  // [2] accumulator ready
+  uint64_t* tempty = tfull + 2;    // [2] first CTA: accumulator drained by both CTAs
+  uint32_t* done = reinterpret_cast<uint32_t*>(tempty + 2);  // [4] finished tiles, by number mod 4
+  uint32_t* tmem_slot = done + 4;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 2 * kEpiWarps);
+    }
+    for (int i = 0; i < 4; ++i) done[i] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&x0_rows);
+    prefetch_map(&x0_cols);
+    prefetch_map(&x_rows);
+    prefetch_map(&x_cols);
+    prefetch_map(&squares);
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(uint32_t(C::TMEM_COLS))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  griddep_wait();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  griddep_launch();
+  const uint32_t tmem = *tmem_slot;
+  const int pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t kt = 0;
+      bool ok = true;
+      for (Sequence<TALL> t(g, pair, pairs); t.valid() && ok; t.next()) {
+        const int need = t.needs();
+        if (need >= 0) {
+          const uint32_t target = 2 * kEpiWarps * (uint32_t(need) / 4 + 1);
+          const uint32_t* slot = &done[need & 3];
+          if (load_acquire(slot) < target) {
+            const uint64_t t0 = global_ns();
+            while (load_acquire(slot) < target)
+              if (global_ns() - t0 > kWaitLimitNs) {
+                atomicExch(status, CHOL_ERR_WAIT_TIMEOUT);
+                ok = false;
+                break;
+              }
+            if (!ok) break;
+          }
+          asm volatile("fence.proxy.async;" ::: "memory");  // those stores before these copies
+        }
+        const bool first = t.step == 0;
+        const int zx = first ? t.matrix : pair * 2 + ((t.step - 1) & 1);
+        const CUtensorMap* rows = first ? &x0_rows : &x_rows;
+        const CUtensorMap* cols = first ? &x0_cols : &x_cols;
+        const CUtensorMap *ma, *mb;
+        int za = zx, zb = zx;
+        if (t.phase == 1) {
+          ma = mb = &squares;
+          za = zb = pair * 2;
+        } else if (t.phase == 0) {
+          ma = mb = TALL ? cols : rows;
+        } else if (TALL) {
+          ma = rows;
+          mb = &squares;
+          zb = pair * 2 + 1;
+        } else {
+          ma = &squares;
+          za = pair * 2 + 1;
+          mb = cols;
+        }
+        const int a_row = t.tm * kTileM + int(rank) * 128, b_row = t.tn * 256 + int(rank) * 128;
+        const int num_k = (t.k_len() + kBlockK - 1) / kBlockK;
+        const bool amn = t.a_mn(), bmn = t.b_mn();
+        for (int kb = 0; kb < num_k; ++kb, ++kt) {
+          const int s = int(kt % S);
+          if (kt >= uint32_t(S) && !wait_bar(&empty[s], ((kt / S) & 1u) ^ 1u, status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + size_t(s) * C::STAGE;
+          uint8_t* sb = sa + C::A_BYTES;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+          const uint32_t bar = leader_addr(&full[s]);
+          const int kx = kb * kBlockK;
+          if (amn) {
+            tma_load_pair(sa, ma, a_row, kx, za, bar);
+            tma_load_pair(sa + 8192, ma, a_row + 64, kx, za, bar);
+          } else {
+            tma_load_pair(sa, ma, kx, a_row, za, bar);
+          }
+          if (bmn) {
+            tma_load_pair(sb, mb, b_row, kx, zb, bar);
+            tma_load_pair(sb + 8192, mb, b_row + 64, kx, zb, bar);
+          } else {
+            tma_load_pair(sb, mb, kx, b_row, zb, bar);
+          }
+        }
+      }
+      if (!ok && rank == 0)  // copies still in flight write this pair's shared memory
+        for (uint32_t j = kt < uint32_t(S) ? 0 : kt - S; j < kt; ++j)
+          wait_bar(&full[j % S], (j / S) & 1u, status);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (first CTA) ----------------
+    if (rank == 0 && lane == 0) {
+      uint32_t kt = 0, round = 0;
+      bool ok = true;
+      for (Sequence<TALL> t(g, pair, pairs); t.valid() && ok; t.next(), ++round) {
+        const uint32_t buf = round & 1u;
+        if (round >= 2 && !wait_bar(&tempty[buf], ((round >> 1) & 1u) ^ 1u, status)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * 256u;
+        const int k_len = t.k_len(), num_k = (k_len + kBlockK - 1) / kBlockK;
+        const bool amn = t.a_mn(), bmn = t.b_mn();
+        const uint32_t idesc = g.idesc | (uint32_t(amn) << 15) | (uint32_t(bmn) << 16);
+        const uint64_t stepa = amn ? 2048 / 16 : 32 / 16, stepb = bmn ? 2048 / 16 : 32 / 16;
+        for (int kb = 0; kb < num_k; ++kb, ++kt) {
+          const int s = int(kt % S);
+          if (!wait_bar(&full[s], (kt / S) & 1u, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint8_t* sa = smem + size_t(s) * C::STAGE;
+          const uint8_t* sb = sa + C::A_BYTES;
+          const uint64_t da = amn ? sw128_desc_mn(sa) : sw128_desc(sa);
+          const uint64_t db = bmn ? sw128_desc_mn(sb) : sw128_desc(sb);
+          const int left = k_len - kb * kBlockK;
+          const int slabs = left >= kBlockK ? kBlockK / 16 : (left + 15) / 16;
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 16; ++kk) {
+            if (kk >= slabs) break;
+            mma_pair(acc, da + uint64_t(kk) * stepa, db + uint64_t(kk) * stepb, idesc,
+                     (kb | kk) ? 1u : 0u);
+          }
+          commit_pair(&empty[s]);
+        }
+        if (ok) commit_pair(&tfull[buf]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue ----------------
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    float* stage = epi + (warp - 4) * 16 * kEpiLd;
+    uint32_t round = 0;
+    const float inv = 1.f / g.scale;
+    const uint32_t done0 = addr_in(done, 0), done1 = addr_in(done, 1);
+    for (Sequence<TALL> t(g, pair, pairs); t.valid(); t.next(), ++round) {
+      const int row_base = t.tm * kTileM + int(rank) * 128 + q * 32;
+      const int col0 = t.tn * 256 + half * 128;
+      const bool last = t.phase == 2 && t.step + 1 == g.steps;
+      const bool mirror = t.phase < 2 && t.tm > t.tn;
+      const float* cf = g.coef + 3 * t.step;
+      Piece pc;
+      __half* sq = g.sq + int64_t(pair) * 2 * g.s_plane;
+      pc.c = sq, pc.ldc = g.lds, pc.c_plane = 0;
+      pc.alpha = inv, pc.beta = 0.f;
+      pc.out = sq, pc.ldo = g.lds, pc.out_plane = 0;
+      pc.rows = pc.n = g.s;
+      if (t.phase == 1) {
+        pc.alpha = cf[2] * inv, pc.beta = cf[1];
+        pc.out = sq + g.s_plane;
+      } else if (t.phase == 2) {
+        pc.beta = cf[0];
+        pc.c = t.step == 0 ? g.x0 + int64_t(t.matrix) * g.x_plane
+                           : g.x + (int64_t(pair) * 2 + ((t.step - 1) & 1)) * g.x_plane;
+        pc.ldc = g.ldx;
+        pc.out = g.x + (int64_t(pair) * 2 + (t.step & 1)) * g.x_plane;
+        pc.ldo = g.ldx;
+        pc.rows = g.m, pc.n = g.n;
+        if (last) {
+          pc.alpha *= inv, pc.beta *= inv;
+          pc.out = static_cast<char*>(g.out) +
+                   int64_t(t.matrix) * g.out_stride * (g.out_type == LINALG_FP32 ? 4 : 2);
+          pc.ldo = g.ldo;
+          pc.out_type = g.out_type, pc.out_vec = g.out_vec;
+          pc.decay = g.decay, pc.rate = g.rate;
+        }
+      }
+      const uint32_t buf = round & 1u;
+      // C was written by this very thread, one step (or phase) ago
+      uint32_t cw[2][1][16];
+      load_c<kPlanes, false>(pc, row_base + lane, col0, cw[0]);
+      if (!wait_bar(&tfull[buf], (round >> 1) & 1u, status)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * 256u + uint32_t(half * 128) + (uint32_t(q * 32) << 16);
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        if (cc + 1 < 4)
+          load_c<kPlanes, false>(pc, row_base + lane, col0 + cc * 32 + 32, cw[(cc + 1) & 1]);
+        float v[32];
+        tmem_ld32(acc + uint32_t(cc * 32), v);
+        if (!last)
+          finish_piece<kPlanes, false>(pc, v, lane, row_base, col0 + cc * 32, cw[cc & 1], mirror,
+                                       stage);
+        else
+          finish_piece<LAST, false>(pc, v, lane, row_base, col0 + cc * 32, cw[cc & 1], false,
+                                    stage);
+      }
+      tc_fence_before();
+      if (!last) asm volatile("fence.proxy.async;" ::: "memory");  // read next by TMA
+      __syncwarp();
+      if (lane == 0) {
+        arrive_leader(leader_addr(&tempty[buf]));
+        __threadfence();
+        add_release(done0 + (t.number & 3) * 4);
+        add_release(done1 + (t.number & 3) * 4);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(uint32_t(C::TMEM_COLS))
+                 : "memory");
+  }
+}
+
+int64_t blocks(int64_t v) { return (v + 255) / 256; }
+
+template <bool TALL, int LAST>
+int launch(const CUtensorMap (&maps)[5], const FusedArgs& g, int pairs, cudaStream_t q) {
+  return chol::status_from(chol::launch_pdl(
+      fused_kernel<TALL, LAST>, dim3(unsigned(2 * pairs)), dim3(kThreads), C::SMEM, q, true,
+      maps[0], maps[1], maps[2], maps[3], maps[4], g, chol::device_status_ptr()));
+}
+
+}  // namespace
+
+int fused_pairs(int64_t batch) {
+  const int64_t most = sm_count() / 2;
+  return int(batch < most ? batch : most);
+}
+
+// Whether one pair per matrix is the shorter way, by a count of K blocks (512 cycles of MMAs):
+// here every pair runs its matrices' tiles alone, with an exposed chain per phase when a phase is
+// one tile; product by product the tiles of the batch spread over all pairs, at ~6 us (20 blocks)
+// per launch for its start, first tile and last epilogue.
+bool fused_better(int64_t batch, int64_t m, int64_t n) {
+  const int64_t s = m < n ? m : n;
+  if (s <= 128 || m > 4096 || n > 4096) return false;
+  const int64_t pairs = sm_count() / 2;
+  const int64_t bs = blocks(s), lower = bs * (bs + 1) / 2, all = blocks(m) * blocks(n);
+  const int64_t ks = (s + 63) / 64, kl = ((m < n ? n : m) + 63) / 64;
+  const int64_t chain = bs == 1 ? 30 : 8;  // blocks' worth of waiting per step
+  const int64_t fused = ((batch + pairs - 1) / pairs) * (lower * kl + lower * ks + all * ks + chain);
+  auto waves = [&](int64_t tiles) { return (tiles * batch + pairs - 1) / pairs; };
+  const int64_t apart = waves(lower) * kl + waves(lower) * ks + waves(all) * ks + 3 * 20;
+  return fused <= apart;
+}
+
+int launch_fused(const FusedCall& f, cudaStream_t q) {
+  FusedArgs g{};
+  const bool tall = f.m > f.n;
+  const int pairs = fused_pairs(f.batch);
+  g.m = int(f.m), g.n = int(f.n), g.s = int(tall ? f.n : f.m), g.batch = int(f.batch);
+  g.tiles_m = int(blocks(f.m)), g.tiles_n = int(blocks(f.n)), g.tiles_s = int(blocks(g.s));
+  g.steps = f.steps;
+  g.x0 = static_cast<const __half*>(f.x0);
+  g.x = static_cast<__half*>(f.x);
+  g.sq = static_cast<__half*>(f.squares);
+  g.ldx = f.ldx, g.lds = f.lds, g.x_plane = f.x_plane, g.s_plane = f.s_plane;
+  g.scale = f.scale;
+  g.out = f.out, g.ldo = f.ldo, g.out_stride = f.out_stride, g.out_type = f.out_type;
+  const int sector = f.out_type == LINALG_FP32 ? 8 : 16;
+  g.out_vec = (reinterpret_cast<uintptr_t>(f.out) & 31) == 0 && f.ldo % sector == 0 &&
+              f.out_stride % sector == 0;
+  g.decay = f.decay, g.rate = f.rate;
+  g.idesc = (1u << 4) | (32u << 17) | (16u << 24);  // fp16, FP32 sums, 256 x 256
+  for (int i = 0; i < 3 * f.steps; ++i) g.coef[i] = f.coefficients[i];
+  CUtensorMap maps[5];
+  const int64_t two = 2 * pairs;
+  if (!make_operand_map(&maps[0], Operand{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, false}, false, 128) ||
+      !make_operand_map(&maps[1], Operand{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, true}, false, 0) ||
+      !make_operand_map(&maps[2], Operand{f.x, f.m, f.n, f.ldx, two, f.x_plane, false}, false, 128) ||
+      !make_operand_map(&maps[3], Operand{f.x, f.m, f.n, f.ldx, two, f.x_plane, true}, false, 0) ||
+      !make_operand_map(&maps[4], Operand{f.squares, g.s, g.s, f.lds, two, f.s_plane, false}, false, 128))
+    return CHOL_ERR_UNSUPPORTED;
+  if (f.muon)
+    return tall ? launch<true, kMuon>(maps, g, pairs, q) : launch<false, kMuon>(maps, g, pairs, q);
+  return tall ? launch<true, kFinal>(maps, g, pairs, q) : launch<false, kFinal>(maps, g, pairs, q);
+}
+
+template <bool TALL, int LAST>
+cudaError_t set_fused() {
+  return cudaFuncSetAttribute(fused_kernel<TALL, LAST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              int(C::SMEM));
+}
+
+cudaError_t prepare_fused() {
+  cudaError_t e;
+  if ((e = set_fused<false, kFinal>()) != cudaSuccess) return e;
+  if ((e = set_fused<true, kFinal>()) != cudaSuccess) return e;
+  if ((e = set_fused<false, kMuon>()) != cudaSuccess) return e;
+  return set_fused<true, kMuon>();
+}
+
+}  // namespace lin

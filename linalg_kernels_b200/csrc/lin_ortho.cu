@@ -24,6 +24,7 @@
 #include <mutex>
 
 #include "lin_elem.cuh"
+#include "lin_fused.cuh"
 #include "lin_small.cuh"
 
 namespace lin {
@@ -145,6 +146,8 @@ size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
 struct Layout {
   int64_t planes, ldx, lds, side, x_plane, s_plane;
   size_t x_bytes, s_bytes, sums_bytes, total;
+  bool fused;             // one launch: start values, then X and squares per pair
+  size_t px_bytes, ps_bytes;
 };
 
 Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
@@ -159,7 +162,14 @@ Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   l.x_bytes = round256(size_t(batch) * l.planes * l.x_plane * 2);
   l.s_bytes = round256(size_t(batch) * l.planes * l.s_plane * 2);
   l.sums_bytes = round256(size_t(batch) * kMaxParts * sizeof(double));
-  l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
+  l.fused = !split && fused_better(batch, m, n);
+  if (l.fused) {
+    l.px_bytes = round256(size_t(fused_pairs(batch)) * 2 * l.x_plane * 2);
+    l.ps_bytes = round256(size_t(fused_pairs(batch)) * 2 * l.s_plane * 2);
+    l.total = l.x_bytes + l.px_bytes + l.ps_bytes + l.sums_bytes;
+  } else {
+    l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
+  }
   return l;
 }
 
@@ -226,7 +236,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   if (parts > cap) parts = cap;
   if (parts > kMaxParts) parts = kMaxParts;
   p.parts = int(parts < 1 ? 1 : parts);
-  p.sums = reinterpret_cast<double*>(w + 2 * l.x_bytes + 2 * l.s_bytes);
+  p.sums = reinterpret_cast<double*>(w + l.total - l.sums_bytes);
   p.planes = xs[0];
   p.ldx = l.ldx;
   p.scale = scale, p.eps = eps;
@@ -243,6 +253,17 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
               : chol::launch_pdl(scale_kernel<false, false>, grid, block, 0, q, true, p);
   if (e != cudaSuccess) return CHOL_ERR_LAUNCH;
 
+  if (l.fused) {
+    FusedCall f{};
+    f.batch = batch, f.m = m, f.n = n;
+    f.x0 = w, f.x = w + l.x_bytes, f.squares = w + l.x_bytes + l.px_bytes;
+    f.ldx = l.ldx, f.lds = l.lds, f.x_plane = l.x_plane, f.s_plane = l.s_plane;
+    f.scale = scale, f.steps = steps, f.coefficients = coefficients;
+    f.muon = muon;
+    f.out = out->data, f.ldo = out->ld, f.out_stride = out->stride, f.out_type = out->type;
+    f.decay = decay, f.rate = rate;
+    return launch_fused(f, q);
+  }
   const bool tall = m > n;
   const int64_t s = l.side, matrices = batch * l.planes;
   const Operand sq_gram{gram, s, s, l.lds, matrices, l.s_plane, false};
@@ -338,7 +359,8 @@ int prepare_device(int dev) {
       states[dev].status = CHOL_ERR_DEVICE;
       return;
     }
-    if (prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess)
+    if (prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess ||
+        prepare_fused() != cudaSuccess)
       states[dev].status = CHOL_ERR_DEVICE;
     if (prev != dev) cudaSetDevice(prev);
   });

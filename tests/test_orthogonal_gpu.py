@@ -69,7 +69,10 @@ SHAPES = [(1, 128, 128), (3, 64, 64), (2, 256, 256), (1, 512, 512), (2, 200, 328
           # on chip: one matrix or several per tile, split over 2, 4 and 8 CTAs, odd sizes
           (1, 128, 512), (2, 128, 513), (1, 100, 700), (2, 700, 100), (1, 90, 1537), (1, 4096, 128),
           (1, 127, 4096), (5, 1, 3000), (6, 43, 64), (9, 31, 1), (7, 64, 129), (130, 1, 5),
-          (3, 1536, 20)]
+          (3, 1536, 20),
+          # one launch per batch, a CTA pair per matrix: one tile, two blocks, odd edges, both ways
+          (1, 256, 256), (3, 130, 190), (80, 256, 256), (5, 512, 512), (40, 300, 520),
+          (40, 520, 300), (76, 384, 640), (150, 129, 257)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
