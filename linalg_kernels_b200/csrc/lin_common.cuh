@@ -49,11 +49,11 @@ struct Product {
   bool symmetric = false;
   int64_t m = 0, n = 0, k = 0, batch = 1;
   float alpha = 1.f, beta = 0.f;
-  // kBatch, kPlanes: C and the output are fp16 planes; matrix i, plane p at
+  float diag = 0.f;  // kPlanes: added to the diagonal
+  // kPlanes: C and the output are fp16 planes; matrix i, plane p at
   // base + (i * planes + p) * plane elements, rows ldc / ldo apart
   const void* c = nullptr;
   int64_t ldc = 0, c_plane = 0;
-  // kFinal, kMuon (C as planes, the output the caller's) and kStore16
   void* out = nullptr;
   int64_t ldo = 0, out_stride = 0;
   int out_type = 0;  // LINALG_BF16 / LINALG_FP16 / LINALG_FP32

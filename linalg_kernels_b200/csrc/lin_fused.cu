@@ -23,21 +23,17 @@ namespace {
 
 using namespace tile;
 
-using C = Cfg<256>;
+using C = Cfg<256, 2, 0>;
 constexpr int S = C::STAGES;
 
 struct FusedArgs {
   int m, n, s, batch;             // s: the smaller side
   int tiles_m, tiles_n, tiles_s;  // 256-wide blocks of rows, columns, smaller side
   int steps;
-  const __half* x0;  // [batch] start values
-  __half* x;         // [pair][2]
-  __half* sq;        // [pair][2]: G, B
-  int64_t ldx, lds, x_plane, s_plane;
-  float scale;
+  float scale, poly_scale;
   void* out;
   int64_t ldo, out_stride;
-  int out_type, out_vec;
+  int out_type, out_vec, out_boxes;
   float decay, rate;
   uint32_t idesc;  // K-major operands
   float coef[3 * LINALG_MAX_STEPS];
@@ -52,41 +48,32 @@ struct Sequence {
   int before;                                    // number of the first tile of the phase before
   int tm, tn;
   __device__ __forceinline__ Sequence(const FusedArgs& a, int pair, int p)
-      : g(a), matrix(pair), pairs(p), step(0), phase(0), index(0), number(0), before(0) {
+      : g(a), matrix(pair), pairs(p), step(0), phase(0), index(0), number(0), before(0), tm(0), tn(0) {
     count = lower();
-    place();
   }
   __device__ __forceinline__ int lower() const { return g.tiles_s * (g.tiles_s + 1) / 2; }
   __device__ __forceinline__ bool valid() const { return matrix < g.batch; }
-  __device__ __forceinline__ void place() {
-    if (phase < 2) {
-      tm = int((sqrtf(8.f * float(index) + 1.f) - 1.f) * 0.5f);
-      while (tm * (tm + 1) / 2 > index) --tm;
-      while ((tm + 1) * (tm + 2) / 2 <= index) ++tm;
-      tn = index - tm * (tm + 1) / 2;
-    } else if (TALL) {  // by columns: the first need only B's first rows
-      tn = index / g.tiles_m;
-      tm = index - tn * g.tiles_m;
-    } else {
-      tm = index / g.tiles_n;
-      tn = index - tm * g.tiles_n;
-    }
-  }
   __device__ __forceinline__ void next() {
     ++number;
-    if (++index == count) {
-      before = number - count;
-      index = 0;
-      if (++phase == 3) {
-        phase = 0;
-        if (++step == g.steps) {
-          step = 0;
-          matrix += pairs;
-        }
+    if (++index < count) {  // lower triangle by rows; X by rows, or by columns when tall (the first
+                            // then need only B's first rows)
+      if (TALL && phase == 2) {
+        if (++tm == g.tiles_m) tm = 0, ++tn;
+      } else if (++tn == (phase < 2 ? tm + 1 : g.tiles_n)) {
+        tn = 0, ++tm;
       }
-      count = phase < 2 ? lower() : g.tiles_m * g.tiles_n;
+      return;
     }
-    place();
+    before = number - count;
+    index = tm = tn = 0;
+    if (++phase == 3) {
+      phase = 0;
+      if (++step == g.steps) {
+        step = 0;
+        matrix += pairs;
+      }
+    }
+    count = phase < 2 ? lower() : g.tiles_m * g.tiles_n;
   }
   // Number of the last tile that this one reads from the phase before it; -1: none.
   __device__ __forceinline__ int needs() const {
@@ -126,17 +113,22 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                  const __grid_constant__ CUtensorMap x0_cols,
                  const __grid_constant__ CUtensorMap x_rows,
                  const __grid_constant__ CUtensorMap x_cols,
-                 const __grid_constant__ CUtensorMap squares, const FusedArgs g, int* status) {
+                 const __grid_constant__ CUtensorMap squares,
+                 const __grid_constant__ CUtensorMap x_out,
+                 const __grid_constant__ CUtensorMap squares_out,
+                 const __grid_constant__ CUtensorMap squares_mirror,
+                 const __grid_constant__ CUtensorMap result, const FusedArgs g, int* status) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  float* epi = reinterpret_cast<float*>(smem + size_t(S) * C::STAGE);
+  uint8_t* epi = smem + size_t(S) * C::STAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(S) * C::STAGE + C::EPI);
   uint64_t* full = bars;           // [S] first CTA: a stage of both CTAs has landed
   uint64_t* empty = bars + S;      // [S] the MMAs have read the stage
   uint64_t* tfull = bars + 2 * S;  // [2] accumulator ready
   uint64_t* tempty = tfull + 2;    // [2] first CTA: accumulator drained by both CTAs
-  uint32_t* done = reinterpret_cast<uint32_t*>(tempty + 2);  // [4] finished tiles, by number mod 4
+  uint64_t* c_bars = tempty + 2;   // [2 * kEpiWarps] C's boxes
+  uint32_t* done = reinterpret_cast<uint32_t*>(c_bars + 2 * kEpiWarps);  // [4] finished tiles, by number mod 4
   uint32_t* tmem_slot = done + 4;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -150,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 2 * kEpiWarps);
     }
+    for (int b = 0; b < 2 * kEpiWarps; ++b) mbar_init(&c_bars[b], 1);
     for (int i = 0; i < 4; ++i) done[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&x0_rows);
@@ -289,72 +282,105 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
     const int q = warp & 3, half = (warp - 4) >> 2;
-    float* stage = epi + (warp - 4) * 16 * kEpiLd;
+    using Epi = WarpEpilogue<128, 2, false>;
+    Epi ep{epi + (warp - 4) * 2 * kBoxBytes, c_bars + 2 * (warp - 4), 0u, lane};
     uint32_t round = 0;
     const float inv = 1.f / g.scale;
     const uint32_t done0 = addr_in(done, 0), done1 = addr_in(done, 1);
+    int reported = 0;  // tiles reported as finished
+    // Reports the next unreported tile; `newer`: stores issued since that may still be in flight.
+    auto report = [&](int newer) {
+      if (lane == 0) {
+        if (newer == 0)
+          boxes_written();
+        else if (newer == 1)
+          asm volatile("cp.async.bulk.wait_group 1;" ::: "memory");
+        else
+          asm volatile("cp.async.bulk.wait_group 2;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+        add_release(done0 + (reported & 3) * 4);
+        add_release(done1 + (reported & 3) * 4);
+      }
+      ++reported;
+    };
     for (Sequence<TALL> t(g, pair, pairs); t.valid(); t.next(), ++round) {
       const int row_base = t.tm * kTileM + int(rank) * 128 + q * 32;
       const int col0 = t.tn * 256 + half * 128;
       const bool last = t.phase == 2 && t.step + 1 == g.steps;
       const bool mirror = t.phase < 2 && t.tm > t.tn;
       const float* cf = g.coef + 3 * t.step;
-      Piece pc;
-      __half* sq = g.sq + int64_t(pair) * 2 * g.s_plane;
-      pc.c = sq, pc.ldc = g.lds, pc.c_plane = 0;
-      pc.alpha = inv, pc.beta = 0.f;
-      pc.out = sq, pc.ldo = g.lds, pc.out_plane = 0;
-      pc.rows = pc.n = g.s;
+      Out o;
+      o.alpha = inv, o.beta = 0.f, o.diag = 0.f;
+      o.rows = o.n = g.s;
+      o.map = o.c_map = &squares_out, o.mirror = &squares_mirror;
+      o.z = o.z_c = pair * 2;
+      o.y = 0;
+      o.boxes = 2;
+      o.type = LINALG_FP16;
+      o.weights = 0;
       if (t.phase == 1) {
-        pc.alpha = cf[2] * inv, pc.beta = cf[1];
-        pc.out = sq + g.s_plane;
+        o.alpha = cf[2] * inv * inv * g.poly_scale, o.beta = cf[1] * inv * g.poly_scale;
+        o.diag = cf[0] * g.poly_scale;
+        o.z = pair * 2 + 1;
       } else if (t.phase == 2) {
-        pc.beta = cf[0];
-        pc.c = t.step == 0 ? g.x0 + int64_t(t.matrix) * g.x_plane
-                           : g.x + (int64_t(pair) * 2 + ((t.step - 1) & 1)) * g.x_plane;
-        pc.ldc = g.ldx;
-        pc.out = g.x + (int64_t(pair) * 2 + (t.step & 1)) * g.x_plane;
-        pc.ldo = g.ldx;
-        pc.rows = g.m, pc.n = g.n;
+        o.alpha = 1.f / g.poly_scale;
+        o.rows = g.m, o.n = g.n;
+        o.map = &x_out;
+        o.z = pair * 2 + (t.step & 1);
         if (last) {
-          pc.alpha *= inv, pc.beta *= inv;
-          pc.out = static_cast<char*>(g.out) +
-                   int64_t(t.matrix) * g.out_stride * (g.out_type == LINALG_FP32 ? 4 : 2);
-          pc.ldo = g.ldo;
-          pc.out_type = g.out_type, pc.out_vec = g.out_vec;
-          pc.decay = g.decay, pc.rate = g.rate;
+          o.alpha *= inv;
+          o.map = &result;
+          o.z = t.matrix;
+          o.boxes = LAST == kMuon ? 0 : g.out_boxes;
+          o.out = static_cast<char*>(g.out) +
+                  int64_t(t.matrix) * g.out_stride * (g.out_type == LINALG_FP32 ? 4 : 2);
+          o.ldo = g.ldo, o.type = g.out_type, o.vec = g.out_vec;
+          o.weights = LAST == kMuon, o.decay = g.decay, o.rate = g.rate;
         }
       }
       const uint32_t buf = round & 1u;
-      // C was written by this very thread, one step (or phase) ago
-      uint32_t cw[2][1][16];
-      load_c<kPlanes, false>(pc, row_base + lane, col0, cw[0]);
-      if (!wait_bar(&tfull[buf], (round >> 1) & 1u, status)) break;
+      // The tile before this one is reported once its boxes are in memory: now, if this tile's
+      // accumulator is still to come (it may depend on that report); else behind the first box.
+      if (reported < t.number) {
+        const bool ready = __shfl_sync(0xffffffffu, try_wait_cluster(&tfull[buf], (round >> 1) & 1u), 0);
+        if (!ready) report(0);
+      }
+      // C (G's tile) was stored by this very warp, one phase ago, and reported
+      ep.load_c(o, row_base, col0);
+      bool ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256u + uint32_t(half * 128) + (uint32_t(q * 32) << 16);
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        if (cc + 1 < 4)
-          load_c<kPlanes, false>(pc, row_base + lane, col0 + cc * 32 + 32, cw[(cc + 1) & 1]);
-        float v[32];
-        tmem_ld32(acc + uint32_t(cc * 32), v);
-        if (!last)
-          finish_piece<kPlanes, false>(pc, v, lane, row_base, col0 + cc * 32, cw[cc & 1], mirror,
-                                       stage);
-        else
-          finish_piece<LAST, false>(pc, v, lane, row_base, col0 + cc * 32, cw[cc & 1], false,
-                                    stage);
+      auto get = [&](int c, float (&v)[32]) { tmem_ld32(acc + uint32_t(c), v); };
+      if (!last || ep.by_box(o, row_base)) {
+#pragma unroll 1
+        for (int b = 0; b < Epi::BOXES; ++b) {
+          if (!last)
+            ok = ep.template box<true>(o, b, row_base, col0 + b * 64, mirror, status,
+                                       [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); }) && ok;
+          else
+            ok = ep.template box<false>(o, b, row_base, col0 + b * 64, false, status,
+                                        [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); }) && ok;
+          if (b == 0 && reported < t.number) {
+            const bool stored = col0 < o.n && row_base < o.rows;
+            report(!stored ? 0 : (mirror ? 2 : 1));
+          }
+        }
+        if (!ok) break;
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          get(c, v);
+          ep.direct(o, row_base, col0 + c, v);
+        }
+        if (reported < t.number) report(0);
       }
       tc_fence_before();
-      if (!last) asm volatile("fence.proxy.async;" ::: "memory");  // read next by TMA
       __syncwarp();
-      if (lane == 0) {
-        arrive_leader(leader_addr(&tempty[buf]));
-        __threadfence();
-        add_release(done0 + (t.number & 3) * 4);
-        add_release(done1 + (t.number & 3) * 4);
-      }
+      if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
     }
+    if (lane == 0) boxes_written();
   }
   tc_fence_before();
   __syncthreads();
@@ -370,10 +396,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 int64_t blocks(int64_t v) { return (v + 255) / 256; }
 
 template <bool TALL, int LAST>
-int launch(const CUtensorMap (&maps)[5], const FusedArgs& g, int pairs, cudaStream_t q) {
+int launch(const CUtensorMap (&maps)[9], const FusedArgs& g, int pairs, cudaStream_t q) {
   return chol::status_from(chol::launch_pdl(
       fused_kernel<TALL, LAST>, dim3(unsigned(2 * pairs)), dim3(kThreads), C::SMEM, q, true,
-      maps[0], maps[1], maps[2], maps[3], maps[4], g, chol::device_status_ptr()));
+      maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], maps[8], g, chol::device_status_ptr()));
 }
 
 }  // namespace
@@ -407,11 +433,7 @@ int launch_fused(const FusedCall& f, cudaStream_t q) {
   g.m = int(f.m), g.n = int(f.n), g.s = int(tall ? f.n : f.m), g.batch = int(f.batch);
   g.tiles_m = int(blocks(f.m)), g.tiles_n = int(blocks(f.n)), g.tiles_s = int(blocks(g.s));
   g.steps = f.steps;
-  g.x0 = static_cast<const __half*>(f.x0);
-  g.x = static_cast<__half*>(f.x);
-  g.sq = static_cast<__half*>(f.squares);
-  g.ldx = f.ldx, g.lds = f.lds, g.x_plane = f.x_plane, g.s_plane = f.s_plane;
-  g.scale = f.scale;
+  g.scale = f.scale, g.poly_scale = f.poly_scale;
   g.out = f.out, g.ldo = f.ldo, g.out_stride = f.out_stride, g.out_type = f.out_type;
   const int sector = f.out_type == LINALG_FP32 ? 8 : 16;
   g.out_vec = (reinterpret_cast<uintptr_t>(f.out) & 31) == 0 && f.ldo % sector == 0 &&
@@ -419,14 +441,23 @@ int launch_fused(const FusedCall& f, cudaStream_t q) {
   g.decay = f.decay, g.rate = f.rate;
   g.idesc = (1u << 4) | (32u << 17) | (16u << 24);  // fp16, FP32 sums, 256 x 256
   for (int i = 0; i < 3 * f.steps; ++i) g.coef[i] = f.coefficients[i];
-  CUtensorMap maps[5];
+  CUtensorMap maps[9];
   const int64_t two = 2 * pairs;
-  if (!make_operand_map(&maps[0], Operand{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, false}, false, 128) ||
-      !make_operand_map(&maps[1], Operand{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, true}, false, 0) ||
-      !make_operand_map(&maps[2], Operand{f.x, f.m, f.n, f.ldx, two, f.x_plane, false}, false, 128) ||
-      !make_operand_map(&maps[3], Operand{f.x, f.m, f.n, f.ldx, two, f.x_plane, true}, false, 0) ||
-      !make_operand_map(&maps[4], Operand{f.squares, g.s, g.s, f.lds, two, f.s_plane, false}, false, 128))
+  const Operand x0{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, false};
+  const Operand x{f.x, f.m, f.n, f.ldx, two, f.x_plane, false};
+  const Operand sq{f.squares, g.s, g.s, f.lds, two, f.s_plane, false};
+  Operand x0_mn = x0, x_mn = x;
+  x0_mn.mn_major = x_mn.mn_major = true;
+  if (!make_operand_map(&maps[0], x0, false, 128) || !make_operand_map(&maps[1], x0_mn, false, 0) ||
+      !make_operand_map(&maps[2], x, false, 128) || !make_operand_map(&maps[3], x_mn, false, 0) ||
+      !make_operand_map(&maps[4], sq, false, 128) || !make_output_map(&maps[5], x, false, false) ||
+      !make_output_map(&maps[6], sq, false, false) || !make_output_map(&maps[7], sq, false, true))
     return CHOL_ERR_UNSUPPORTED;
+  maps[8] = maps[5];
+  if (!f.muon && f.out_type != LINALG_FP32 &&
+      make_output_map(&maps[8], Operand{f.out, f.m, f.n, f.ldo, f.batch, f.out_stride, false},
+                      f.out_type == LINALG_BF16, false))
+    g.out_boxes = 2;
   if (f.muon)
     return tall ? launch<true, kMuon>(maps, g, pairs, q) : launch<false, kMuon>(maps, g, pairs, q);
   return tall ? launch<true, kFinal>(maps, g, pairs, q) : launch<false, kFinal>(maps, g, pairs, q);

@@ -20,11 +20,8 @@
 //                CTA's part of the last block has landed, zeroes the slab's rows that belong to
 //                the next group (they may hold anything, NaN included). (Passing every stage
 //                through this warp cost the weight gradient of 16384 rows 398 us, against XXX.)
-//   warps 4..11  epilogue, overlapped with the next tile (two accumulators): a lane holds 32
-//                columns of one row and reads C and writes the result in 32-byte accesses
-//                straight from registers. (Staging the tile through shared memory for coalesced
-//                rows took the bandwidth the operands need, and C loaded where it is used left
-//                each piece waiting for L2: b640n512 4.80 ms, against XXX ms.)
+//   warps 4..11  epilogue, overlapped with the next tile (two accumulators): TMEM -> registers ->
+//                boxes in shared memory -> TMA stores (lin_tile.cuh).
 //
 // The grid is persistent: one pair per two SMs, tiles round-robin. Groups' sizes are read from
 // device memory by every CTA, so the host needs no synchronisation.
@@ -62,20 +59,31 @@ bool resolve_encode() {
 
 }  // namespace
 
-bool make_operand_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows) {
+namespace {
+bool encode(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_cols, uint32_t box_rows,
+            CUtensorMapSwizzle swizzle) {
   if (!resolve_encode()) return false;
   if ((reinterpret_cast<uintptr_t>(o.base) & 15) || o.ld % 8 || (o.count > 1 && o.stride % 8))
     return false;
   cuuint64_t dims[3] = {cuuint64_t(o.cols), cuuint64_t(o.rows), cuuint64_t(o.count)};
   cuuint64_t strides[2] = {cuuint64_t(o.ld) * 2,
                            cuuint64_t(o.count > 1 ? o.stride : o.ld * o.rows) * 2};
-  cuuint32_t box[3] = {cuuint32_t(tile::kBlockK), cuuint32_t(o.mn_major ? tile::kBlockK : box_rows), 1};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return g_encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void*>(o.base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace
+
+bool make_operand_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows) {
+  return encode(map, o, bf16, tile::kBlockK, o.mn_major ? tile::kBlockK : box_rows,
+                CU_TENSOR_MAP_SWIZZLE_128B);
+}
+bool make_output_map(CUtensorMap* map, const Operand& o, bool bf16, bool mirrored) {
+  return mirrored ? encode(map, o, bf16, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE)
+                  : encode(map, o, bf16, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 namespace {
@@ -88,9 +96,8 @@ struct Args {
   int m, n, k, batch;
   int tiles_m, tiles_n, per_matrix;
   int symmetric;
-  float alpha, beta;
-  const __half* c;
-  int64_t ldc, c_plane;
+  float alpha, beta, diag;
+  int boxes;  // the output through boxes: 1 inside the rows of a group only, 2 everywhere
   void* out;
   int64_t ldo, out_stride;
   int out_type;
@@ -170,16 +177,25 @@ struct Walker {
   }
 };
 
+// Epilogue buffers per warp: two hold C's boxes (and the two planes) of a batch's products; ragged
+// products have no C and need the group tables' space.
+template <int BN, int MODE>
+using ProductCfg = Cfg<BN, MODE == kBatch || BN == 128 ? 2 : 1, MODE == kBatch ? 0 : kTableBytes>;
+
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a,
-                   const __grid_constant__ CUtensorMap map_b, const Args g, int* status) {
-  using C = Cfg<BN>;
+                   const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out,
+                   const __grid_constant__ CUtensorMap map_mirror,
+                   const __grid_constant__ CUtensorMap map_c, const Args g, int* status) {
+  using C = ProductCfg<BN, MODE>;
   constexpr int S = C::STAGES;
+  constexpr int kBufs = MODE == kBatch || BN == 128 ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  float* epi = reinterpret_cast<float*>(smem + size_t(S) * C::STAGE);
+  uint8_t* epi = smem + size_t(S) * C::STAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(S) * C::STAGE + C::EPI);
   uint64_t* full = bars;             // [S] first CTA: a stage of both CTAs has landed
   uint64_t* landed = bars + S;       // [S] kRaggedK: this CTA's part of a group's last block landed
@@ -187,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* tfull = bars + 3 * S;    // [2] accumulator ready
   uint64_t* tempty = tfull + 2;      // [2] first CTA: accumulator drained by both CTAs
   uint64_t* clean = tempty + 2;      // [S] kRaggedK, first CTA: the other CTA's part is clean
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(clean + S);
+  uint64_t* c_bars = clean + S;      // [2 * kEpiWarps] C's boxes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_bars + 2 * kEpiWarps);
   int* start = reinterpret_cast<int*>(smem + size_t(S) * C::STAGE + C::EPI + 512);
   int* first = start + kMaxGroups + 4;
 
@@ -204,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 2 * kEpiWarps);
     }
+    for (int b = 0; b < 2 * kEpiWarps; ++b) mbar_init(&c_bars[b], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&map_a);
     prefetch_map(&map_b);
@@ -423,44 +441,57 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; half of the columns
-    float* tile = epi + (warp - 4) * 16 * kEpiLd;
-    constexpr int kCols = BN / 2, kChunks = kCols / 32;
+    constexpr int kCols = BN / 2;
+    using Epi = WarpEpilogue<kCols, kBufs, SPLIT>;
+    Epi ep{epi + (warp - 4) * kBufs * kBoxBytes, c_bars + 2 * (warp - 4), 0u, lane};
     uint32_t round = 0;
+    constexpr int P = SPLIT ? 2 : 1;
+    Out o;
+    o.alpha = g.alpha, o.beta = EPI == kPlanes ? g.beta : 0.f, o.diag = EPI == kPlanes ? g.diag : 0.f;
+    o.n = g.n;
+    o.map = &map_out, o.mirror = &map_mirror, o.c_map = &map_c;
+    o.boxes = EPI == kMuon ? 0 : g.boxes;
+    o.ldo = g.ldo, o.type = EPI == kPlanes ? LINALG_FP16 : g.out_type, o.vec = g.out_vec;
+    o.weights = EPI == kMuon, o.decay = g.decay, o.rate = g.rate;
     for (int t = pair; t < total; t += pairs) {
       walk.at(t, w);
       const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
       const int row_base = w.tm * kTileM + int(rank) * 128 + q * 32;  // within the matrix or group
       const int col0 = w.tn * BN + half * kCols;
       const bool mirror = EPI == kPlanes && g.symmetric && w.tm * kTileM > w.tn * BN + BN - 1;
-
-      constexpr int P = SPLIT ? 2 : 1;
-      Piece pc;
-      pc.c = g.c + int64_t(w.index) * P * g.c_plane;
-      pc.ldc = g.ldc, pc.c_plane = g.c_plane;
-      pc.alpha = g.alpha, pc.beta = g.beta;
+      o.rows = w.rows;
+      o.z = MODE == kRaggedM ? 0 : w.index * (EPI == kPlanes ? P : 1);
+      o.z_c = w.index * P;
+      o.y = w.row0;
       const int size = EPI != kPlanes && g.out_type == LINALG_FP32 ? 4 : 2;
-      pc.out = static_cast<char*>(g.out) +
-               (int64_t(MODE == kRaggedM ? 0 : w.index) * (EPI == kPlanes ? P : 1) * g.out_stride +
-                int64_t(w.row0) * g.ldo) * size;
-      pc.ldo = g.ldo, pc.out_plane = g.out_stride;
-      pc.out_type = g.out_type;
-      pc.out_vec = g.out_vec;
-      pc.decay = g.decay, pc.rate = g.rate;
-      pc.rows = w.rows, pc.n = g.n;
+      o.out = static_cast<char*>(g.out) + (int64_t(MODE == kRaggedM ? 0 : w.index) * g.out_stride +
+                                           int64_t(w.row0) * g.ldo) * size;
+      constexpr bool kC = EPI == kPlanes;  // C, the diagonal, mirrored tiles
+      const bool by_box = ep.by_box(o, row_base);
       if (num_k == 0) {  // nothing to sum: zeros (rows of no group, a group without rows)
-        const uint32_t none[P][16] = {};
-#pragma unroll 1
-        for (int cc = 0; cc < kChunks; ++cc) {
-          float v[32];
+        auto zeros = [](int, float (&v)[32]) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
-          finish_piece<EPI, SPLIT>(pc, v, lane, row_base, col0 + cc * 32, none, false, tile);
+        };
+#pragma unroll 1
+        for (int c = 0; c < kCols; c += 64) {
+          if (by_box) {
+            ep.template box<false>(o, c / 64, row_base, col0 + c, false, status, zeros);
+          } else {
+#pragma unroll 1
+            for (int h = 0; h < 64; h += 32) {
+              float v[32];
+              zeros(0, v);
+              ep.direct(o, row_base, col0 + c + h, v);
+            }
+          }
         }
         continue;
       }
       bool ok = true;
-      if (SPLIT) {
-        float sum[kChunks][32];
+      if (kC) ep.load_c(o, row_base, col0);
+      if constexpr (SPLIT) {
+        float sum[2][32];
         const int chunks = (num_k + kChunk - 1) / kChunk;
         for (int ch = 0; ch < chunks; ++ch, ++round) {
           const uint32_t buf = round & 1u;
@@ -470,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +
                                (uint32_t(q * 32) << 16);
 #pragma unroll
-          for (int cc = 0; cc < kChunks; ++cc) {
+          for (int cc = 0; cc < 2; ++cc) {
             float v[32];
             tmem_ld32(acc + uint32_t(cc * 32), v);
 #pragma unroll
@@ -480,28 +511,39 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           __syncwarp();
           if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
         }
-        if (!ok) break;
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if constexpr (kC) {
+          ok = ep.template box<kC>(o, 0, row_base, col0, mirror, status, [&](int h, float (&v)[32]) {
 #pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc) {
-          uint32_t cw[P][16];
-          load_c<EPI, SPLIT>(pc, row_base + lane, col0 + cc * 32, cw);
-          finish_piece<EPI, SPLIT>(pc, sum[cc], lane, row_base, col0 + cc * 32, cw, mirror, tile);
+            for (int j = 0; j < 32; ++j) v[j] = sum[h][j];
+          });
+        } else {
+          ep.direct(o, row_base, col0, sum[0]);
+          ep.direct(o, row_base, col0 + 32, sum[1]);
         }
+        if (!ok) break;
       } else {
         const uint32_t buf = round & 1u;
-        uint32_t cw[2][P][16];
-        load_c<EPI, SPLIT>(pc, row_base + lane, col0, cw[0]);
-        if (!wait_bar(&tfull[buf], (round >> 1) & 1u, status)) break;
+        ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +
                              (uint32_t(q * 32) << 16);
-#pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc) {
-          if (cc + 1 < kChunks)
-            load_c<EPI, SPLIT>(pc, row_base + lane, col0 + cc * 32 + 32, cw[(cc + 1) & 1]);
-          float v[32];
-          tmem_ld32(acc + uint32_t(cc * 32), v);
-          finish_piece<EPI, SPLIT>(pc, v, lane, row_base, col0 + cc * 32, cw[cc & 1], mirror, tile);
+        if (by_box) {
+#pragma unroll 1
+          for (int b = 0; b < Epi::BOXES; ++b)
+            ok = ep.template box<kC>(o, b, row_base, col0 + b * 64, mirror, status,
+                                     [&](int h, float (&v)[32]) {
+                                       tmem_ld32(acc + uint32_t(b * 64 + h * 32), v);
+                                     }) && ok;
+          if (!ok) break;
+        } else if constexpr (!kC) {
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 32) {
+            float v[32];
+            tmem_ld32(acc + uint32_t(c), v);
+            ep.direct(o, row_base, col0 + c, v);
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -509,6 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         ++round;
       }
     }
+    if (lane == 0) boxes_written();  // they read this CTA's shared memory
   }
   // The other CTA's barriers and shared memory are used until both are done.
   tc_fence_before();
@@ -528,7 +571,8 @@ int g_sms = 148;
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 cudaError_t set_smem() {
   return cudaFuncSetAttribute(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<BN>::SMEM));
+                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              int(ProductCfg<BN, MODE>::SMEM));
 }
 
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
@@ -554,14 +598,28 @@ int launch(const Product& p, cudaStream_t q) {
   if (per > 0x7fffffffLL || total > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;
   if (total == 0) return CHOL_OK;
   g.per_matrix = int(per);
-  g.alpha = p.alpha, g.beta = p.beta;
-  g.c = static_cast<const __half*>(p.c);
-  g.ldc = p.ldc, g.c_plane = p.c_plane;
+  g.alpha = p.alpha, g.beta = p.beta, g.diag = p.diag;
   g.out = p.out;
   g.ldo = p.ldo, g.out_stride = p.out_stride, g.out_type = p.out_type;
   const int sector = p.out_type == LINALG_FP32 ? 8 : 16;
   g.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % sector == 0 &&
               p.out_stride % sector == 0;
+  // the output's boxes, where its type and alignment allow: by group rows when these are ragged
+  CUtensorMap mo = ma, mm = ma, mc = ma;
+  if (EPI == kPlanes || (EPI != kMuon && p.out_type != LINALG_FP32)) {
+    const int64_t planes = EPI == kPlanes && SPLIT ? 2 : 1;
+    const Operand out{p.out, MODE == kRaggedM ? p.total_rows : p.m, p.n, p.ldo,
+                      MODE == kRaggedM ? 1 : p.batch * planes, p.out_stride, false};
+    const bool b16 = EPI != kPlanes && p.out_type == LINALG_BF16;
+    if ((EPI == kPlanes || !SPLIT) && make_output_map(&mo, out, b16, false))
+      g.boxes = MODE == kRaggedM ? 1 : 2;
+    if (EPI == kPlanes && (!g.boxes || !make_output_map(&mm, out, false, true)))
+      return CHOL_ERR_UNSUPPORTED;
+    if (EPI == kPlanes && p.beta != 0.f &&
+        !make_output_map(&mc, Operand{p.c, p.m, p.n, p.ldc, p.batch * planes, p.c_plane, false},
+                         false, false))
+      return CHOL_ERR_UNSUPPORTED;
+  }
   g.decay = p.decay, g.rate = p.rate;
   g.offsets = p.offsets, g.offsets64 = p.offsets64;
   g.total_rows = int(p.total_rows), g.fill = p.fill;
@@ -572,8 +630,8 @@ int launch(const Product& p, cudaStream_t q) {
   if (pairs > total) pairs = total;
   return chol::status_from(chol::launch_pdl(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
                                             dim3(unsigned(2 * pairs)), dim3(kThreads),
-                                            Cfg<BN>::SMEM, q, true, ma, mb, g,
-                                            chol::device_status_ptr()));
+                                            ProductCfg<BN, MODE>::SMEM, q, true, ma, mb, mo, mm,
+                                            mc, g, chol::device_status_ptr()));
 }
 
 // BN = 256 wherever the tiles still fill the GPU: the wider tile moves a third less shared

@@ -1,13 +1,16 @@
 // lin_ortho.cu — Newton-Schulz orthogonalisation of a batch of matrices, alone and inside the
 // optimiser step around it.
 //
-//   X = u / (||u||_F + eps);  per step  G = X X^T,  B = b G + c G G,  X <- a X + B X
+//   X = u / (||u||_F + eps);  per step  G = X X^T,  B = a I + b G + c G G,  X <- B X
 //
-// (from the right, G = X^T X, X <- a X + X B, when the matrices are taller than wide, so G is
+// (from the right, G = X^T X, X <- X B, when the matrices are taller than wide, so G is
 // always the smaller square). One step is three products of lin_gemm.cu: G and B are
 // symmetric, so only the tiles on and below the diagonal are computed and each is written twice.
 // Per step 3 m^2 n + m^3 multiply-adds (m the smaller side) instead of the full products'
 // 4 m^2 n + 2 m^3.
+//
+// a stands on B's diagonal, so that the third product reads no old X: one more rounding per row, of
+// the size of X's own.
 //
 // Number format: X, G and B are fp16, scaled by a power of two, and not bf16: |X|, |G| <= ~1.3
 // and |B| <= ~3, so fp16's range is enough, and its 11 bits make each rounding 8 times smaller
@@ -220,8 +223,9 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   __half* gram = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
   __half* poly = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
   const bool muon = momentum != nullptr;
-  // the largest entries, ~3 in B, stay a factor 5 (full) to 20 (half) under fp16's largest
-  const float scale = split ? 4096.f : 1024.f;
+  // X and G: entries up to ~1.3, a factor 12 (full) to 50 (half) under fp16's largest; B, with a
+  // on its diagonal, up to ~4: a factor 8 to 16
+  const float scale = split ? 4096.f : 1024.f, poly_scale = split ? 2048.f : 1024.f;
 
   Prep p{};
   p.x = device_matrix(x);
@@ -258,7 +262,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     f.batch = batch, f.m = m, f.n = n;
     f.x0 = w, f.x = w + l.x_bytes, f.squares = w + l.x_bytes + l.px_bytes;
     f.ldx = l.ldx, f.lds = l.lds, f.x_plane = l.x_plane, f.s_plane = l.s_plane;
-    f.scale = scale, f.steps = steps, f.coefficients = coefficients;
+    f.scale = scale, f.poly_scale = poly_scale, f.steps = steps, f.coefficients = coefficients;
     f.muon = muon;
     f.out = out->data, f.ldo = out->ld, f.out_stride = out->stride, f.out_type = out->type;
     f.decay = decay, f.rate = rate;
@@ -283,29 +287,29 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     g.out = gram, g.ldo = l.lds, g.out_stride = l.s_plane;
     int st = launch_product(g, q);
     if (st != CHOL_OK) return st;
-    Product f;  // B = b G + c G G
+    Product f;  // B = a I + b G + c G G
     f.a = f.b = sq_gram;
     f.epilogue = kPlanes;
     f.split = split;
     f.symmetric = true;
     f.m = f.n = f.k = s, f.batch = batch;
-    f.alpha = c / scale, f.beta = b;
+    f.alpha = c * (poly_scale / (scale * scale)), f.beta = b * (poly_scale / scale);
     f.c = gram, f.ldc = l.lds, f.c_plane = l.s_plane;
+    f.diag = a * poly_scale;
     f.out = poly, f.ldo = l.lds, f.out_stride = l.s_plane;
     if ((st = launch_product(f, q)) != CHOL_OK) return st;
-    Product u;  // X <- a X + B X or a X + X B
+    Product u;  // X <- B X or X B
     u.a = tall ? rows_x : sq_poly;
     u.b = tall ? sq_poly : cols_x;
     u.split = split;
     u.m = m, u.n = n, u.k = s, u.batch = batch;
-    u.alpha = 1.f / scale, u.beta = a;
-    u.c = cur, u.ldc = l.ldx, u.c_plane = l.x_plane;
+    u.alpha = 1.f / poly_scale;
     if (k + 1 < steps) {
       u.epilogue = kPlanes;
       u.out = xs[(k + 1) & 1], u.ldo = l.ldx, u.out_stride = l.x_plane;
     } else {
       u.epilogue = muon ? kMuon : kFinal;
-      u.alpha /= scale, u.beta /= scale;
+      u.alpha /= scale;
       u.out = out->data, u.ldo = out->ld, u.out_stride = out->stride, u.out_type = out->type;
       u.decay = decay, u.rate = rate;
     }

@@ -12,6 +12,8 @@ namespace lin {
 
 // Tensor map of an operand; boxes of 64 columns x box_rows (64 x 64 when MN-major). (lin_gemm.cu)
 bool make_operand_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows);
+// Map of an output's (or C's) boxes: 64 columns x 32 rows, or 32 x 64 unswizzled for mirrored ones.
+bool make_output_map(CUtensorMap* map, const Operand& o, bool bf16, bool mirrored);
 
 namespace tile {
 
@@ -26,17 +28,22 @@ constexpr int kEpiWarps = 8;
 constexpr int kEpiLd = 33;      // staging row stride in floats: conflict-free by row and by column
 constexpr int kChunk = 4;       // split: K blocks per drained accumulator
 
-template <int BN>
+constexpr int kBoxBytes = 32 * 128;  // one warp's 32 rows x 64 columns of 16 bits
+
+// BUFS: boxes of staging per epilogue warp. TABLE: bytes for the group tables.
+template <int BN, int BUFS, int TABLE_BYTES>
 struct Cfg {
-  static constexpr int STAGES = BN == 256 ? 6 : 8;
+  static constexpr int STAGES = BN == 256 ? 5 : 6;
   static constexpr int A_BYTES = 128 * kBlockK * 2;
   static constexpr int B_BYTES = BN / 2 * kBlockK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int EPI = kEpiWarps * 16 * kEpiLd * 4;  // half a piece per warp
-  static constexpr int TABLE = 2 * (kMaxGroups + 4) * 4;  // group starts and first tiles
+  static constexpr int EPI = kEpiWarps * BUFS * kBoxBytes;
+  static constexpr int TABLE = TABLE_BYTES;
   static constexpr size_t SMEM = size_t(STAGES) * STAGE + EPI + 512 + TABLE + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
+constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // group starts and first tiles
 
 // ------------------------------- device helpers ---------------------------------------
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -190,119 +197,57 @@ __device__ __forceinline__ void write_one(T* p, float v, bool weights, float dec
   *p = from_float<T>(v);
 }
 
-// What a warp does with a 32 x 32 piece of accumulators (a lane holds 32 columns of one row):
-// alpha * acc + beta * C, to the output. All pointers are those of one matrix (or group).
-struct Piece {
-  const __half* c;  // fp16 plane(s), rows ldc apart; 32-byte aligned rows
-  int64_t ldc, c_plane;
-  float alpha, beta;
-  void* out;  // kPlanes: plane 0, rows on 32-byte boundaries; else the caller's element (0, 0)
-  int64_t ldo, out_plane;
-  int out_type, out_vec;  // out_vec: rows of the caller's matrix start on 32-byte boundaries
-  float decay, rate;      // kMuon
-  int rows, n;            // rows and columns of the output
+// What an epilogue warp does with its accumulators (a lane holds columns of one row):
+// alpha * acc (+ beta * C) (+ diag on the diagonal), to the output. Results and C pass through
+// shared memory in boxes of 32 rows x 64 columns that TMA copies: a lane's own 32-byte accesses
+// reach half a sector a cycle per SM, 4096 cycles for a 128 x 256 half tile, and took longer
+// than its MMAs (b640n512 3.4 ms).
+struct Out {
+  float alpha, beta, diag;
+  int rows, n;  // rows and columns of the output
+  // boxes (TMA): plane p of the output at z + p; C likewise; `y`: row 0's coordinate
+  const CUtensorMap *map, *mirror, *c_map;
+  int z, z_c, y;
+  int boxes;  // the output is written by boxes (else, and where a box would pass the rows: below)
+  // the caller's matrix, any alignment
+  void* out;
+  int64_t ldo;
+  int type, vec;  // vec: rows start on 32-byte boundaries
+  int weights;    // out <- decay * out - rate * value
+  float decay, rate;
 };
 
-// C of one piece, this lane's row (whole pieces only; loaded ahead of their use).
-template <int EPI, bool SPLIT>
-__device__ __forceinline__ void load_c(const Piece& g, int row, int gc0,
-                                       uint32_t (&cw)[SPLIT ? 2 : 1][16]) {
-  if (EPI == kStore16 || g.beta == 0.f || row >= g.rows || gc0 + 32 > g.n) return;
-  const __half* cp = g.c + int64_t(row) * g.ldc + gc0;
-#pragma unroll
-  for (int p = 0; p < (SPLIT ? 2 : 1); ++p) {
-    ldg32(cp + p * g.c_plane, cw[p]);
-    ldg32(cp + p * g.c_plane + 16, cw[p] + 8);
-  }
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const void* src, int x, int y,
+                                          int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's box stores have read shared memory / have written global memory.
+__device__ __forceinline__ void boxes_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void boxes_written() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+// 16-byte chunk c of row r of a box (128-byte rows, 128-byte swizzle).
+__device__ __forceinline__ uint4* box_chunk(uint8_t* box, int r, int c) {
+  return reinterpret_cast<uint4*>(box + r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// `mirror`: a symmetric result's tile below the diagonal is written to its transposed place too.
-// `stage`: 16 rows of kEpiLd floats of this warp's own.
-template <int EPI, bool SPLIT>
-__device__ __forceinline__ void finish_piece(const Piece& g, float (&v)[32], int lane, int row_base,
-                                             int gc0, const uint32_t (&cw)[SPLIT ? 2 : 1][16],
-                                             bool mirror, float* stage) {
-  constexpr int P = SPLIT ? 2 : 1;
-  if (gc0 >= g.n || row_base >= g.rows) return;
+// 32 columns of this lane's row straight to the caller's matrix.
+template <typename T>
+__device__ __forceinline__ void write_direct(const Out& g, float (&v)[32], int lane, int row_base,
+                                             int gc0, float* stage) {
   const int row = row_base + lane;
   const int cols = g.n - gc0 < 32 ? g.n - gc0 : 32;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] *= g.alpha;
-  if (EPI != kStore16 && g.beta != 0.f) {
-    if (cols == 32) {
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float c0, c1;
-          unpack<__half>(cw[p][j], c0, c1);
-          v[2 * j] = fmaf(g.beta, c0, v[2 * j]);
-          v[2 * j + 1] = fmaf(g.beta, c1, v[2 * j + 1]);
-        }
-    } else if (row < g.rows) {
-      const __half* cp = g.c + int64_t(row) * g.ldc + gc0;
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < cols)
-          for (int p = 0; p < P; ++p)
-            v[j] = fmaf(g.beta, __half2float(cp[p * g.c_plane + j]), v[j]);
-    }
-  }
-  if (EPI == kPlanes) {
-    // rows of the workspace are padded to whole 32-byte sectors
-    __half* o = static_cast<__half*>(g.out);
-#pragma unroll
-    for (int p = 0; p < P; ++p, o += g.out_plane) {
-      uint32_t h[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) h[j] = pack<__half>(v[2 * j], v[2 * j + 1]);
-      if (row < g.rows) {
-        __half* q0 = o + int64_t(row) * g.ldo + gc0;
-        if (cols == 32) {
-          stg32(q0, h);
-          stg32(q0 + 16, h + 8);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)  // the pad after an odd last column exists
-            if (2 * j < cols) reinterpret_cast<uint32_t*>(q0)[j] = h[j];
-        }
-      }
-      if (mirror) {
-        // the transposed piece (its columns all exist): neighbouring lanes exchange halves, so that
-        // an even lane writes column 2j and an odd one column 2j + 1 of two rows
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, h[j], 1);
-          const uint32_t two = (lane & 1) ? __byte_perm(other, h[j], 0x7632)
-                                          : __byte_perm(h[j], other, 0x5410);
-          const int r = row & ~1;
-          if (r < g.rows)
-            *reinterpret_cast<uint32_t*>(o + int64_t(gc0 + 2 * j + (lane & 1)) * g.ldo + r) = two;
-        }
-      }
-      if (SPLIT && p == 0) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float c0, c1;
-          unpack<__half>(h[j], c0, c1);
-          v[2 * j] -= c0;
-          v[2 * j + 1] -= c1;
-        }
-      }
-    }
-    return;
-  }
-  constexpr bool kWeights = EPI == kMuon;
-  if (cols == 32 && g.out_vec) {
-    if (row < g.rows) {
-      const int64_t at = int64_t(row) * g.ldo + gc0;
-      if (g.out_type == LINALG_BF16)
-        write_row(static_cast<__nv_bfloat16*>(g.out) + at, v, kWeights, g.decay, g.rate);
-      else if (g.out_type == LINALG_FP16)
-        write_row(static_cast<__half*>(g.out) + at, v, kWeights, g.decay, g.rate);
-      else if (EPI != kStore16)
-        write_row(static_cast<float*>(g.out) + at, v, kWeights, g.decay, g.rate);
-    }
+  T* out = static_cast<T*>(g.out);
+  if (cols == 32 && g.vec) {
+    if (row < g.rows)
+      write_row(out + int64_t(row) * g.ldo + gc0, v, g.weights, g.decay, g.rate);
     return;
   }
   // rows that do not start on sectors, or the last columns: through shared memory, half a piece at
@@ -317,20 +262,188 @@ __device__ __forceinline__ void finish_piece(const Piece& g, float (&v)[32], int
     const int left = g.rows - row_base - h, rows = left < 16 ? left : 16;
     if (lane < cols) {
 #pragma unroll 4
-      for (int r = 0; r < rows; ++r) {
-        const float x = stage[r * kEpiLd + lane];
-        const int64_t at = int64_t(row_base + h + r) * g.ldo + gc0 + lane;
-        if (g.out_type == LINALG_BF16)
-          write_one(static_cast<__nv_bfloat16*>(g.out) + at, x, kWeights, g.decay, g.rate);
-        else if (g.out_type == LINALG_FP16)
-          write_one(static_cast<__half*>(g.out) + at, x, kWeights, g.decay, g.rate);
-        else if (EPI != kStore16)
-          write_one(static_cast<float*>(g.out) + at, x, kWeights, g.decay, g.rate);
-      }
+      for (int r = 0; r < rows; ++r)
+        write_one(out + int64_t(row_base + h + r) * g.ldo + gc0 + lane, stage[r * kEpiLd + lane],
+                  g.weights, g.decay, g.rate);
     }
     __syncwarp();
   }
 }
+
+// The epilogue of one warp's 32 rows x COLS columns (a multiple of 64).
+template <int COLS, int BUFS, bool SPLIT>
+struct WarpEpilogue {
+  static constexpr int P = SPLIT ? 2 : 1;
+  static constexpr int BOXES = COLS / 64;
+  static_assert(!SPLIT || (BOXES == 1 && BUFS == 2), "planes take a buffer each");
+  uint8_t* bufs;        // BUFS boxes of this warp, 1024-byte aligned
+  uint64_t* c_bar;      // [2] this warp's
+  uint32_t c_phase;     // bit b: parity of the next wait on c_bar[b]
+  int lane;
+
+  __device__ __forceinline__ uint8_t* buf(int b) const { return bufs + (b % BUFS) * kBoxBytes; }
+
+  // C's boxes, ahead of the accumulator (needs a buffer per box).
+  __device__ __forceinline__ void load_c(const Out& g, int row_base, int col0) {
+    if (g.beta == 0.f) return;
+    if (lane == 0) {
+      boxes_read();
+#pragma unroll
+      for (int b = 0; b < (SPLIT ? 2 : BOXES); ++b) {
+        mbar_expect_tx(&c_bar[b], kBoxBytes);
+        tma_load_3d(buf(b), g.c_map, col0 + (SPLIT ? 0 : b * 64), g.y + row_base,
+                    g.z_c + (SPLIT ? b : 0), &c_bar[b]);
+      }
+    }
+  }
+  // Waits for what load_c asked for.
+  __device__ __forceinline__ bool wait_c(const Out& g, int b, int* status) {
+    if (g.beta == 0.f) return true;
+    const bool ok = mbar_wait(&c_bar[b], c_phase >> b & 1u, status);
+    c_phase ^= 1u << b;
+    return __all_sync(0xffffffffu, ok);
+  }
+
+  // Whether this warp's rows go out by boxes.
+  __device__ __forceinline__ bool by_box(const Out& g, int row_base) const {
+    return g.boxes && (g.boxes == 2 || row_base + 32 <= g.rows);
+  }
+
+  // One box (64 columns from gc0): get(h, v) gives accumulators of columns 32 h .. 32 h + 31. The
+  // caller keeps this the only code between a tile's barriers: it runs from the instruction cache.
+  template <bool HAS_C, typename Get>
+  __device__ __forceinline__ bool box(const Out& g, int b, int row_base, int gc0, bool mirror,
+                                      int* status, const Get& get) {
+    bool ok = true;
+    if (HAS_C) {
+      ok = wait_c(g, b, status);
+      if (SPLIT) ok = wait_c(g, 1, status) && ok;
+      if (!ok) return false;
+    }
+    if (gc0 >= g.n || row_base >= g.rows) return true;
+    const bool with_c = HAS_C && g.beta != 0.f;
+    if (!with_c) {
+      if (lane == 0) boxes_read();
+      __syncwarp();
+    }
+    uint8_t* hi = buf(b);
+    uint8_t* lo = SPLIT ? buf(1) : nullptr;
+    uint32_t packed[32];
+    uint32_t packed_lo[SPLIT ? 32 : 1];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[32];
+      get(h, v);
+      const float2 alpha = make_float2(g.alpha, g.alpha), beta = make_float2(g.beta, g.beta);
+      if (with_c) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 w = *box_chunk(hi, lane, h * 4 + c);
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+          uint4 wl = make_uint4(0, 0, 0, 0);
+          if (SPLIT) wl = *box_chunk(lo, lane, h * 4 + c);
+          const uint32_t wls[4] = {wl.x, wl.y, wl.z, wl.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2 x = __half22float2(*reinterpret_cast<const __half2*>(&ws[e]));
+            if (SPLIT) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&wls[e]));
+              x.x += y.x;  // exact: hi + lo has 22 bits
+              x.y += y.y;
+            }
+            float* p = v + c * 8 + 2 * e;
+            const float2 t = chol::ffma2(beta, x, make_float2(0.f, 0.f));
+            const float2 r = chol::ffma2(alpha, make_float2(p[0], p[1]), t);
+            p[0] = r.x;
+            p[1] = r.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 r = chol::ffma2(alpha, make_float2(v[j], v[j + 1]), make_float2(0.f, 0.f));
+          v[j] = r.x;
+          v[j + 1] = r.y;
+        }
+      }
+      if (HAS_C && g.diag != 0.f && gc0 + 32 * h == row_base) {  // the same for the whole warp
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += j == lane ? g.diag : 0.f;
+      }
+      if (!HAS_C && g.type == LINALG_BF16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          packed[h * 16 + j] = pack<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          packed[h * 16 + j] = pack<__half>(v[2 * j], v[2 * j + 1]);
+          if (SPLIT) {
+            float c0, c1;
+            unpack<__half>(packed[h * 16 + j], c0, c1);
+            packed_lo[SPLIT ? h * 16 + j : 0] = pack<__half>(v[2 * j] - c0, v[2 * j + 1] - c1);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int o = h * 16 + c * 4;
+        *box_chunk(hi, lane, h * 4 + c) =
+            make_uint4(packed[o], packed[o + 1], packed[o + 2], packed[o + 3]);
+        if (SPLIT)
+          *box_chunk(lo, lane, h * 4 + c) =
+              make_uint4(packed_lo[SPLIT ? o : 0], packed_lo[SPLIT ? o + 1 : 0],
+                         packed_lo[SPLIT ? o + 2 : 0], packed_lo[SPLIT ? o + 3 : 0]);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      store_box(g.map, hi, gc0, g.y + row_base, g.z);
+      if (SPLIT) store_box(g.map, lo, gc0, g.y + row_base, g.z + 1);
+    }
+    if (HAS_C && mirror) {
+      // the transposed box, 64 rows of 64 bytes: neighbouring lanes exchange halves, so that an
+      // even lane writes row 2j and an odd one row 2j + 1, two columns each
+      if (lane == 0) boxes_read();
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        uint32_t* t = reinterpret_cast<uint32_t*>(p ? lo : hi);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const uint32_t own = p ? packed_lo[SPLIT ? j : 0] : packed[j];
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+          t[(2 * j + (lane & 1)) * 16 + (lane >> 1)] = (lane & 1) ? __byte_perm(other, own, 0x7632)
+                                                                  : __byte_perm(own, other, 0x5410);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        store_box(g.mirror, hi, row_base, gc0, g.z);
+        if (SPLIT) store_box(g.mirror, lo, row_base, gc0, g.z + 1);
+      }
+    }
+    return true;
+  }
+
+  // 32 columns from gc0 straight to the caller's matrix.
+  __device__ __forceinline__ void direct(const Out& g, int row_base, int gc0, float (&v)[32]) {
+    if (gc0 >= g.n || row_base >= g.rows) return;
+    if (lane == 0) boxes_read();
+    __syncwarp();
+    float* stage = reinterpret_cast<float*>(bufs);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= g.alpha;
+    if (g.type == LINALG_BF16)
+      write_direct<__nv_bfloat16>(g, v, lane, row_base, gc0, stage);
+    else if (g.type == LINALG_FP16)
+      write_direct<__half>(g, v, lane, row_base, gc0, stage);
+    else
+      write_direct<float>(g, v, lane, row_base, gc0, stage);
+  }
+};
 
 }  // namespace tile
 }  // namespace lin
