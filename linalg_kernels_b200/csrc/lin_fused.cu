@@ -30,7 +30,10 @@ struct FusedArgs {
   int m, n, s, batch;             // s: the smaller side
   int tiles_m, tiles_n, tiles_s;  // 256-wide blocks of rows, columns, smaller side
   int steps;
-  float scale, poly_scale;
+  __half* x;         // [pair][2]
+  __half* sq;        // [pair][2]: G, B
+  int64_t ldx, lds, x_plane, s_plane;
+  float scale;
   void* out;
   int64_t ldo, out_stride;
   int out_type, out_vec, out_boxes;
@@ -97,8 +100,8 @@ __device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
   asm volatile("ld.acquire.cluster.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
   return v;
 }
-__device__ __forceinline__ void add_release(uint32_t cluster_addr) {
-  asm volatile("red.release.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_addr), "r"(1u)
+__device__ __forceinline__ void add_relaxed(uint32_t cluster_addr) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_addr), "r"(1u)
                : "memory");
 }
 __device__ __forceinline__ uint32_t addr_in(const void* p, uint32_t rank) {
@@ -114,9 +117,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                  const __grid_constant__ CUtensorMap x_rows,
                  const __grid_constant__ CUtensorMap x_cols,
                  const __grid_constant__ CUtensorMap squares,
-                 const __grid_constant__ CUtensorMap x_out,
-                 const __grid_constant__ CUtensorMap squares_out,
-                 const __grid_constant__ CUtensorMap squares_mirror,
                  const __grid_constant__ CUtensorMap result, const FusedArgs g, int* status) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -285,24 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     using Epi = WarpEpilogue<128, 2, false>;
     Epi ep{epi + (warp - 4) * 2 * kBoxBytes, c_bars + 2 * (warp - 4), 0u, lane};
     uint32_t round = 0;
-    const float inv = 1.f / g.scale;
+    const float x_inv = 1.f / g.scale, g_inv = x_inv * x_inv;  // scales: X, G its square, B 1
     const uint32_t done0 = addr_in(done, 0), done1 = addr_in(done, 1);
-    int reported = 0;  // tiles reported as finished
-    // Reports the next unreported tile; `newer`: stores issued since that may still be in flight.
-    auto report = [&](int newer) {
-      if (lane == 0) {
-        if (newer == 0)
-          boxes_written();
-        else if (newer == 1)
-          asm volatile("cp.async.bulk.wait_group 1;" ::: "memory");
-        else
-          asm volatile("cp.async.bulk.wait_group 2;" ::: "memory");
-        asm volatile("fence.proxy.async;" ::: "memory");
-        add_release(done0 + (reported & 3) * 4);
-        add_release(done1 + (reported & 3) * 4);
-      }
-      ++reported;
-    };
     for (Sequence<TALL> t(g, pair, pairs); t.valid(); t.next(), ++round) {
       const int row_base = t.tm * kTileM + int(rank) * 128 + q * 32;
       const int col0 = t.tn * 256 + half * 128;
@@ -310,28 +294,27 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       const bool mirror = t.phase < 2 && t.tm > t.tn;
       const float* cf = g.coef + 3 * t.step;
       Out o;
-      o.alpha = inv, o.beta = 0.f, o.diag = 0.f;
+      o.alpha = 1.f, o.beta = 0.f, o.diag = 0.f;
       o.rows = o.n = g.s;
-      o.map = o.c_map = &squares_out, o.mirror = &squares_mirror;
-      o.z = o.z_c = pair * 2;
+      o.map = &result;
+      o.z = t.matrix;
       o.y = 0;
-      o.boxes = 2;
+      o.boxes = LAST == kMuon ? 0 : g.out_boxes;
       o.type = LINALG_FP16;
       o.weights = 0;
+      o.ldo = g.lds;
+      __half* sq = g.sq + int64_t(pair) * 2 * g.s_plane;  // G, then B
+      __half* to = sq;
       if (t.phase == 1) {
-        o.alpha = cf[2] * inv * inv * g.poly_scale, o.beta = cf[1] * inv * g.poly_scale;
-        o.diag = cf[0] * g.poly_scale;
-        o.z = pair * 2 + 1;
+        o.alpha = cf[2] * g_inv * g_inv, o.beta = cf[1] * g_inv;
+        o.diag = cf[0];
+        to = sq + g.s_plane;
       } else if (t.phase == 2) {
-        o.alpha = 1.f / g.poly_scale;
         o.rows = g.m, o.n = g.n;
-        o.map = &x_out;
-        o.z = pair * 2 + (t.step & 1);
+        o.ldo = g.ldx;
+        to = g.x + (int64_t(pair) * 2 + (t.step & 1)) * g.x_plane;
         if (last) {
-          o.alpha *= inv;
-          o.map = &result;
-          o.z = t.matrix;
-          o.boxes = LAST == kMuon ? 0 : g.out_boxes;
+          o.alpha = x_inv;
           o.out = static_cast<char*>(g.out) +
                   int64_t(t.matrix) * g.out_stride * (g.out_type == LINALG_FP32 ? 4 : 2);
           o.ldo = g.ldo, o.type = g.out_type, o.vec = g.out_vec;
@@ -339,34 +322,30 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
       }
       const uint32_t buf = round & 1u;
-      // The tile before this one is reported once its boxes are in memory: now, if this tile's
-      // accumulator is still to come (it may depend on that report); else behind the first box.
-      if (reported < t.number) {
-        const bool ready = __shfl_sync(0xffffffffu, try_wait_cluster(&tfull[buf], (round >> 1) & 1u), 0);
-        if (!ready) report(0);
-      }
-      // C (G's tile) was stored by this very warp, one phase ago, and reported
-      ep.load_c(o, row_base, col0);
+      // C (G's tile) was written by this very warp, a phase ago
+      uint4 cw[8];
+      if (o.beta != 0.f) ep.fetch_c(o, sq, row_base, col0, cw);
       bool ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256u + uint32_t(half * 128) + (uint32_t(q * 32) << 16);
       auto get = [&](int c, float (&v)[32]) { tmem_ld32(acc + uint32_t(c), v); };
-      if (!last || ep.by_box(o, row_base)) {
+      if (!last) {
+        if (t.index == 0 && t.phase == 0 && t.step == 0) {  // the result's boxes of a matrix before
+          if (lane == 0) boxes_read();
+          __syncwarp();
+        }
 #pragma unroll 1
         for (int b = 0; b < Epi::BOXES; ++b) {
-          if (!last)
-            ok = ep.template box<true>(o, b, row_base, col0 + b * 64, mirror, status,
-                                       [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); }) && ok;
-          else
-            ok = ep.template box<false>(o, b, row_base, col0 + b * 64, false, status,
-                                        [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); }) && ok;
-          if (b == 0 && reported < t.number) {
-            const bool stored = col0 < o.n && row_base < o.rows;
-            report(!stored ? 0 : (mirror ? 2 : 1));
-          }
+          ep.box_now(o, to, b, row_base, col0 + b * 64, mirror, cw,
+                     [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); });
+          if (b == 0 && o.beta != 0.f) ep.fetch_c(o, sq, row_base, col0 + 64, cw);
         }
-        if (!ok) break;
+      } else if (ep.by_box(o, row_base)) {
+#pragma unroll 1
+        for (int b = 0; b < Epi::BOXES; ++b)
+          ep.template box<false>(o, b, row_base, col0 + b * 64, false, status,
+                                 [&](int h, float (&v)[32]) { get(b * 64 + h * 32, v); });
       } else {
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
@@ -374,11 +353,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           get(c, v);
           ep.direct(o, row_base, col0 + c, v);
         }
-        if (reported < t.number) report(0);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
+      if (lane == 0) {
+        arrive_leader_relaxed(leader_addr(&tempty[buf]));
+        __threadfence();  // the warp's stores, before the report
+        add_relaxed(done0 + (t.number & 3) * 4);
+        add_relaxed(done1 + (t.number & 3) * 4);
+      }
     }
     if (lane == 0) boxes_written();
   }
@@ -396,10 +379,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 int64_t blocks(int64_t v) { return (v + 255) / 256; }
 
 template <bool TALL, int LAST>
-int launch(const CUtensorMap (&maps)[9], const FusedArgs& g, int pairs, cudaStream_t q) {
+int launch(const CUtensorMap (&maps)[6], const FusedArgs& g, int pairs, cudaStream_t q) {
   return chol::status_from(chol::launch_pdl(
       fused_kernel<TALL, LAST>, dim3(unsigned(2 * pairs)), dim3(kThreads), C::SMEM, q, true,
-      maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], maps[8], g, chol::device_status_ptr()));
+      maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], g, chol::device_status_ptr()));
 }
 
 }  // namespace
@@ -422,8 +405,12 @@ bool fused_better(int64_t batch, int64_t m, int64_t n) {
   const int64_t chain = bs == 1 ? 30 : 8;  // blocks' worth of waiting per step
   const int64_t fused = ((batch + pairs - 1) / pairs) * (lower * kl + lower * ks + all * ks + chain);
   auto waves = [&](int64_t tiles) { return (tiles * batch + pairs - 1) / pairs; };
-  const int64_t apart = waves(lower) * kl + waves(lower) * ks + waves(all) * ks + 3 * 20;
-  return fused <= apart;
+  int64_t apart = waves(lower) * kl + waves(lower) * ks + waves(all) * ks;
+  // beyond L2 the products stream X four times, G and B twice each through HBM (~1.7 MB a block's time)
+  const int64_t bytes = batch * 2 * (4 * m * n + 4 * s * s);
+  if (batch * 2 * (2 * m * n + 2 * s * s) > (int64_t(100) << 20) && bytes / 1700000 > apart)
+    apart = bytes / 1700000;
+  return fused <= apart + 3 * 20;
 }
 
 int launch_fused(const FusedCall& f, cudaStream_t q) {
@@ -433,7 +420,10 @@ int launch_fused(const FusedCall& f, cudaStream_t q) {
   g.m = int(f.m), g.n = int(f.n), g.s = int(tall ? f.n : f.m), g.batch = int(f.batch);
   g.tiles_m = int(blocks(f.m)), g.tiles_n = int(blocks(f.n)), g.tiles_s = int(blocks(g.s));
   g.steps = f.steps;
-  g.scale = f.scale, g.poly_scale = f.poly_scale;
+  g.x = static_cast<__half*>(f.x);
+  g.sq = static_cast<__half*>(f.squares);
+  g.ldx = f.ldx, g.lds = f.lds, g.x_plane = f.x_plane, g.s_plane = f.s_plane;
+  g.scale = f.scale;
   g.out = f.out, g.ldo = f.ldo, g.out_stride = f.out_stride, g.out_type = f.out_type;
   const int sector = f.out_type == LINALG_FP32 ? 8 : 16;
   g.out_vec = (reinterpret_cast<uintptr_t>(f.out) & 31) == 0 && f.ldo % sector == 0 &&
@@ -441,7 +431,7 @@ int launch_fused(const FusedCall& f, cudaStream_t q) {
   g.decay = f.decay, g.rate = f.rate;
   g.idesc = (1u << 4) | (32u << 17) | (16u << 24);  // fp16, FP32 sums, 256 x 256
   for (int i = 0; i < 3 * f.steps; ++i) g.coef[i] = f.coefficients[i];
-  CUtensorMap maps[9];
+  CUtensorMap maps[6];
   const int64_t two = 2 * pairs;
   const Operand x0{f.x0, f.m, f.n, f.ldx, f.batch, f.x_plane, false};
   const Operand x{f.x, f.m, f.n, f.ldx, two, f.x_plane, false};
@@ -450,12 +440,11 @@ int launch_fused(const FusedCall& f, cudaStream_t q) {
   x0_mn.mn_major = x_mn.mn_major = true;
   if (!make_operand_map(&maps[0], x0, false, 128) || !make_operand_map(&maps[1], x0_mn, false, 0) ||
       !make_operand_map(&maps[2], x, false, 128) || !make_operand_map(&maps[3], x_mn, false, 0) ||
-      !make_operand_map(&maps[4], sq, false, 128) || !make_output_map(&maps[5], x, false, false) ||
-      !make_output_map(&maps[6], sq, false, false) || !make_output_map(&maps[7], sq, false, true))
+      !make_operand_map(&maps[4], sq, false, 128))
     return CHOL_ERR_UNSUPPORTED;
-  maps[8] = maps[5];
+  maps[5] = maps[0];
   if (!f.muon && f.out_type != LINALG_FP32 &&
-      make_output_map(&maps[8], Operand{f.out, f.m, f.n, f.ldo, f.batch, f.out_stride, false},
+      make_output_map(&maps[5], Operand{f.out, f.m, f.n, f.ldo, f.batch, f.out_stride, false},
                       f.out_type == LINALG_BF16, false))
     g.out_boxes = 2;
   if (f.muon)

@@ -11,7 +11,7 @@ struct FusedCall {
   void* x;         // fused_pairs(batch) * 2 such matrices
   void* squares;   // fused_pairs(batch) * 2 squares of the smaller side, rows lds apart
   int64_t ldx, lds, x_plane, s_plane;
-  float scale, poly_scale;  // powers of two on X and G, and on B
+  float scale;     // X's (G has its square, B 1)
   int steps;
   const float* coefficients;
   bool muon;  // out <- decay * out - rate * result, else out <- result

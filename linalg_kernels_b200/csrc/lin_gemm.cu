@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
+          if (lane == 0) arrive_leader_relaxed(leader_addr(&tempty[buf]));
         }
         if (!__all_sync(0xffffffffu, ok)) break;
         if constexpr (kC) {
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_leader(leader_addr(&tempty[buf]));
+        if (lane == 0) arrive_leader_relaxed(leader_addr(&tempty[buf]));
         ++round;
       }
     }

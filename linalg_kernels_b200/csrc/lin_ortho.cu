@@ -223,9 +223,13 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   __half* gram = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
   __half* poly = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
   const bool muon = momentum != nullptr;
-  // X and G: entries up to ~1.3, a factor 12 (full) to 50 (half) under fp16's largest; B, with a
-  // on its diagonal, up to ~4: a factor 8 to 16
-  const float scale = split ? 4096.f : 1024.f, poly_scale = split ? 2048.f : 1024.f;
+  // Scales: X's is a power of two, G's its square (the sums are stored as they are), B's 1 in half
+  // precision. Entries of G up to ~1.3 stay a factor 50 (half) or 12 (full) under fp16's
+  // largest; X's small ones (1 / sqrt(m n) at the start) clear of its subnormals. B, with a
+  // on its diagonal, needs no scale: what its subnormals lose, 3e-8 per entry, is small against
+  // the rounding of its diagonal; the planes of full precision keep 22 bits with 2048.
+  const float scale = split ? 64.f : 32.f, gram_scale = scale * scale;
+  const float poly_scale = split ? 2048.f : 1.f;
 
   Prep p{};
   p.x = device_matrix(x);
@@ -262,7 +266,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     f.batch = batch, f.m = m, f.n = n;
     f.x0 = w, f.x = w + l.x_bytes, f.squares = w + l.x_bytes + l.px_bytes;
     f.ldx = l.ldx, f.lds = l.lds, f.x_plane = l.x_plane, f.s_plane = l.s_plane;
-    f.scale = scale, f.poly_scale = poly_scale, f.steps = steps, f.coefficients = coefficients;
+    f.scale = scale, f.steps = steps, f.coefficients = coefficients;
     f.muon = muon;
     f.out = out->data, f.ldo = out->ld, f.out_stride = out->stride, f.out_type = out->type;
     f.decay = decay, f.rate = rate;
@@ -283,7 +287,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     g.split = split;
     g.symmetric = true;
     g.m = g.n = s, g.k = tall ? m : n, g.batch = batch;
-    g.alpha = 1.f / scale;
+    g.alpha = 1.f;
     g.out = gram, g.ldo = l.lds, g.out_stride = l.s_plane;
     int st = launch_product(g, q);
     if (st != CHOL_OK) return st;
@@ -293,7 +297,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     f.split = split;
     f.symmetric = true;
     f.m = f.n = f.k = s, f.batch = batch;
-    f.alpha = c * (poly_scale / (scale * scale)), f.beta = b * (poly_scale / scale);
+    f.alpha = c * (poly_scale / (gram_scale * gram_scale)), f.beta = b * (poly_scale / gram_scale);
     f.c = gram, f.ldc = l.lds, f.c_plane = l.s_plane;
     f.diag = a * poly_scale;
     f.out = poly, f.ldo = l.lds, f.out_stride = l.s_plane;

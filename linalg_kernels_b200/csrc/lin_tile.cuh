@@ -5,6 +5,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "chol_tc_ptx.cuh"
 #include "lin_common.cuh"
 
@@ -74,6 +76,24 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "memory");
   return ok != 0;
 }
+// Whether the phase has completed, without waiting (try_wait suspends the thread for a while).
+__device__ __forceinline__ bool test_bar(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The same without ordering memory: for a drained accumulator, whose reads tcgen05.wait::ld and
+// tcgen05.fence::before_thread_sync have ordered (a release costs ~1000 cycles here).
+__device__ __forceinline__ void arrive_leader_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
 // Bounded wait at cluster scope.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* status) {
   if (try_wait_cluster(bar, parity)) return true;
@@ -138,13 +158,17 @@ __device__ __forceinline__ void stg32(void* p, const uint32_t* r) {
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// Two values in one word (one instruction).
 template <typename T>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   if constexpr (sizeof(T) == 4) {
     return 0;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-    alignas(4) T h[2] = {from_float<T>(a), from_float<T>(b)};
-    return *reinterpret_cast<const uint32_t*>(h);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
 template <typename T>
@@ -230,6 +254,15 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, const void* sr
 __device__ __forceinline__ void boxes_read() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
+// The same but for the newest `newer` (0, 1 or 2).
+__device__ __forceinline__ void boxes_read_but(int newer) {
+  if (newer == 0)
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  else if (newer == 1)
+    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  else
+    asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+}
 __device__ __forceinline__ void boxes_written() {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
@@ -280,6 +313,7 @@ struct WarpEpilogue {
   uint64_t* c_bar;      // [2] this warp's
   uint32_t c_phase;     // bit b: parity of the next wait on c_bar[b]
   int lane;
+  int newest = 0;       // stores of the box before, which uses the other buffer (if there are two)
 
   __device__ __forceinline__ uint8_t* buf(int b) const { return bufs + (b % BUFS) * kBoxBytes; }
 
@@ -309,27 +343,14 @@ struct WarpEpilogue {
     return g.boxes && (g.boxes == 2 || row_base + 32 <= g.rows);
   }
 
-  // One box (64 columns from gc0): get(h, v) gives accumulators of columns 32 h .. 32 h + 31. The
-  // caller keeps this the only code between a tile's barriers: it runs from the instruction cache.
+  // One box's values, rounded, into its buffer: get(h, v) gives accumulators of columns 32 h ..
+  // 32 h + 31 of this lane's row. with_c: the buffer holds C.
   template <bool HAS_C, typename Get>
-  __device__ __forceinline__ bool box(const Out& g, int b, int row_base, int gc0, bool mirror,
-                                      int* status, const Get& get) {
-    bool ok = true;
-    if (HAS_C) {
-      ok = wait_c(g, b, status);
-      if (SPLIT) ok = wait_c(g, 1, status) && ok;
-      if (!ok) return false;
-    }
-    if (gc0 >= g.n || row_base >= g.rows) return true;
-    const bool with_c = HAS_C && g.beta != 0.f;
-    if (!with_c) {
-      if (lane == 0) boxes_read();
-      __syncwarp();
-    }
+  __device__ __forceinline__ void fill(const Out& g, int b, int row_base, int gc0, bool with_c,
+                                       const Get& get, uint32_t (&packed)[32],
+                                       uint32_t (&packed_lo)[SPLIT ? 32 : 1]) {
     uint8_t* hi = buf(b);
     uint8_t* lo = SPLIT ? buf(1) : nullptr;
-    uint32_t packed[32];
-    uint32_t packed_lo[SPLIT ? 32 : 1];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[32];
@@ -358,7 +379,7 @@ struct WarpEpilogue {
             p[1] = r.y;
           }
         }
-      } else {
+      } else if (g.alpha != 1.f) {
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           const float2 r = chol::ffma2(alpha, make_float2(v[j], v[j + 1]), make_float2(0.f, 0.f));
@@ -396,6 +417,46 @@ struct WarpEpilogue {
                          packed_lo[SPLIT ? o + 2 : 0], packed_lo[SPLIT ? o + 3 : 0]);
       }
     }
+  }
+
+  // The transposed box, 64 rows of 64 bytes, in place of one that has been read: neighbouring lanes
+  // exchange halves, so that an even lane writes row 2j and an odd one row 2j + 1, two columns
+  // each.
+  __device__ __forceinline__ void transpose(uint8_t* box, const uint32_t* packed) {
+    uint32_t* t = reinterpret_cast<uint32_t*>(box);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, packed[j], 1);
+      t[(2 * j + (lane & 1)) * 16 + (lane >> 1)] = (lane & 1)
+                                                       ? __byte_perm(other, packed[j], 0x7632)
+                                                       : __byte_perm(packed[j], other, 0x5410);
+    }
+  }
+
+  // One box (64 columns from gc0) to memory by TMA.
+  template <bool HAS_C, typename Get>
+  __device__ __forceinline__ bool box(const Out& g, int b, int row_base, int gc0, bool mirror,
+                                      int* status, const Get& get) {
+    bool ok = true;
+    if (HAS_C) {
+      ok = wait_c(g, b, status);
+      if (SPLIT) ok = wait_c(g, 1, status) && ok;
+      if (!ok) return false;
+    }
+    if (gc0 >= g.n || row_base >= g.rows) {
+      newest = 0;
+      return true;
+    }
+    const bool with_c = HAS_C && g.beta != 0.f;
+    if (!with_c) {
+      if (lane == 0) boxes_read_but(BUFS == 2 && !SPLIT ? newest : 0);
+      __syncwarp();
+    }
+    newest = mirror ? 2 : 1;
+    uint8_t* hi = buf(b);
+    uint8_t* lo = SPLIT ? buf(1) : nullptr;
+    uint32_t packed[32], packed_lo[SPLIT ? 32 : 1];
+    fill<HAS_C>(g, b, row_base, gc0, with_c, get, packed, packed_lo);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -403,21 +464,10 @@ struct WarpEpilogue {
       if (SPLIT) store_box(g.map, lo, gc0, g.y + row_base, g.z + 1);
     }
     if (HAS_C && mirror) {
-      // the transposed box, 64 rows of 64 bytes: neighbouring lanes exchange halves, so that an
-      // even lane writes row 2j and an odd one row 2j + 1, two columns each
       if (lane == 0) boxes_read();
       __syncwarp();
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        uint32_t* t = reinterpret_cast<uint32_t*>(p ? lo : hi);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const uint32_t own = p ? packed_lo[SPLIT ? j : 0] : packed[j];
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
-          t[(2 * j + (lane & 1)) * 16 + (lane >> 1)] = (lane & 1) ? __byte_perm(other, own, 0x7632)
-                                                                  : __byte_perm(own, other, 0x5410);
-        }
-      }
+      transpose(hi, packed);
+      if (SPLIT) transpose(lo, packed_lo);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -426,6 +476,55 @@ struct WarpEpilogue {
       }
     }
     return true;
+  }
+
+  // The same with the warp's own coalesced accesses, for results that another tile waits for: TMA
+  // works off its queue in order, so a store waits behind the loads that the producer has ahead
+  // (3000 to 8000 cycles until it is complete, against ~1000 here). c, o: plane 0 of the matrix,
+  // fp16, rows of whole 32-byte sectors.
+  __device__ __forceinline__ void fetch_c(const Out& g, const __half* c, int row_base, int gc0,
+                                          uint4 (&w)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row_base + i * 4 + (lane >> 3), col = gc0 + (lane & 7) * 8;
+      if (row < g.rows && col < g.n)
+        w[i] = *reinterpret_cast<const uint4*>(c + int64_t(row) * g.ldo + col);
+    }
+  }
+  template <typename Get>
+  __device__ __forceinline__ void box_now(const Out& g, __half* o, int b, int row_base, int gc0,
+                                          bool mirror, const uint4 (&w)[8], const Get& get) {
+    if (gc0 >= g.n || row_base >= g.rows) return;
+    const bool with_c = g.beta != 0.f;
+    uint8_t* box = buf(b);
+    __syncwarp();  // the box before has been read
+    if (with_c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *box_chunk(box, i * 4 + (lane >> 3), lane & 7) = w[i];
+      __syncwarp();
+    }
+    uint32_t packed[32], none[SPLIT ? 32 : 1];
+    fill<true>(g, b, row_base, gc0, with_c, get, packed, none);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), row = row_base + r, col = gc0 + (lane & 7) * 8;
+      const uint4 x = *box_chunk(box, r, lane & 7);
+      if (row < g.rows && col < g.n)
+        *reinterpret_cast<uint4*>(o + int64_t(row) * g.ldo + col) = x;
+    }
+    if (mirror) {
+      __syncwarp();
+      transpose(box, packed);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 8 + (lane >> 2), row = gc0 + r, col = row_base + (lane & 3) * 8;
+        const uint4 x = *reinterpret_cast<const uint4*>(box + r * 64 + (lane & 3) * 16);
+        if (row < g.n && col < g.rows)
+          *reinterpret_cast<uint4*>(o + int64_t(row) * g.ldo + col) = x;
+      }
+    }
   }
 
   // 32 columns from gc0 straight to the caller's matrix.
