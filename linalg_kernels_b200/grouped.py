@@ -54,32 +54,43 @@ def _check_offsets(offsets, like: torch.Tensor, groups: int | None = None) -> in
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` with contiguous rows that start on 16-byte boundaries (as the bulk copies need), a
     copy with padded rows where it has not."""
-    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and t.stride(-2) % 8 == 0 and
-            t.stride(-2) >= t.shape[-1] and
-            (t.dim() < 3 or (t.stride(0) % 8 == 0 and
-                             t.stride(0) >= t.shape[-1] + (t.shape[-2] - 1) * t.stride(-2)))):
+    shape, stride = t.shape, t.stride()
+    rows, cols, ld = shape[-2], shape[-1], stride[-2]
+    if stride[-1] == 1 and not ld & 7 and ld >= cols and not t.data_ptr() & 15 and (
+            len(shape) < 3 or (not stride[0] & 7 and stride[0] >= cols + (rows - 1) * ld)):
         return t
-    cols = t.shape[-1]
-    padded = t.new_empty(*t.shape[:-1], (cols + 7) // 8 * 8)[..., :cols]
+    padded = t.new_empty(*shape[:-1], (cols + 7) // 8 * 8)[..., :cols]
     return padded.copy_(t)
 
 
-def _matrix(t: torch.Tensor) -> tuple[int, int, int, int]:
-    return t.data_ptr(), t.stride(-2), (t.stride(0) if t.dim() == 3 else 0), _TYPES[t.dtype]
+def _aligned_weights(w: torch.Tensor) -> torch.Tensor:
+    """The same for (groups, k, n) weights, in the order in which they lie in memory."""
+    if _stored_transposed(w):
+        return _aligned(w.transpose(1, 2)).transpose(1, 2)
+    return _aligned(w)
 
 
-def _on_device(t: torch.Tensor, call):
-    if t.device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(t.device):
-        return call()
+def _stored_transposed(w: torch.Tensor) -> bool:
+    return w.stride(1) == 1 and w.stride(2) != 1
+
+
+_call = None  # the binding's (grouped_matmul, grouped_outer), once loaded
+
+
+def _binding():
+    global _call
+    if _call is None:
+        lib = _lib.linalg()
+        _call = lib.grouped_matmul, lib.grouped_outer
+    return _call
 
 
 def _matmul(x, w, offsets, out=None):
+    """x and w aligned (_aligned, _aligned_weights); on x's device."""
     rows, k = x.shape
     groups, _, n = w.shape
     fill = out is None
-    if out is None:
+    if fill:
         out = x.new_empty(rows, n)
     if rows == 0 or n == 0:
         return out
@@ -87,21 +98,20 @@ def _matmul(x, w, offsets, out=None):
         if groups and not fill:
             raise ValueError("out needs k > 0")
         return out.zero_() if fill else out
-    w_rows_k = not (w.stride(1) == 1 and w.stride(2) != 1)
-
-    def call():
-        a = _aligned(x)
-        b = _aligned(w if w_rows_k else w.transpose(1, 2))
-        return _lib.linalg().grouped_matmul(
-            *_matrix(a), *_matrix(b), *_matrix(out), int(w_rows_k), offsets.data_ptr(),
-            int(offsets.dtype == torch.int64), groups, rows, k, n, int(fill),
-            _lib.current_queue(x.device))
-
-    _lib.check(_on_device(x, call), "linalg_grouped_matmul")
+    transposed = _stored_transposed(w)
+    stride = w.stride()
+    kind = _TYPES[x.dtype]
+    status = (_call or _binding())[0](
+        x.data_ptr(), x.stride(0), 0, kind, w.data_ptr(), stride[2 if transposed else 1], stride[0],
+        kind, out.data_ptr(), out.stride(0), 0, kind, not transposed, offsets.data_ptr(),
+        offsets.dtype is torch.int64, groups, rows, k, n, fill, _lib.current_queue(x.device.index))
+    if status:
+        _lib.check(status, "linalg_grouped_matmul")
     return out
 
 
 def _outer(a, b, offsets, groups, out=None):
+    """a and b aligned; on a's device."""
     rows, k = a.shape
     n = b.shape[1]
     if out is None:
@@ -110,32 +120,49 @@ def _outer(a, b, offsets, groups, out=None):
         return out
     if rows == 0:
         return out.zero_()
-
-    def call():
-        p, q = _aligned(a), _aligned(b)
-        return _lib.linalg().grouped_outer(
-            *_matrix(p), *_matrix(q), *_matrix(out), offsets.data_ptr(),
-            int(offsets.dtype == torch.int64), groups, rows, k, n, _lib.current_queue(a.device))
-
-    _lib.check(_on_device(a, call), "linalg_grouped_outer")
+    kind = _TYPES[a.dtype]
+    status = (_call or _binding())[1](
+        a.data_ptr(), a.stride(0), 0, kind, b.data_ptr(), b.stride(0), 0, kind, out.data_ptr(),
+        out.stride(1), out.stride(0), kind, offsets.data_ptr(), offsets.dtype is torch.int64, groups,
+        rows, k, n, _lib.current_queue(a.device.index))
+    if status:
+        _lib.check(status, "linalg_grouped_outer")
     return out
+
+
+_single: bool | None = None
+
+
+def _on_device(t: torch.Tensor, call):
+    """Runs ``call`` with t's device current."""
+    global _single
+    if _single is None:
+        _single = torch.cuda.device_count() == 1
+    if _single or t.device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(t.device):
+        return call()
 
 
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
+        # the aligned operands serve the backward pass too: a copy is made once
+        x, w = _aligned(x), _aligned_weights(w)
         ctx.save_for_backward(x, w, offsets)
         return _matmul(x, w, offsets)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
+    def backward(ctx, dy):  # (autograd has made the device current)
         x, w, offsets = ctx.saved_tensors
+        need = ctx.needs_input_grad
         dx = dw = None
-        if ctx.needs_input_grad[0]:
+        dy = _aligned(dy)
+        if need[0]:
             dx = _matmul(dy, w.transpose(1, 2), offsets)
-        if ctx.needs_input_grad[1]:
-            if w.stride(1) == 1 and w.stride(2) != 1:  # stored (groups, n, k): so is its gradient
+        if need[1]:
+            if _stored_transposed(w):  # stored (groups, n, k): so is its gradient
                 dw = _outer(dy, x, offsets, w.shape[0]).transpose(1, 2)
             else:
                 dw = _outer(x, dy, offsets, w.shape[0])
@@ -192,12 +219,12 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     _check_offsets(offsets, x, w.shape[0])
     if out is not None:
         _check_out(out, (x.shape[0], w.shape[2]), x, "out", (x, w))
-        _matmul(x, w, offsets, out)
+        _on_device(x, lambda: _matmul(_aligned(x), _aligned_weights(w), offsets, out))
         torch.autograd.graph.increment_version(out)
         return out
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        return _GroupedMatmul.apply(x, w, offsets)
-    return _matmul(x, w, offsets)
+        return _on_device(x, lambda: _GroupedMatmul.apply(x, w, offsets))
+    return _on_device(x, lambda: _matmul(_aligned(x), _aligned_weights(w), offsets))
 
 
 def grouped_outer(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, *,
@@ -217,7 +244,7 @@ def grouped_outer(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, *,
         raise RuntimeError("grouped_outer has no derivative: call it under torch.no_grad()")
     if out is not None:
         _check_out(out, (groups, a.shape[1], b.shape[1]), a, "out", (a, b))
-    result = _outer(a, b, offsets, groups, out)
+    result = _on_device(a, lambda: _outer(_aligned(a), _aligned(b), offsets, groups, out))
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return result
