@@ -235,48 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   }
   griddep_wait();  // before any read of what earlier kernels wrote
   if (MODE != kBatch && warp == 0) {
-    // group starts: clamped to [0, total_rows], non-decreasing; kRaggedM: their first tiles
-    int high = 0;
-    for (int e0 = 0; e0 <= g.batch; e0 += 32) {
-      const int e = e0 + lane;
-      int64_t v = 0;
-      if (e <= g.batch)
-        v = g.offsets64 ? static_cast<const int64_t*>(g.offsets)[e]
-                        : int64_t(static_cast<const int32_t*>(g.offsets)[e]);
-      v = v < 0 ? 0 : (v > g.total_rows ? g.total_rows : v);
-      int x = int(v);
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d && y > x) x = y;
-      }
-      if (x < high) x = high;
-      if (e <= g.batch) start[e] = x;
-      high = __shfl_sync(0xffffffffu, x, 31);
-    }
-    __syncwarp();
-    if (MODE == kRaggedM) {
-      const int groups = g.batch + (g.fill ? 2 : 0);
-      int base = 0;
-      for (int e0 = 0; e0 < groups; e0 += 32) {
-        const int e = e0 + lane;
-        int rows = 0;
-        if (e < g.batch)
-          rows = start[e + 1] - start[e];
-        else if (e < groups)
-          rows = e == g.batch ? g.total_rows - start[g.batch] : start[0];
-        const int tiles = (rows + kTileM - 1) / kTileM * g.tiles_n;
-        int x = tiles;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, x, d);
-          if (lane >= d) x += y;
-        }
-        if (e < groups) first[e] = base + x - tiles;
-        base += __shfl_sync(0xffffffffu, x, 31);
-      }
-      if (lane == 0) first[groups] = base;
-    }
+    group_starts(start, g.offsets, g.offsets64, g.batch, g.total_rows);
+    if (MODE == kRaggedM)
+      group_tiles(first, start, g.batch, g.fill, g.total_rows, kTileM, g.tiles_n);
   }
   tc_fence_before();
   __syncthreads();

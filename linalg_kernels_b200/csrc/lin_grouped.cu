@@ -1,5 +1,5 @@
 // lin_grouped.cu — C-ABI entry points of the products grouped by offsets (lin_gemm.cu).
-#include "lin_common.cuh"
+#include "lin_few.cuh"
 
 namespace lin {
 namespace {
@@ -55,6 +55,7 @@ int linalg_grouped_matmul(const linalg_matrix* x, const linalg_matrix* w, int w_
   p.out = y->data, p.ldo = y->ld, p.out_stride = 0, p.out_type = y->type;
   p.offsets = offsets, p.offsets64 = offsets64 != 0;
   p.total_rows = rows, p.fill = fill != 0;
+  if (few_better(p)) return launch_few(p, static_cast<cudaStream_t>(queue));
   return launch_product(p, static_cast<cudaStream_t>(queue));
 }
 

@@ -27,7 +27,8 @@
 #include <mutex>
 
 #include "lin_elem.cuh"
-#include "lin_fused.cuh"
+#include "lin_few.cuh"
+#include "lin_mid.cuh"
 #include "lin_small.cuh"
 
 namespace lin {
@@ -149,13 +150,11 @@ size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
 struct Layout {
   int64_t planes, ldx, lds, side, x_plane, s_plane;
   size_t x_bytes, s_bytes, sums_bytes, total;
-  bool fused;             // one launch: start values, then X and squares per pair
-  size_t px_bytes, ps_bytes;
 };
 
 Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   Layout l{};
-  if (small_supported(m, n, split)) return l;  // on chip: no workspace
+  if (small_supported(m, n, split) || mid_supported(m, n, split)) return l;  // on chip
   l.planes = split ? 2 : 1;
   l.side = m < n ? m : n;
   l.ldx = round16(n);
@@ -165,14 +164,7 @@ Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   l.x_bytes = round256(size_t(batch) * l.planes * l.x_plane * 2);
   l.s_bytes = round256(size_t(batch) * l.planes * l.s_plane * 2);
   l.sums_bytes = round256(size_t(batch) * kMaxParts * sizeof(double));
-  l.fused = !split && fused_better(batch, m, n);
-  if (l.fused) {
-    l.px_bytes = round256(size_t(fused_pairs(batch)) * 2 * l.x_plane * 2);
-    l.ps_bytes = round256(size_t(fused_pairs(batch)) * 2 * l.s_plane * 2);
-    l.total = l.x_bytes + l.px_bytes + l.ps_bytes + l.sums_bytes;
-  } else {
-    l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
-  }
+  l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
   return l;
 }
 
@@ -217,6 +209,9 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   if (small_supported(m, n, split))
     return launch_small(x, momentum, out, batch, m, n, beta, nesterov, decay, rate, steps,
                         coefficients, eps, split, q);
+  if (mid_supported(m, n, split))
+    return launch_mid_ortho(x, momentum, out, batch, m, n, beta, nesterov, decay, rate, steps,
+                            coefficients, eps, q);
   const Layout l = layout(batch, m, n, split);
   uint8_t* w = static_cast<uint8_t*>(workspace);
   __half* xs[2] = {reinterpret_cast<__half*>(w), reinterpret_cast<__half*>(w + l.x_bytes)};
@@ -261,17 +256,6 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
               : chol::launch_pdl(scale_kernel<false, false>, grid, block, 0, q, true, p);
   if (e != cudaSuccess) return CHOL_ERR_LAUNCH;
 
-  if (l.fused) {
-    FusedCall f{};
-    f.batch = batch, f.m = m, f.n = n;
-    f.x0 = w, f.x = w + l.x_bytes, f.squares = w + l.x_bytes + l.px_bytes;
-    f.ldx = l.ldx, f.lds = l.lds, f.x_plane = l.x_plane, f.s_plane = l.s_plane;
-    f.scale = scale, f.steps = steps, f.coefficients = coefficients;
-    f.muon = muon;
-    f.out = out->data, f.ldo = out->ld, f.out_stride = out->stride, f.out_type = out->type;
-    f.decay = decay, f.rate = rate;
-    return launch_fused(f, q);
-  }
   const bool tall = m > n;
   const int64_t s = l.side, matrices = batch * l.planes;
   const Operand sq_gram{gram, s, s, l.lds, matrices, l.s_plane, false};
@@ -368,7 +352,8 @@ int prepare_device(int dev) {
       return;
     }
     if (prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess ||
-        prepare_fused() != cudaSuccess)
+        prepare_few() != cudaSuccess ||
+        prepare_mid_ortho() != cudaSuccess)
       states[dev].status = CHOL_ERR_DEVICE;
     if (prev != dev) cudaSetDevice(prev);
   });

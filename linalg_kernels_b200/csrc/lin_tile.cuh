@@ -221,6 +221,58 @@ __device__ __forceinline__ void write_one(T* p, float v, bool weights, float dec
   *p = from_float<T>(v);
 }
 
+// The group tables, by one warp. start[0 .. groups]: first rows, clamped to [0, rows] and to the
+// largest before them.
+__device__ __forceinline__ void group_starts(int* start, const void* offsets, int offsets64,
+                                             int groups, int rows) {
+  const int lane = threadIdx.x & 31;
+  int high = 0;
+  for (int e0 = 0; e0 <= groups; e0 += 32) {
+    const int e = e0 + lane;
+    int64_t v = 0;
+    if (e <= groups)
+      v = offsets64 ? static_cast<const int64_t*>(offsets)[e]
+                    : int64_t(static_cast<const int32_t*>(offsets)[e]);
+    v = v < 0 ? 0 : (v > rows ? rows : v);
+    int x = int(v);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d && y > x) x = y;
+    }
+    if (x < high) x = high;
+    if (e <= groups) start[e] = x;
+    high = __shfl_sync(0xffffffffu, x, 31);
+  }
+  __syncwarp();
+}
+// first[0 .. n]: first tiles of the groups (of tile_rows rows by tiles_n column tiles) and, with
+// fill, of two more: the rows behind the last group and those before the first.
+__device__ __forceinline__ void group_tiles(int* first, const int* start, int groups, int fill,
+                                            int rows, int tile_rows, int tiles_n) {
+  const int lane = threadIdx.x & 31;
+  const int n = groups + (fill ? 2 : 0);
+  int base = 0;
+  for (int e0 = 0; e0 < n; e0 += 32) {
+    const int e = e0 + lane;
+    int count = 0;
+    if (e < groups)
+      count = start[e + 1] - start[e];
+    else if (e < n)
+      count = e == groups ? rows - start[groups] : start[0];
+    const int tiles = (count + tile_rows - 1) / tile_rows * tiles_n;
+    int x = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (e < n) first[e] = base + x - tiles;
+    base += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) first[n] = base;
+}
+
 // What an epilogue warp does with its accumulators (a lane holds columns of one row):
 // alpha * acc (+ beta * C) (+ diag on the diagonal), to the output. Results and C pass through
 // shared memory in boxes of 32 rows x 64 columns that TMA copies: a lane's own 32-byte accesses
@@ -476,55 +528,6 @@ struct WarpEpilogue {
       }
     }
     return true;
-  }
-
-  // The same with the warp's own coalesced accesses, for results that another tile waits for: TMA
-  // works off its queue in order, so a store waits behind the loads that the producer has ahead
-  // (3000 to 8000 cycles until it is complete, against ~1000 here). c, o: plane 0 of the matrix,
-  // fp16, rows of whole 32-byte sectors.
-  __device__ __forceinline__ void fetch_c(const Out& g, const __half* c, int row_base, int gc0,
-                                          uint4 (&w)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = row_base + i * 4 + (lane >> 3), col = gc0 + (lane & 7) * 8;
-      if (row < g.rows && col < g.n)
-        w[i] = *reinterpret_cast<const uint4*>(c + int64_t(row) * g.ldo + col);
-    }
-  }
-  template <typename Get>
-  __device__ __forceinline__ void box_now(const Out& g, __half* o, int b, int row_base, int gc0,
-                                          bool mirror, const uint4 (&w)[8], const Get& get) {
-    if (gc0 >= g.n || row_base >= g.rows) return;
-    const bool with_c = g.beta != 0.f;
-    uint8_t* box = buf(b);
-    __syncwarp();  // the box before has been read
-    if (with_c) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *box_chunk(box, i * 4 + (lane >> 3), lane & 7) = w[i];
-      __syncwarp();
-    }
-    uint32_t packed[32], none[SPLIT ? 32 : 1];
-    fill<true>(g, b, row_base, gc0, with_c, get, packed, none);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3), row = row_base + r, col = gc0 + (lane & 7) * 8;
-      const uint4 x = *box_chunk(box, r, lane & 7);
-      if (row < g.rows && col < g.n)
-        *reinterpret_cast<uint4*>(o + int64_t(row) * g.ldo + col) = x;
-    }
-    if (mirror) {
-      __syncwarp();
-      transpose(box, packed);
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 8 + (lane >> 2), row = gc0 + r, col = row_base + (lane & 3) * 8;
-        const uint4 x = *reinterpret_cast<const uint4*>(box + r * 64 + (lane & 3) * 16);
-        if (row < g.n && col < g.rows)
-          *reinterpret_cast<uint4*>(o + int64_t(row) * g.ldo + col) = x;
-      }
-    }
   }
 
   // 32 columns from gc0 straight to the caller's matrix.

@@ -30,7 +30,8 @@ def test_library_exports_and_binding():
 def test_workspace():
     f = _lib.load().linalg_orthogonalize_workspace
     assert f(0, 5, 5, 1) == 0 and f(2, 0, 5, 1) == 0 and f(2, 5, 0, 1) == 0
-    assert f(5, 128, 4096, 1) == 0 and f(5, 4096, 100, 1) == 0 and f(5, 129, 130, 1) > 0
+    assert f(5, 128, 4096, 1) == 0 and f(5, 4096, 100, 1) == 0 and f(5, 129, 256, 1) == 0
+    assert f(5, 129, 257, 1) > 0 and f(5, 129, 256, 2) > 0
     assert f(5, 128, 1536, 2) == 0 and f(5, 128, 1537, 2) > 0
     # two X and two squares of fp16, twice that for full precision
     assert f(3, 512, 1024, 1) >= 3 * 2 * 2 * (512 * 1024 + 512 * 512)
@@ -89,8 +90,8 @@ def test_muon_refusals_of_the_c_entry():
     assert _muon(grad=_m(1 << 20)) == BAD  # the parameter's own memory
     assert _muon(momentum=_m((1 << 22) + 64)) == BAD
     assert _muon(param=_m(1 << 20, stride=0), batch=2) == BAD
-    wide = [_m(1 << k, ld=200) for k in (20, 22)]
-    assert _muon(wide[0], wide[1], _m(1 << 24, ld=200, kind=2), m=200) == SPACE
+    wide = [_m(1 << k, ld=300) for k in (20, 22)]
+    assert _muon(wide[0], wide[1], _m(1 << 24, ld=300, kind=2), m=300) == SPACE
 
 
 def _mul(x=None, w=None, y=None, off=4096, off64=0, groups=2, rows=10, k=64, n=64, fill=1):
@@ -131,9 +132,9 @@ def test_binding_checks_its_arguments():
         lib.orthogonalize(*range(16), 0.0, 5)  # not a buffer
     # a coefficient buffer shorter than the steps is refused, not read past its end
     short = bytes(4 * 3)
-    x, out = (4096, 200, 4096, 0), (1 << 20, 200, 4096, 0)
-    assert lib.orthogonalize(*x, *out, 1, 200, 200, 2, 1, 4096, 0, 0, 0.0, short) == BAD
-    assert lib.orthogonalize(*x, *out, 1, 200, 200, 1, 1, 4096, 0, 0, 0.0, short) == SPACE
+    x, out = (4096, 300, 4096, 0), (1 << 20, 300, 4096, 0)
+    assert lib.orthogonalize(*x, *out, 1, 300, 300, 2, 1, 4096, 0, 0, 0.0, short) == BAD
+    assert lib.orthogonalize(*x, *out, 1, 300, 300, 1, 1, 4096, 0, 0, 0.0, short) == SPACE
 
 
 def test_wrappers_refuse_what_has_no_gpu_path():

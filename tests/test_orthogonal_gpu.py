@@ -70,9 +70,9 @@ SHAPES = [(1, 128, 128), (3, 64, 64), (2, 256, 256), (1, 512, 512), (2, 200, 328
           (1, 128, 512), (2, 128, 513), (1, 100, 700), (2, 700, 100), (1, 90, 1537), (1, 4096, 128),
           (1, 127, 4096), (5, 1, 3000), (6, 43, 64), (9, 31, 1), (7, 64, 129), (130, 1, 5),
           (3, 1536, 20),
-          # one launch per batch, a CTA pair per matrix: one tile, two blocks, odd edges, both ways
-          (1, 256, 256), (3, 130, 190), (80, 256, 256), (5, 512, 512), (40, 300, 520),
-          (40, 520, 300), (76, 384, 640), (150, 129, 257)]
+          # on chip over two CTAs, odd edges, both ways; and just beyond
+          (1, 256, 256), (3, 130, 190), (80, 256, 256), (2, 200, 256), (2, 256, 200), (1, 129, 129),
+          (3, 255, 131), (3, 131, 255), (2, 257, 256), (150, 129, 257), (5, 512, 512), (40, 300, 520)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -125,7 +125,7 @@ def test_magnitudes(magnitude):
     assert _far(got, exact) <= tol
 
 
-@pytest.mark.parametrize("m,n", [(48, 80), (10, 30), (30, 10), (128, 128), (60, 900), (300, 260)])
+@pytest.mark.parametrize("m,n", [(48, 80), (10, 30), (30, 10), (128, 128), (60, 900), (200, 250), (300, 260)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_zero_and_non_finite_matrices(m, n, dtype):
     """(Matrices of 48 x 80 and 10 x 30 share a tile.)"""
@@ -184,7 +184,8 @@ def test_empty():
         assert orthogonalize(x).shape == x.shape
 
 
-@pytest.mark.parametrize("shape", [(1, 128, 128), (2, 256, 512), (3, 200, 100)])
+@pytest.mark.parametrize("shape", [(1, 128, 128), (2, 256, 512), (3, 200, 100), (2, 200, 230),
+                                   (3, 251, 145)])
 @pytest.mark.parametrize("types", [(torch.bfloat16, torch.bfloat16, torch.float32),
                                    (torch.float32, torch.float32, torch.float32),
                                    (torch.float32, torch.bfloat16, torch.bfloat16),
