@@ -27,10 +27,12 @@
 // device memory by every CTA, so the host needs no synchronisation.
 //
 // `split`: FP32 accuracy. An operand is a pair of fp16 planes, x = hi + lo (22 bits), and the
-// product is lo hi + hi lo + hi hi (lo lo, < 2^-22, is dropped). The accumulator rounds toward
-// zero at every MMA, an error that grows with the number of steps, so it is drained every 256 of
-// K into registers (rounded to nearest) with the small terms summed first: 16 full-size steps
-// per drain.
+// product is lo hi + hi lo + hi hi (lo lo, < 2^-22, is dropped), all three from one stage that holds
+// both planes of both operands. The accumulator rounds toward zero at every MMA, an error that
+// grows with the number of steps, so it is drained into registers (rounded to nearest) after each K
+// block, the small terms summed first: 4 full-size steps per drain. (Error of the iteration
+// against 64 bits, 3 x 1001 x 601: 4.5e-6 with a drain per 256 of K, 2.3e-6 per 128, 1.4e-6 per 64,
+// where FP32 products have 3.0e-6.)
 //
 // Every wait is bounded (2 s of %globaltimer); one that runs out records
 // CHOL_ERR_WAIT_TIMEOUT in the library's status word and ends the launch.
@@ -179,8 +181,9 @@ struct Walker {
 
 // Epilogue buffers per warp: two hold C's boxes (and the two planes) of a batch's products; ragged
 // products have no C and need the group tables' space.
-template <int BN, int MODE>
-using ProductCfg = Cfg<BN, MODE == kBatch || BN == 128 ? 2 : 1, MODE == kBatch ? 0 : kTableBytes>;
+template <int BN, int MODE, bool SPLIT>
+using ProductCfg = Cfg<BN, MODE == kBatch || BN == 128 ? 2 : 1, MODE == kBatch ? 0 : kTableBytes,
+                       SPLIT ? 2 : 1>;
 
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                    const __grid_constant__ CUtensorMap map_out,
                    const __grid_constant__ CUtensorMap map_mirror,
                    const __grid_constant__ CUtensorMap map_c, const Args g, int* status) {
-  using C = ProductCfg<BN, MODE>;
+  using C = ProductCfg<BN, MODE, SPLIT>;
   constexpr int S = C::STAGES;
   constexpr int kBufs = MODE == kBatch || BN == 128 ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -264,18 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         constexpr int planes = SPLIT ? 2 : 1;
         const int za = MODE == kBatch ? w.index * planes : 0;
         const int zb = MODE == kRaggedK ? 0 : w.index * planes;
-        const int steps = SPLIT ? 3 * num_k : num_k;
-        for (int i = 0; i < steps; ++i, ++kt) {
-          int kb = i, pa = 0, pb = 0;
-          if (SPLIT) {  // per chunk: lo hi, hi lo, hi hi
-            const int c0 = i / (3 * kChunk) * kChunk;
-            const int len = num_k - c0 < kChunk ? num_k - c0 : kChunk;
-            const int r = i - 3 * c0;
-            const int combo = r / len;
-            kb = c0 + r - combo * len;
-            pa = combo == 0;
-            pb = combo == 1;
-          }
+        for (int kb = 0; kb < num_k; ++kb, ++kt) {
           const int s = int(kt % S);
           if (kt >= uint32_t(S) && !wait_bar(&empty[s], ((kt / S) & 1u) ^ 1u, status)) {
             ok = false;
@@ -294,17 +286,22 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             tails &= ~(1u << s);
           }
           const int kx = w.k0 + kb * kBlockK;
-          if (AMN) {
-            tma_load_pair(sa, &map_a, a_row, kx, za + pa, bar);
-            tma_load_pair(sa + 8192, &map_a, a_row + 64, kx, za + pa, bar);
-          } else {
-            tma_load_pair(sa, &map_a, kx, a_row, za + pa, bar);
-          }
-          if (BMN) {
-            tma_load_pair(sb, &map_b, b_row, kx, zb + pb, bar);
-            if (BN == 256) tma_load_pair(sb + 8192, &map_b, b_row + 64, kx, zb + pb, bar);
-          } else {
-            tma_load_pair(sb, &map_b, kx, b_row, zb + pb, bar);
+#pragma unroll
+          for (int p = 0; p < planes; ++p) {
+            uint8_t* pa = sa + p * C::A_PLANE;
+            uint8_t* pb = sb + p * C::B_PLANE;
+            if (AMN) {
+              tma_load_pair(pa, &map_a, a_row, kx, za + p, bar);
+              tma_load_pair(pa + 8192, &map_a, a_row + 64, kx, za + p, bar);
+            } else {
+              tma_load_pair(pa, &map_a, kx, a_row, za + p, bar);
+            }
+            if (BMN) {
+              tma_load_pair(pb, &map_b, b_row, kx, zb + p, bar);
+              if (BN == 256) tma_load_pair(pb + 8192, &map_b, b_row + 64, kx, zb + p, bar);
+            } else {
+              tma_load_pair(pb, &map_b, kx, b_row, zb + p, bar);
+            }
           }
         }
       }
@@ -324,8 +321,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         walk.at(t, w);
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
         if (num_k == 0) continue;
-        const int chunks = SPLIT ? (num_k + kChunk - 1) / kChunk : 1;
-        for (int ch = 0; ch < chunks && ok; ++ch, ++round) {
+        const int rounds = SPLIT ? num_k : 1;  // split: an accumulator per K block
+        for (int r = 0; r < rounds && ok; ++r, ++round) {
           const uint32_t buf = round & 1u;
           if (round >= 2 && !wait_bar(&tempty[buf], ((round >> 1) & 1u) ^ 1u, status)) {
             ok = false;
@@ -333,10 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
           tc_fence_after();
           const uint32_t acc = tmem + buf * uint32_t(BN);
-          const int c0 = SPLIT ? ch * kChunk : 0;
-          const int len = SPLIT ? (num_k - c0 < kChunk ? num_k - c0 : kChunk) : num_k;
-          const int steps = SPLIT ? 3 * len : len;
-          for (int i = 0; i < steps; ++i, ++kt) {
+          for (int kb = SPLIT ? r : 0; kb < (SPLIT ? r + 1 : num_k); ++kb, ++kt) {
             const int s = int(kt % S);
             if (!wait_bar(&full[s], (kt / S) & 1u, status)) {
               ok = false;
@@ -345,16 +339,21 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             tc_fence_after();
             const uint8_t* sa = smem + size_t(s) * C::STAGE;
             const uint8_t* sb = sa + C::A_BYTES;
-            const uint64_t da = AMN ? sw128_desc_mn(sa) : sw128_desc(sa);
-            const uint64_t db = BMN ? sw128_desc_mn(sb) : sw128_desc(sb);
-            const int kb = c0 + (SPLIT ? i % len : i);
             const int left = w.k_len - kb * kBlockK;  // the last block: only its 16-wide slabs
             const int slabs = left >= kBlockK ? kBlockK / 16 : (left + 15) / 16;
 #pragma unroll
-            for (int kk = 0; kk < kBlockK / 16; ++kk) {
-              if (kk >= slabs) break;
-              mma_pair(acc, da + uint64_t(kk * (AMN ? 2048 : 32) / 16),
-                       db + uint64_t(kk * (BMN ? 2048 : 32) / 16), g.idesc, (i | kk) ? 1u : 0u);
+            for (int c = SPLIT ? 0 : 2; c < 3; ++c) {  // lo hi, hi lo, hi hi
+              const uint8_t* pa = sa + (c == 0 ? C::A_PLANE : 0);
+              const uint8_t* pb = sb + (c == 1 ? C::B_PLANE : 0);
+              const uint64_t da = AMN ? sw128_desc_mn(pa) : sw128_desc(pa);
+              const uint64_t db = BMN ? sw128_desc_mn(pb) : sw128_desc(pb);
+#pragma unroll
+              for (int kk = 0; kk < kBlockK / 16; ++kk) {
+                if (kk >= slabs) break;
+                mma_pair(acc, da + uint64_t(kk * (AMN ? 2048 : 32) / 16),
+                         db + uint64_t(kk * (BMN ? 2048 : 32) / 16), g.idesc,
+                         SPLIT ? (c | kk ? 1u : 0u) : (kb | kk ? 1u : 0u));
+              }
             }
             commit_pair(&empty[s]);
           }
@@ -408,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t round = 0;
     constexpr int P = SPLIT ? 2 : 1;
     Out o;
-    o.alpha = g.alpha, o.beta = EPI == kPlanes ? g.beta : 0.f, o.diag = EPI == kPlanes ? g.diag : 0.f;
+    o.alpha = g.alpha, o.beta = EPI == kPlanes || SPLIT ? g.beta : 0.f;
+    o.diag = EPI == kPlanes ? g.diag : 0.f;
     o.n = g.n;
     o.map = &map_out, o.mirror = &map_mirror, o.c_map = &map_c;
     o.boxes = EPI == kMuon ? 0 : g.boxes;
@@ -450,11 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         continue;
       }
       bool ok = true;
-      if (kC) ep.load_c(o, row_base, col0);
+      if (kC || SPLIT) ep.load_c(o, row_base, col0);
       if constexpr (SPLIT) {
         float sum[2][32];
-        const int chunks = (num_k + kChunk - 1) / kChunk;
-        for (int ch = 0; ch < chunks; ++ch, ++round) {
+        for (int ch = 0; ch < num_k; ++ch, ++round) {
           const uint32_t buf = round & 1u;
           ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
           if (!ok) break;
@@ -479,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             for (int j = 0; j < 32; ++j) v[j] = sum[h][j];
           });
         } else {
+          ok = ep.add_c(o, sum, status);
           ep.direct(o, row_base, col0, sum[0]);
           ep.direct(o, row_base, col0 + 32, sum[1]);
         }
@@ -533,7 +533,7 @@ template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 cudaError_t set_smem() {
   return cudaFuncSetAttribute(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              int(ProductCfg<BN, MODE>::SMEM));
+                              int(ProductCfg<BN, MODE, SPLIT>::SMEM));
 }
 
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
@@ -567,20 +567,19 @@ int launch(const Product& p, cudaStream_t q) {
               p.out_stride % sector == 0;
   // the output's boxes, where its type and alignment allow: by group rows when these are ragged
   CUtensorMap mo = ma, mm = ma, mc = ma;
-  if (EPI == kPlanes || (EPI != kMuon && p.out_type != LINALG_FP32)) {
-    const int64_t planes = EPI == kPlanes && SPLIT ? 2 : 1;
+  const int64_t planes = SPLIT ? 2 : 1;
+  if (EPI == kPlanes || (!SPLIT && EPI != kMuon && p.out_type != LINALG_FP32)) {
     const Operand out{p.out, MODE == kRaggedM ? p.total_rows : p.m, p.n, p.ldo,
                       MODE == kRaggedM ? 1 : p.batch * planes, p.out_stride, false};
     const bool b16 = EPI != kPlanes && p.out_type == LINALG_BF16;
-    if ((EPI == kPlanes || !SPLIT) && make_output_map(&mo, out, b16, false))
-      g.boxes = MODE == kRaggedM ? 1 : 2;
+    if (make_output_map(&mo, out, b16, false)) g.boxes = MODE == kRaggedM ? 1 : 2;
     if (EPI == kPlanes && (!g.boxes || !make_output_map(&mm, out, false, true)))
       return CHOL_ERR_UNSUPPORTED;
-    if (EPI == kPlanes && p.beta != 0.f &&
-        !make_output_map(&mc, Operand{p.c, p.m, p.n, p.ldc, p.batch * planes, p.c_plane, false},
-                         false, false))
-      return CHOL_ERR_UNSUPPORTED;
   }
+  if ((EPI == kPlanes || SPLIT) && p.beta != 0.f &&
+      !make_output_map(&mc, Operand{p.c, p.m, p.n, p.ldc, p.batch * planes, p.c_plane, false}, false,
+                       false))
+    return CHOL_ERR_UNSUPPORTED;
   g.decay = p.decay, g.rate = p.rate;
   g.offsets = p.offsets, g.offsets64 = p.offsets64;
   g.total_rows = int(p.total_rows), g.fill = p.fill;
@@ -591,7 +590,7 @@ int launch(const Product& p, cudaStream_t q) {
   if (pairs > total) pairs = total;
   return chol::status_from(chol::launch_pdl(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
                                             dim3(unsigned(2 * pairs)), dim3(kThreads),
-                                            ProductCfg<BN, MODE>::SMEM, q, true, ma, mb, mo, mm,
+                                            ProductCfg<BN, MODE, SPLIT>::SMEM, q, true, ma, mb, mo, mm,
                                             mc, g, chol::device_status_ptr()));
 }
 

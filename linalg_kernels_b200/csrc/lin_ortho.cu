@@ -283,7 +283,9 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     f.m = f.n = f.k = s, f.batch = batch;
     f.alpha = c * (poly_scale / (gram_scale * gram_scale)), f.beta = b * (poly_scale / gram_scale);
     f.c = gram, f.ldc = l.lds, f.c_plane = l.s_plane;
-    f.diag = a * poly_scale;
+    // half precision: a on B's diagonal (see above); full: a X is added in FP32 at the end, not summed
+    // by the tensor core, whose rounding towards zero would weigh on the largest term
+    f.diag = split ? 0.f : a * poly_scale;
     f.out = poly, f.ldo = l.lds, f.out_stride = l.s_plane;
     if ((st = launch_product(f, q)) != CHOL_OK) return st;
     Product u;  // X <- B X or X B
@@ -292,12 +294,13 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     u.split = split;
     u.m = m, u.n = n, u.k = s, u.batch = batch;
     u.alpha = 1.f / poly_scale;
+    if (split) u.beta = a, u.c = cur, u.ldc = l.ldx, u.c_plane = l.x_plane;
     if (k + 1 < steps) {
       u.epilogue = kPlanes;
       u.out = xs[(k + 1) & 1], u.ldo = l.ldx, u.out_stride = l.x_plane;
     } else {
       u.epilogue = muon ? kMuon : kFinal;
-      u.alpha /= scale;
+      u.alpha /= scale, u.beta /= scale;
       u.out = out->data, u.ldo = out->ld, u.out_stride = out->stride, u.out_type = out->type;
       u.decay = decay, u.rate = rate;
     }

@@ -471,9 +471,12 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-    // B takes a on its diagonal (its scale is 1), so that X <- B X needs no old X: one more rounding
-    // of 2^-12 per row, as X's own, for half of that epilogue's instructions
-    const float fb = cb * g.inv_gram, fc = cc * g.inv_gram * g.inv_gram;
+    // half precision: B takes a on its diagonal (its scale is 1), so that X <- B X needs no old X: one
+    // more rounding of 2^-12 per row, as X's own, for half of that epilogue's instructions. Full:
+    // a X is added in FP32 at the end, not summed by the tensor core, whose rounding towards zero
+    // would weigh on the largest term; and B keeps 22 bits with a scale of 2048.
+    constexpr float kPoly = SPLIT ? 2048.f : 1.f;
+    const float fb = cb * g.inv_gram * kPoly, fc = cc * g.inv_gram * g.inv_gram * kPoly;
 #pragma unroll
     for (int n = 0; n < GROUPS; ++n) {
       const int q = win0 + part + n * PARTS;
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
             add8(y, *reinterpret_cast<const uint4*>(gs + at), fb);
             if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), fb);
           }
-          if (q * 32 == q32) {  // the same for the whole warp
+          if (!SPLIT && q * 32 == q32) {  // the same for the whole warp
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               y[e] += j + e == diag ? ca : 0.f;  // a select: branches would part the warp
@@ -550,11 +553,15 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
 #pragma unroll
           for (int j = 0; j < 16; j += 8) {
             float y[8];
+            const uint32_t at = chunk_at(row, c0 + h * 16 + j);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = v[j + e];
+            for (int e = 0; e < 8; ++e) y[e] = SPLIT ? v[j + e] * (1.f / kPoly) : v[j + e];
+            if (SPLIT) {
+              add8(y, *reinterpret_cast<const uint4*>(xs + at), ca);
+              add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca);
+            }
             uint4 hi, lo;
             round8v<SPLIT>(y, hi, lo);
-            const uint32_t at = chunk_at(row, c0 + h * 16 + j);
             *reinterpret_cast<uint4*>(xs + at) = hi;
             if (SPLIT) *reinterpret_cast<uint4*>(xs + x_plane + at) = lo;
           }
@@ -576,7 +583,12 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
         for (int j = 0; j < 32; j += 8) {
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * g.inv_x;
+          for (int e = 0; e < 8; ++e) y[e] = v[j + e] * (g.inv_x / kPoly);
+          if (SPLIT) {
+            const uint32_t at = chunk_at(row, c0 + j);
+            add8(y, *reinterpret_cast<const uint4*>(xs + at), ca * g.inv_x);
+            add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca * g.inv_x);
+          }
           if (g.tall) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) stage[(h * 32 + j + e) * 128 + row] = y[e];

@@ -28,16 +28,18 @@ constexpr int kTileM = 256;     // rows of a pair's tile
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kEpiLd = 33;      // staging row stride in floats: conflict-free by row and by column
-constexpr int kChunk = 4;       // split: K blocks per drained accumulator
 
 constexpr int kBoxBytes = 32 * 128;  // one warp's 32 rows x 64 columns of 16 bits
 
-// BUFS: boxes of staging per epilogue warp. TABLE: bytes for the group tables.
-template <int BN, int BUFS, int TABLE_BYTES>
+// BUFS: boxes of staging per epilogue warp. TABLE: bytes for the group tables. PLANES: of each
+// operand in a stage.
+template <int BN, int BUFS, int TABLE_BYTES, int PLANES>
 struct Cfg {
-  static constexpr int STAGES = BN == 256 ? 5 : 6;
-  static constexpr int A_BYTES = 128 * kBlockK * 2;
-  static constexpr int B_BYTES = BN / 2 * kBlockK * 2;
+  static constexpr int STAGES = PLANES == 2 ? 3 : (BN == 256 ? 5 : 6);
+  static constexpr int A_PLANE = 128 * kBlockK * 2;
+  static constexpr int B_PLANE = BN / 2 * kBlockK * 2;
+  static constexpr int A_BYTES = PLANES * A_PLANE;
+  static constexpr int B_BYTES = PLANES * B_PLANE;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int EPI = kEpiWarps * BUFS * kBoxBytes;
   static constexpr int TABLE = TABLE_BYTES;
@@ -527,6 +529,31 @@ struct WarpEpilogue {
         if (SPLIT) store_box(g.mirror, lo, row_base, gc0, g.z + 1);
       }
     }
+    return true;
+  }
+
+  // SPLIT, the caller's matrix: sum += beta / alpha * C, of the boxes that load_c has asked for.
+  __device__ __forceinline__ bool add_c(const Out& g, float (&sum)[2][32], int* status) {
+    if (g.beta == 0.f) return true;
+    bool ok = wait_c(g, 0, status);
+    ok = wait_c(g, 1, status) && ok;
+    if (!ok) return false;
+    const float f = g.beta / g.alpha;  // alpha is a power of two
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 a = *box_chunk(buf(0), lane, h * 4 + c), b = *box_chunk(buf(1), lane, h * 4 + c);
+        const uint32_t as[4] = {a.x, a.y, a.z, a.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&as[e]));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&bs[e]));
+          float* p = sum[h] + c * 8 + 2 * e;
+          p[0] = fmaf(f, x.x + y.x, p[0]);
+          p[1] = fmaf(f, x.y + y.y, p[1]);
+        }
+      }
     return true;
   }
 
