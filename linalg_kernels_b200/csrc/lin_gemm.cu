@@ -472,13 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           if (lane == 0) arrive_leader_relaxed(leader_addr(&tempty[buf]));
         }
         if (!__all_sync(0xffffffffu, ok)) break;
+        ok = ep.add_c(o, sum, status);
         if constexpr (kC) {
-          ok = ep.template box<kC>(o, 0, row_base, col0, mirror, status, [&](int h, float (&v)[32]) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = sum[h][j];
-          });
+          ep.planes(o, row_base, col0, mirror, sum);
         } else {
-          ok = ep.add_c(o, sum, status);
           ep.direct(o, row_base, col0, sum[0]);
           ep.direct(o, row_base, col0 + 32, sum[1]);
         }

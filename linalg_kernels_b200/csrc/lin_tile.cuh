@@ -401,10 +401,8 @@ struct WarpEpilogue {
   // 32 h + 31 of this lane's row. with_c: the buffer holds C.
   template <bool HAS_C, typename Get>
   __device__ __forceinline__ void fill(const Out& g, int b, int row_base, int gc0, bool with_c,
-                                       const Get& get, uint32_t (&packed)[32],
-                                       uint32_t (&packed_lo)[SPLIT ? 32 : 1]) {
+                                       const Get& get, uint32_t (&packed)[32]) {
     uint8_t* hi = buf(b);
-    uint8_t* lo = SPLIT ? buf(1) : nullptr;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[32];
@@ -415,17 +413,9 @@ struct WarpEpilogue {
         for (int c = 0; c < 4; ++c) {
           const uint4 w = *box_chunk(hi, lane, h * 4 + c);
           const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-          uint4 wl = make_uint4(0, 0, 0, 0);
-          if (SPLIT) wl = *box_chunk(lo, lane, h * 4 + c);
-          const uint32_t wls[4] = {wl.x, wl.y, wl.z, wl.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float2 x = __half22float2(*reinterpret_cast<const __half2*>(&ws[e]));
-            if (SPLIT) {
-              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&wls[e]));
-              x.x += y.x;  // exact: hi + lo has 22 bits
-              x.y += y.y;
-            }
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&ws[e]));
             float* p = v + c * 8 + 2 * e;
             const float2 t = chol::ffma2(beta, x, make_float2(0.f, 0.f));
             const float2 r = chol::ffma2(alpha, make_float2(p[0], p[1]), t);
@@ -451,24 +441,13 @@ struct WarpEpilogue {
           packed[h * 16 + j] = pack<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          packed[h * 16 + j] = pack<__half>(v[2 * j], v[2 * j + 1]);
-          if (SPLIT) {
-            float c0, c1;
-            unpack<__half>(packed[h * 16 + j], c0, c1);
-            packed_lo[SPLIT ? h * 16 + j : 0] = pack<__half>(v[2 * j] - c0, v[2 * j + 1] - c1);
-          }
-        }
+        for (int j = 0; j < 16; ++j) packed[h * 16 + j] = pack<__half>(v[2 * j], v[2 * j + 1]);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int o = h * 16 + c * 4;
         *box_chunk(hi, lane, h * 4 + c) =
             make_uint4(packed[o], packed[o + 1], packed[o + 2], packed[o + 3]);
-        if (SPLIT)
-          *box_chunk(lo, lane, h * 4 + c) =
-              make_uint4(packed_lo[SPLIT ? o : 0], packed_lo[SPLIT ? o + 1 : 0],
-                         packed_lo[SPLIT ? o + 2 : 0], packed_lo[SPLIT ? o + 3 : 0]);
       }
     }
   }
@@ -494,7 +473,6 @@ struct WarpEpilogue {
     bool ok = true;
     if (HAS_C) {
       ok = wait_c(g, b, status);
-      if (SPLIT) ok = wait_c(g, 1, status) && ok;
       if (!ok) return false;
     }
     if (gc0 >= g.n || row_base >= g.rows) {
@@ -503,42 +481,38 @@ struct WarpEpilogue {
     }
     const bool with_c = HAS_C && g.beta != 0.f;
     if (!with_c) {
-      if (lane == 0) boxes_read_but(BUFS == 2 && !SPLIT ? newest : 0);
+      if (lane == 0) boxes_read_but(BUFS == 2 ? newest : 0);
       __syncwarp();
     }
     newest = mirror ? 2 : 1;
     uint8_t* hi = buf(b);
-    uint8_t* lo = SPLIT ? buf(1) : nullptr;
-    uint32_t packed[32], packed_lo[SPLIT ? 32 : 1];
-    fill<HAS_C>(g, b, row_base, gc0, with_c, get, packed, packed_lo);
+    uint32_t packed[32];
+    fill<HAS_C>(g, b, row_base, gc0, with_c, get, packed);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
       store_box(g.map, hi, gc0, g.y + row_base, g.z);
-      if (SPLIT) store_box(g.map, lo, gc0, g.y + row_base, g.z + 1);
     }
     if (HAS_C && mirror) {
       if (lane == 0) boxes_read();
       __syncwarp();
       transpose(hi, packed);
-      if (SPLIT) transpose(lo, packed_lo);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         store_box(g.mirror, hi, row_base, gc0, g.z);
-        if (SPLIT) store_box(g.mirror, lo, row_base, gc0, g.z + 1);
       }
     }
     return true;
   }
 
-  // SPLIT, the caller's matrix: sum += beta / alpha * C, of the boxes that load_c has asked for.
+  // SPLIT: sum += beta / alpha * C, of the boxes that load_c has asked for.
   __device__ __forceinline__ bool add_c(const Out& g, float (&sum)[2][32], int* status) {
     if (g.beta == 0.f) return true;
     bool ok = wait_c(g, 0, status);
     ok = wait_c(g, 1, status) && ok;
     if (!ok) return false;
-    const float f = g.beta / g.alpha;  // alpha is a power of two
+    const float f = g.beta / g.alpha;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -555,6 +529,56 @@ struct WarpEpilogue {
         }
       }
     return true;
+  }
+
+  // SPLIT: alpha * sum as two planes, 64 columns from gc0. Nothing but the sums stays in registers
+  // (with packed copies they went to local memory, 2200 cycles for each drain).
+  __device__ __forceinline__ void planes(const Out& g, int row_base, int gc0, bool mirror,
+                                         const float (&sum)[2][32]) {
+    if (gc0 >= g.n || row_base >= g.rows) return;
+    uint8_t *hi = buf(0), *lo = buf(1);
+    if (lane == 0) boxes_read();
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = g.alpha * sum[c >> 2][(c & 3) * 8 + 2 * e];
+        const float y = g.alpha * sum[c >> 2][(c & 3) * 8 + 2 * e + 1];
+        h[e] = pack<__half>(x, y);
+        float a, b;
+        unpack<__half>(h[e], a, b);
+        l[e] = pack<__half>(x - a, y - b);
+      }
+      *box_chunk(hi, lane, c) = make_uint4(h[0], h[1], h[2], h[3]);
+      *box_chunk(lo, lane, c) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      store_box(g.map, hi, gc0, g.y + row_base, g.z);
+      store_box(g.map, lo, gc0, g.y + row_base, g.z + 1);
+    }
+    if (!mirror) return;
+    if (lane == 0) boxes_read();
+    __syncwarp();
+#pragma unroll 1
+    for (int p = 0; p < 2; ++p) {
+      uint8_t* box = p ? lo : hi;
+      uint32_t packed[32];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 w = *box_chunk(box, lane, c);
+        packed[4 * c] = w.x, packed[4 * c + 1] = w.y;
+        packed[4 * c + 2] = w.z, packed[4 * c + 3] = w.w;
+      }
+      __syncwarp();
+      transpose(box, packed);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) store_box(g.mirror, box, row_base, gc0, g.z + p);
+    }
   }
 
   // 32 columns from gc0 straight to the caller's matrix.
