@@ -26,7 +26,7 @@
 
 #include <mutex>
 
-#include "lin_elem.cuh"
+#include "lin_chip.cuh"
 #include "lin_few.cuh"
 #include "lin_mid.cuh"
 #include "lin_small.cuh"
@@ -50,29 +50,77 @@ struct Prep {
   __half* planes;     // X: [batch][P][rows][ldx]
   int64_t ldx;
   float scale, eps;
+  int path;  // types: see walk_types
 };
 
-// The iteration's start value u of one chunk: the input itself, or the momentum average.
-template <bool MUON, bool UPDATE>
-__device__ __forceinline__ void start_value(const Prep& p, int64_t i, int64_t r, int c, int count,
-                                            float (&u)[8]) {
-  load_any(p.x, i * p.x.stride + r * p.x.ld + c, u, count);
-  if (MUON) {
-    float mo[8];
-    const int64_t at = i * p.momentum.stride + r * p.momentum.ld + c;
-    load_any(p.momentum, at, mo, count);
-    if (UPDATE) {
+// The start value u of U chunks per thread, the loads of all of them in flight: the input itself, or
+// the momentum average (updated on the way with UPDATE). body(chunk's row, column, count, u).
+template <bool MUON, bool UPDATE, typename TX, typename TM, typename Body>
+__device__ __forceinline__ void walk(const Prep& p, int64_t i, int part, const Body& body) {
+  constexpr int U = MUON ? 2 : 4;
+  const int64_t stride = int64_t(p.parts) * kPrepThreads;
+  for (int64_t t0 = int64_t(part) * kPrepThreads + threadIdx.x; t0 < p.chunks; t0 += U * stride) {
+    Eight<TX> x[U];
+    Eight<TM> mo[MUON ? U : 1];
+    int64_t r[U];
+    int c[U];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mo[j] = fmaf(p.beta, mo[j], p.gain * u[j]);
-      store_any(p.momentum, at, mo, count);  // mo: as stored
+    for (int q = 0; q < U; ++q) {
+      const int64_t t = t0 + q * stride;
+      // (32-bit division where the chunks of a matrix allow it)
+      r[q] = p.chunks <= 0x7fffffff ? int(t) / p.chunks_row : t / p.chunks_row;
+      c[q] = int(t - r[q] * p.chunks_row) * 8;
+      if (t >= p.chunks) {
+        c[q] = -1;
+        continue;
+      }
+      const int count = p.n - c[q] < 8 ? p.n - c[q] : 8;
+      x[q].load(p.x, i * p.x.stride + r[q] * p.x.ld + c[q], count);
+      if (MUON)
+        mo[MUON ? q : 0].load(p.momentum, i * p.momentum.stride + r[q] * p.momentum.ld + c[q], count);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = p.nesterov ? fmaf(p.beta, mo[j], p.gain * u[j]) : mo[j];
+    for (int q = 0; q < U; ++q) {
+      if (c[q] < 0) continue;
+      const int count = p.n - c[q] < 8 ? p.n - c[q] : 8;
+      float u[8];
+      x[q].get(u);
+      if (MUON) {
+        float m[8];
+        mo[MUON ? q : 0].get(m);
+        if (UPDATE) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m[j] = fmaf(p.beta, m[j], p.gain * u[j]);
+          // m: as stored
+          Eight<TM>::put(p.momentum, i * p.momentum.stride + r[q] * p.momentum.ld + c[q], m, count);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = p.nesterov ? fmaf(p.beta, m[j], p.gain * u[j]) : m[j];
+      }
+      body(r[q], c[q], count, u);
+    }
+  }
+}
+// The same for the matrices' types: whole aligned chunks of the common ones, else any.
+template <bool MUON, bool UPDATE, typename Body>
+__device__ __forceinline__ void walk_types(const Prep& p, int64_t i, int part, const Body& body) {
+  switch (p.path) {
+    case 1:
+      walk<MUON, UPDATE, __nv_bfloat16, float>(p, i, part, body);
+      break;
+    case 2:
+      walk<MUON, UPDATE, float, float>(p, i, part, body);
+      break;
+    case 3:
+      walk<MUON, UPDATE, __nv_bfloat16, __nv_bfloat16>(p, i, part, body);
+      break;
+    default:
+      walk<MUON, UPDATE, Any, Any>(p, i, part, body);
   }
 }
 
-// Sum of squares of each block's share, with the momentum updated on the way. Bound by HBM:
-// reads the input (and reads and writes the momentum) once.
+// Sum of squares of each block's share, with the momentum updated on the way. Bound by HBM: reads
+// the input (and reads and writes the momentum) once.
 template <bool MUON>
 __global__ void __launch_bounds__(kPrepThreads) sum_kernel(const Prep p) {
   griddep_wait();
@@ -80,17 +128,9 @@ __global__ void __launch_bounds__(kPrepThreads) sum_kernel(const Prep p) {
   const int64_t i = blockIdx.x / p.parts;
   const int part = int(blockIdx.x - i * p.parts);
   double sum = 0.0;
-  for (int64_t t = int64_t(part) * kPrepThreads + threadIdx.x; t < p.chunks;
-       t += int64_t(p.parts) * kPrepThreads) {
-    const int64_t r = t / p.chunks_row;
-    const int c = int(t - r * p.chunks_row) * 8;
-    const int count = p.n - c < 8 ? p.n - c : 8;
-    float u[8];
-    start_value<MUON, true>(p, i, r, c, count, u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) sum += double(u[j]) * double(u[j]);
-  }
+  walk_types<MUON, true>(p, i, part, [&](int64_t, int, int count, const float (&u)[8]) {
+    sum += chip::squares8(u, count);
+  });
   __shared__ double warp_sum[kPrepThreads / 32];
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -121,13 +161,7 @@ __global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
   __syncthreads();
   const float2 f = factor;
   constexpr int P = SPLIT ? 2 : 1;
-  for (int64_t t = int64_t(part) * kPrepThreads + threadIdx.x; t < p.chunks;
-       t += int64_t(p.parts) * kPrepThreads) {
-    const int64_t r = t / p.chunks_row;
-    const int c = int(t - r * p.chunks_row) * 8;
-    const int count = p.n - c < 8 ? p.n - c : 8;
-    float u[8];
-    start_value<MUON, false>(p, i, r, c, count, u);
+  walk_types<MUON, false>(p, i, part, [&](int64_t r, int c, int count, const float (&u)[8]) {
     alignas(16) __half hi[8], lo[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -140,7 +174,7 @@ __global__ void __launch_bounds__(kPrepThreads) scale_kernel(const Prep p) {
     *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
     if (SPLIT)
       *reinterpret_cast<uint4*>(o + p.rows * p.ldx) = *reinterpret_cast<const uint4*>(lo);
-  }
+  });
 }
 
 // rows of the workspace start on 32-byte sectors
@@ -233,6 +267,12 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   p.rows = m, p.n = int(n);
   p.chunks_row = int((n + 7) / 8);
   p.chunks = m * p.chunks_row;
+  if (n % 8 == 0 && p.x.vec) {
+    const bool mo32 = !muon || (momentum->type == LINALG_FP32 && p.momentum.vec);
+    const bool mo16 = muon && momentum->type == LINALG_BF16 && p.momentum.vec;
+    if (x->type == LINALG_BF16) p.path = mo32 ? 1 : (mo16 ? 3 : 0);
+    if (x->type == LINALG_FP32) p.path = mo32 ? 2 : 0;
+  }
   // about 4 chunks a thread, at most ~16 blocks per SM over the batch
   int64_t parts = (p.chunks + kPrepThreads * 4 - 1) / (kPrepThreads * 4);
   const int64_t cap = (int64_t(sm_count()) * 16 + batch - 1) / batch;
