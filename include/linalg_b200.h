@@ -48,7 +48,7 @@ typedef struct {
 /* Bytes of device workspace (256-byte aligned) of linalg_orthogonalize and linalg_muon_update
    for `batch` m x n matrices at a working precision (HALF or FULL; AUTO counts as FULL). 0 where
    the iteration runs on chip (smaller side <= 128 and the other within a cluster's shared
-   memory). */
+   memory; in half precision also both sides <= 256). */
 CHOL_API size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n,
                                                int precision);
 
@@ -58,7 +58,7 @@ CHOL_API size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t
  * (from the right with A = X^T X when m > n), and out = X. coefficients: 3 * steps host floats
  * (a, b, c of each step). x and out may be the same array; partial overlap is not allowed.
  * A matrix with a NaN or an infinity yields NaN; the other matrices of the batch are not
- * affected. A zero matrix yields zeros.
+ * affected. A zero matrix yields zeros (with eps > 0).
  */
 CHOL_API int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64_t batch,
                                   int64_t m, int64_t n, int steps, const float* coefficients,

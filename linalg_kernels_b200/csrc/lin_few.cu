@@ -261,7 +261,7 @@ int launch(const Product& p, cudaStream_t q) {
             (uint32_t(NT >> 3) << 17) | (8u << 24);
   // an upper bound: every group may end in a partial tile
   const int64_t total = ((p.total_rows + NT - 1) / NT + p.batch + 2) * g.tiles_n;
-  if (total > 0x7fffffffLL) return CHOL_ERR_UNSUPPORTED;
+  if (total > 0x7fffffffLL - 1024) return CHOL_ERR_UNSUPPORTED;  // tile numbers step past it
   const int64_t ctas = total < sm_count() ? total : sm_count();
   return chol::status_from(chol::launch_pdl(few_kernel<NT, AMN, T>, dim3(unsigned(ctas)),
                                             dim3(kFewThreads), FewCfg<NT>::SMEM, q, true, mw, mx, g,

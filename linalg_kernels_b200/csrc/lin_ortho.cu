@@ -36,7 +36,6 @@ namespace lin {
 namespace {
 
 constexpr int kPrepThreads = 256;
-constexpr int kMaxParts = 2048;
 
 struct Prep {
   Matrix x, momentum;  // x: the input, or the gradient
@@ -186,6 +185,16 @@ struct Layout {
   size_t x_bytes, s_bytes, sums_bytes, total;
 };
 
+// Blocks per matrix of the first passes: about 4 chunks a thread, at most ~16 blocks per SM over the
+// batch.
+int64_t prep_parts(int64_t batch, int64_t m, int64_t n) {
+  const int64_t chunks = m * ((n + 7) / 8);
+  int64_t parts = (chunks + kPrepThreads * 4 - 1) / (kPrepThreads * 4);
+  const int64_t cap = (int64_t(sm_count()) * 16 + batch - 1) / batch;
+  if (parts > cap) parts = cap;
+  return parts < 1 ? 1 : parts;
+}
+
 Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   Layout l{};
   if (small_supported(m, n, split) || mid_supported(m, n, split)) return l;  // on chip
@@ -197,7 +206,7 @@ Layout layout(int64_t batch, int64_t m, int64_t n, bool split) {
   l.s_plane = l.side * l.lds;
   l.x_bytes = round256(size_t(batch) * l.planes * l.x_plane * 2);
   l.s_bytes = round256(size_t(batch) * l.planes * l.s_plane * 2);
-  l.sums_bytes = round256(size_t(batch) * kMaxParts * sizeof(double));
+  l.sums_bytes = round256(size_t(batch) * prep_parts(batch, m, n) * sizeof(double));
   l.total = 2 * l.x_bytes + 2 * l.s_bytes + l.sums_bytes;
   return l;
 }
@@ -273,12 +282,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
     if (x->type == LINALG_BF16) p.path = mo32 ? 1 : (mo16 ? 3 : 0);
     if (x->type == LINALG_FP32) p.path = mo32 ? 2 : 0;
   }
-  // about 4 chunks a thread, at most ~16 blocks per SM over the batch
-  int64_t parts = (p.chunks + kPrepThreads * 4 - 1) / (kPrepThreads * 4);
-  const int64_t cap = (int64_t(sm_count()) * 16 + batch - 1) / batch;
-  if (parts > cap) parts = cap;
-  if (parts > kMaxParts) parts = kMaxParts;
-  p.parts = int(parts < 1 ? 1 : parts);
+  p.parts = int(prep_parts(batch, m, n));
   p.sums = reinterpret_cast<double*>(w + l.total - l.sums_bytes);
   p.planes = xs[0];
   p.ldx = l.ldx;

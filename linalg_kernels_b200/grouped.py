@@ -17,6 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .orthogonal import _written
 
 __all__ = ["grouped_matmul", "grouped_outer"]
 
@@ -220,7 +221,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     if out is not None:
         _check_out(out, (x.shape[0], w.shape[2]), x, "out", (x, w))
         _on_device(x, lambda: _matmul(_aligned(x), _aligned_weights(w), offsets, out))
-        torch.autograd.graph.increment_version(out)
+        _written(out)
         return out
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _on_device(x, lambda: _GroupedMatmul.apply(x, w, offsets))
@@ -246,5 +247,5 @@ def grouped_outer(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, *,
         _check_out(out, (groups, a.shape[1], b.shape[1]), a, "out", (a, b))
     result = _on_device(a, lambda: _outer(_aligned(a), _aligned(b), offsets, groups, out))
     if out is not None:
-        torch.autograd.graph.increment_version(out)
+        _written(out)
     return result

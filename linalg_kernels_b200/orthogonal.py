@@ -189,11 +189,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     contiguous rows or columns is copied first). coefficients: ``(a, b, c)``, or one triple for
     each of the ``steps``. The Frobenius norm is taken in 64 bits. precision: ``"half"`` works in
     fp16 with FP32 sums (an error of ~1e-3 of the result's norm, below bfloat16's own rounding),
-    ``"full"`` in split fp16 (~4e-6, three times the products); None takes ``"half"`` for
+    ``"full"`` in split fp16 (~2e-6, as FP32 products would; three times the products); None takes ``"half"`` for
     bfloat16 and ``"full"`` otherwise. out: written and returned instead of a new tensor; may
     be ``x`` itself.
 
-    A zero matrix gives zeros; a matrix with a NaN or an infinity gives NaN and leaves the
+    A zero matrix gives zeros (with eps > 0); a matrix with a NaN or an infinity gives NaN and leaves the
     others of the batch alone. It has no derivative: call it under ``torch.no_grad()`` or on a
     detached tensor.
     """
@@ -206,7 +206,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     _remember(steps, coefficients, eps, precision, coef)
     if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
         raise RuntimeError("orthogonalize has no derivative: call it under torch.no_grad()")
-    if out is None:
+    given = out is not None
+    if not given:
         out = (torch.empty_like(x.transpose(-2, -1), memory_format=torch.contiguous_format)
                .transpose(-2, -1) if _is_transposed(x)
                else torch.empty_like(x, memory_format=torch.contiguous_format))
@@ -235,8 +236,16 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
             ws.data_ptr() if need else 0, need, _lib.current_queue(x.device), eps, coef)
 
     _lib.check(_on_device(x, call), "linalg_orthogonalize")
-    torch.autograd.graph.increment_version(out)
+    if given:
+        _written(out)
     return out
+
+
+def _written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that they were written in place (inference tensors keep no versions)."""
+    tracked = [t for t in tensors if not t.is_inference()]
+    if tracked:
+        torch.autograd.graph.increment_version(tracked)
 
 
 _single: bool | None = None
@@ -323,5 +332,5 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
             1.0 - lr * weight_decay, lr * scale, eps, coef)
 
     _lib.check(_on_device(param, call), "linalg_muon_update")
-    torch.autograd.graph.increment_version((param, momentum))
+    _written(param, momentum)
     return param

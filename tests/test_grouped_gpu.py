@@ -270,6 +270,26 @@ def test_graph_replays_other_group_sizes():
     _close(dw, want, size, 160)
 
 
+def test_capture_with_few_rows_and_inference_mode():
+    x, w = _randn(1, 40, 128), _randn(2, 8, 128, 192)
+    offsets = torch.tensor([0, 3, 3, 10, 12, 20, 25, 30, 38], device=DEV, dtype=torch.int32)
+    grouped_matmul(x, w, offsets)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = grouped_matmul(x, w, offsets)
+    offsets.copy_(torch.tensor([1, 1, 2, 30, 31, 31, 32, 39, 40], device=DEV))
+    x.mul_(2)
+    graph.replay()
+    want, size = _reference(x, w, offsets.tolist())
+    _close(y, want, size, 128)
+    with torch.inference_mode():
+        out = torch.empty(40, 192, device=DEV, dtype=torch.bfloat16)
+        grouped_matmul(x, w, offsets, out=out)
+        assert torch.equal(grouped_matmul(x, w, offsets)[1:], out[1:])
+        grouped_outer(x, out, offsets, out=torch.empty(8, 128, 192, device=DEV, dtype=torch.bfloat16))
+
+
 def test_two_queues():
     x, w = _randn(1, 900, 256), _randn(2, 6, 256, 512)
     offs = [torch.tensor(o, device=DEV) for o in ([0, 5, 300, 300, 600, 880, 900],

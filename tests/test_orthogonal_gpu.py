@@ -282,6 +282,32 @@ def test_two_queues_and_graph():
     assert torch.equal(param, ref) and torch.equal(mom, ref_m)
 
 
+@pytest.mark.parametrize("shape", [(3, 64, 64), (2, 100, 900), (2, 200, 256), (2, 300, 260)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_capture_of_every_kernel(shape, dtype):
+    """One launch per tile, clusters, pairs and the products, captured and replayed twice."""
+    x, other = _input(1, shape, dtype), _input(2, shape, dtype)
+    want = orthogonalize(other)
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = orthogonalize(static)
+    static.copy_(other)
+    for _ in range(2):
+        y.zero_()
+        graph.replay()
+        assert torch.equal(y, want)
+
+
+def test_inference_mode():
+    with torch.inference_mode():
+        x = _input(1, (2, 60, 70), torch.bfloat16)
+        y = orthogonalize(x)
+        assert torch.equal(orthogonalize(x, out=torch.empty_like(x)), y)
+        p, m = x.clone(), torch.zeros(2, 60, 70, device=DEV)
+        muon_update_(p, x, m, lr=0.1)
+
+
 def test_large_batch_past_32_bit_offsets():
     """The last matrix of an input longer than 2^31 elements gets its own result."""
     batch, m, n = 130, 2048, 8200
