@@ -13,20 +13,27 @@ struct Matrix {
   int vec;  // rows of 8 elements can be accessed 16 bytes at a time
 };
 
-template <typename T>
-__device__ __forceinline__ void load8t(const T* p, float (&v)[8], int count, bool vec) {
-  if (vec && count == 8) {
-    alignas(16) T h[8];
-#pragma unroll
-    for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-      reinterpret_cast<uint4*>(h)[j] = reinterpret_cast<const uint4*>(p)[j];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_float(h[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
-  }
+inline Matrix device_matrix(const linalg_matrix* x) {
+  Matrix d{x->data, x->ld, x->stride, x->type, 0};
+  const int per16 = x->type == LINALG_FP32 ? 4 : 8;
+  d.vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->ld % per16 == 0 &&
+          x->stride % per16 == 0;
+  return d;
 }
+// Which instance reads (in: 1 bf16 with a momentum of fp32 or none, 2 fp32 with fp32 or none, 3 bf16
+// with bf16) or writes (out: 1 bf16, 2 fp32) the matrices in whole aligned chunks of eight columns;
+// 0: the one for any types, alignment and number of columns.
+inline int input_path(const Matrix& x, const Matrix* momentum, int64_t n) {
+  if (n % 8 || !x.vec || (momentum != nullptr && !momentum->vec)) return 0;
+  const int m = momentum == nullptr ? LINALG_FP32 : momentum->type;
+  if (x.type == LINALG_BF16) return m == LINALG_FP32 ? 1 : (m == LINALG_BF16 ? 3 : 0);
+  return x.type == LINALG_FP32 && m == LINALG_FP32 ? 2 : 0;
+}
+inline int output_path(const Matrix& x, int64_t n) {
+  if (n % 8 || !x.vec) return 0;
+  return x.type == LINALG_BF16 ? 1 : (x.type == LINALG_FP32 ? 2 : 0);
+}
+
 template <typename T>
 __device__ __forceinline__ void store8t(T* p, float (&v)[8], int count, bool vec) {
   alignas(16) T h[8];
@@ -44,14 +51,6 @@ __device__ __forceinline__ void store8t(T* p, float (&v)[8], int count, bool vec
     for (int j = 0; j < 8; ++j)
       if (j < count) p[j] = h[j];
   }
-}
-__device__ __forceinline__ void load_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
-  if (x.type == LINALG_BF16)
-    load8t(static_cast<const __nv_bfloat16*>(x.data) + at, v, count, x.vec);
-  else if (x.type == LINALG_FP16)
-    load8t(static_cast<const __half*>(x.data) + at, v, count, x.vec);
-  else
-    load8t(static_cast<const float*>(x.data) + at, v, count, x.vec);
 }
 __device__ __forceinline__ void store_any(const Matrix& x, int64_t at, float (&v)[8], int count) {
   if (x.type == LINALG_BF16)

@@ -223,14 +223,6 @@ bool valid_matrix(const linalg_matrix* x, int64_t batch, int64_t m, int64_t n) {
   return true;
 }
 
-Matrix device_matrix(const linalg_matrix* x) {
-  Matrix d{x->data, x->ld, x->stride, x->type, 0};
-  const int per16 = 16 / type_bytes(x->type);
-  d.vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->ld % per16 == 0 &&
-          x->stride % per16 == 0;
-  return d;
-}
-
 // Bytes from the first to one past the last element.
 void extent(const linalg_matrix* x, int64_t batch, int64_t m, int64_t n, uintptr_t* lo,
             uintptr_t* hi) {
@@ -276,12 +268,7 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   p.rows = m, p.n = int(n);
   p.chunks_row = int((n + 7) / 8);
   p.chunks = m * p.chunks_row;
-  if (n % 8 == 0 && p.x.vec) {
-    const bool mo32 = !muon || (momentum->type == LINALG_FP32 && p.momentum.vec);
-    const bool mo16 = muon && momentum->type == LINALG_BF16 && p.momentum.vec;
-    if (x->type == LINALG_BF16) p.path = mo32 ? 1 : (mo16 ? 3 : 0);
-    if (x->type == LINALG_FP32) p.path = mo32 ? 2 : 0;
-  }
+  p.path = input_path(p.x, muon ? &p.momentum : nullptr, n);
   p.parts = int(prep_parts(batch, m, n));
   p.sums = reinterpret_cast<double*>(w + l.total - l.sums_bytes);
   p.planes = xs[0];

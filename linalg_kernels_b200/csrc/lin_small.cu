@@ -12,6 +12,7 @@
 // and share of the columns.
 //
 //   per step:  G = X X^T -> mask, fp16   |   B = a I + b G + c G G -> fp16   |   X <- B X
+//   (the diagonals of G and B stay in FP32, see below)
 //
 // A long matrix is split over a cluster of 2, 4 or 8 CTAs by columns. Only G needs all columns:
 // each CTA writes its FP32 partials to the CTAs that own their columns, which sum them in rank
@@ -21,7 +22,10 @@
 // covers at most 192 columns of K, so it needs no drain.
 //
 // Bound by latency: per step three dependent chains MMA -> TMEM read -> convert -> shared memory,
-// MEASURED_SMALL
+// ~4400 cycles for a 128 x 128 tile (2000 of them MMAs), beside ~9000 for reading and the norm and
+// ~5000 for writing. One 128 x 128 matrix takes 21 us (the products of lin_gemm.cu, 17 launches,
+// took 86), 1024 of 64 x 64 take 35 us, 0.48 TB/s (423 us), an optimiser step on 512 x 128
+// in full precision over 4 CTAs 76 us (203 us).
 #include "lin_chip.cuh"
 #include "lin_small.cuh"
 
@@ -43,9 +47,7 @@ struct SmallArgs {
   int ranks;         // CTAs per cluster
   int steps;
   int nesterov;
-  int in_path, out_path;  // 0: any types and alignment; else whole aligned chunks of these types:
-                          // in 1 bf16 (momentum fp32), 2 fp32 (fp32), 3 bf16 (bf16); out 1 bf16,
-                          // 2 fp32
+  int in_path, out_path;
   float beta, gain, decay, rate;
   float scale, eps;       // of X; G has scale^2, B 1
   float inv_gram, inv_x;  // their reciprocals
@@ -269,7 +271,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
   double* warp_sum = reinterpret_cast<double*>(es);  // [T / 32] (CLUSTER: before es is used)
   double* mat_sum = reinterpret_cast<double*>(es + (CLUSTER ? 65536 : 128));  // [8] per matrix
   float2* factor = reinterpret_cast<float2*>(mat_sum + 8);  // [8]
-  uint64_t* bar = reinterpret_cast<uint64_t*>(factor + 8);
+  float* diag = reinterpret_cast<float*>(factor + 8);  // [128] half precision: G's diagonal
+  float* own = diag + 128;                             // [128] and what a row of X is scaled with
+  uint64_t* bar = reinterpret_cast<uint64_t*>(own + 128);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -388,13 +392,23 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
           const int c0 = q * 32 + h * 16;
           tmem_ld16(tmem + lane_base + uint32_t(c0), v);
           // 16 columns are of one matrix: the pitch is a multiple of 16
-          const bool own = uint32_t(c0 - in_tile * g.pitch) < uint32_t(g.pitch);
+          const bool mine = uint32_t(c0 - in_tile * g.pitch) < uint32_t(g.pitch);
+          if (!SPLIT && q * 32 == q32) {  // the same for the whole warp (selects: no branches)
+            float d = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const bool here = c0 + j == row;
+              d = here ? v[j] : d;
+              v[j] = here ? 0.f : v[j];
+            }
+            if (uint32_t(row - c0) < 16u) diag[row] = d;
+          }
 #pragma unroll
           for (int j = 0; j < 16; j += 8) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              y[e] = own ? v[j + e] : 0.f;
+              y[e] = mine ? v[j + e] : 0.f;
               if (KEEP) gram[KEEP ? h * 16 + j + e : 0] = y[e];
             }
             uint4 hi, lo;
@@ -439,9 +453,18 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
           y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
         }
         const int mt = rr / g.pitch;
-        const bool own = uint32_t(c0 - mt * g.pitch) < uint32_t(g.pitch);
+        const bool mine = uint32_t(c0 - mt * g.pitch) < uint32_t(g.pitch);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = own ? y[e] : 0.f;
+        for (int e = 0; e < 8; ++e) y[e] = mine ? y[e] : 0.f;
+        if (!SPLIT && uint32_t(rr - c0) < 8u) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            d = c0 + e == rr ? y[e] : d;
+            y[e] = c0 + e == rr ? 0.f : y[e];
+          }
+          for (int o = 0; o < g.ranks; ++o) st_remote_f32(remote(smem_u32(diag + rr), o), d);
+        }
         uint4 hi, lo;
         round8v<SPLIT>(y, hi, lo);
         const uint32_t to = smem_u32(gs) + chunk_at(rr, c0);
@@ -471,10 +494,13 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
-    // half precision: B takes a on its diagonal (its scale is 1), so that X <- B X needs no old X: one
-    // more rounding of 2^-12 per row, as X's own, for half of that epilogue's instructions. Full:
-    // a X is added in FP32 at the end, not summed by the tensor core, whose rounding towards zero
-    // would weigh on the largest term; and B keeps 22 bits with a scale of 2048.
+    // Half precision: G and B in shared memory are without their diagonals D, whose rounding would
+    // be the largest error by far (small matrices have few entries to average it, and X X^T of
+    // a wide one is nearly a multiple of I: 32 x 4096 was 4.4e-3 off, now ~1e-3). With G = D + O,
+    //   (G G)_ij = (O O)_ij + (d_i + d_j) O_ij  off the diagonal,  (O O)_ii + d_i^2  on it,
+    // and the diagonal of a I + b G + c G G scales the rows of X in FP32 at the end.
+    // Full: a X is added in FP32 at the end, not summed by the tensor core, whose rounding towards
+    // zero would weigh on the largest term; and B keeps 22 bits with a scale of 2048.
     constexpr float kPoly = SPLIT ? 2048.f : 1.f;
     const float fb = cb * g.inv_gram * kPoly, fc = cc * g.inv_gram * g.inv_gram * kPoly;
 #pragma unroll
@@ -486,35 +512,48 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
         float v[16];
         const int c0 = q * 32 + h * 16;
         tmem_ld16(tmem + lane_base + uint32_t(c0), v);
-        const int diag = row - c0;  // this row's diagonal element, if in these columns
-        if (CLUSTER || !KEEP) {
+        if (!SPLIT && q * 32 == q32) {
+          float oo = 0.f;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] *= fc;
+          for (int j = 0; j < 16; ++j) oo = c0 + j == row ? v[j] : oo;
+          if (uint32_t(row - c0) < 16u) {
+            const float d = diag[row];
+            own[row] = ca + fb * d + fc * (oo + d * d);
+          }
         }
+        const float di = SPLIT ? 0.f : fmaf(fc, diag[row], fb);
 #pragma unroll
         for (int j = 0; j < 16; j += 8) {
           float y[8];
           const uint32_t at = chunk_at(row, c0 + j);
-          if (!CLUSTER && KEEP) {
+          if (SPLIT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = v[j + e] * fc;
+            add8(y, *reinterpret_cast<const uint4*>(gs + at), fb);
+            add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), fb);
+          } else {
+            const float4 d0 = *reinterpret_cast<const float4*>(diag + c0 + j);
+            const float4 d1 = *reinterpret_cast<const float4*>(diag + c0 + j + 4);
+            const float dj[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+            const uint4 w = KEEP ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(gs + at);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-              const float2 t = chol::ffma2(
-                  make_float2(gram[KEEP ? h * 16 + j + e : 0], gram[KEEP ? h * 16 + j + e + 1 : 0]),
-                  make_float2(fb, fb), make_float2(0.f, 0.f));
-              const float2 x = chol::ffma2(make_float2(v[j + e], v[j + e + 1]), make_float2(fc, fc), t);
-              y[e] = x.x;
-              y[e + 1] = x.y;
+              const float2 o =
+                  KEEP ? make_float2(gram[KEEP ? h * 16 + j + e : 0],
+                                     gram[KEEP ? h * 16 + j + e + 1 : 0])
+                       : __half22float2(*reinterpret_cast<const __half2*>(&ws[e / 2]));
+              const float2 f = chol::ffma2(make_float2(fc, fc), make_float2(dj[e], dj[e + 1]),
+                                           make_float2(di, di));  // fb + fc (d_i + d_j)
+              const float2 t = chol::ffma2(f, o, make_float2(0.f, 0.f));
+              const float2 r = chol::ffma2(make_float2(v[j + e], v[j + e + 1]), make_float2(fc, fc), t);
+              y[e] = r.x;
+              y[e + 1] = r.y;
             }
-          } else {
+            if (q * 32 == q32) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = v[j + e];
-            add8(y, *reinterpret_cast<const uint4*>(gs + at), fb);
-            if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(gs + g_plane + at), fb);
-          }
-          if (!SPLIT && q * 32 == q32) {  // the same for the whole warp
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              y[e] += j + e == diag ? ca : 0.f;  // a select: branches would part the warp
+              for (int e = 0; e < 8; ++e) y[e] = c0 + j + e == row ? 0.f : y[e];
+            }
           }
           uint4 hi, lo;
           round8v<SPLIT>(y, hi, lo);
@@ -544,6 +583,7 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
       mma_commit(bar);
     }
     wait();
+    const float row_factor = SPLIT ? ca : own[row];
     if (step + 1 < g.steps) {
       for (int c0 = part * 32; c0 < g.cta_cols; c0 += PARTS * 32) {
 #pragma unroll
@@ -556,10 +596,8 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
             const uint32_t at = chunk_at(row, c0 + h * 16 + j);
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = SPLIT ? v[j + e] * (1.f / kPoly) : v[j + e];
-            if (SPLIT) {
-              add8(y, *reinterpret_cast<const uint4*>(xs + at), ca);
-              add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca);
-            }
+            add8(y, *reinterpret_cast<const uint4*>(xs + at), row_factor);
+            if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca);
             uint4 hi, lo;
             round8v<SPLIT>(y, hi, lo);
             *reinterpret_cast<uint4*>(xs + at) = hi;
@@ -584,11 +622,9 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
           float y[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = v[j + e] * (g.inv_x / kPoly);
-          if (SPLIT) {
-            const uint32_t at = chunk_at(row, c0 + j);
-            add8(y, *reinterpret_cast<const uint4*>(xs + at), ca * g.inv_x);
-            add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca * g.inv_x);
-          }
+          const uint32_t at = chunk_at(row, c0 + j);
+          add8(y, *reinterpret_cast<const uint4*>(xs + at), row_factor * g.inv_x);
+          if (SPLIT) add8(y, *reinterpret_cast<const uint4*>(xs + x_plane + at), ca * g.inv_x);
           if (g.tall) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) stage[(h * 32 + j + e) * 128 + row] = y[e];
@@ -630,7 +666,7 @@ constexpr int kMaxSmem = 227 * 1024;
 size_t smem_bytes(bool split, int ranks, int cta_cols) {
   size_t b = size_t(split ? 2 : 1) * (size_t(cta_cols / 64) + 2) * kBlockBytes;
   b += ranks > 1 ? 65536 : 128;
-  b += 8 * 8 + 8 * 8 + 16 + 1008;  // 1008: to a 1024-byte boundary from a 16-byte one
+  b += 8 * 8 + 8 * 8 + 2 * 128 * 4 + 16 + 1008;  // 1008: to a 1024-byte boundary from a 16-byte one
   // CTAs of different clusters on one SM could wait for each other's TMEM: one CTA per SM
   if (ranks > 1 && b < 118 * 1024) b = 118 * 1024;
   return b;
@@ -657,14 +693,6 @@ int launch(const SmallArgs& g, int64_t tiles, size_t smem, cudaStream_t q) {
       cudaLaunchKernelEx(&cfg, small_kernel<T, SPLIT, MUON, CLUSTER>, g, chol::device_status_ptr()));
 }
 
-Matrix device_side(const linalg_matrix* x) {
-  Matrix d{x->data, x->ld, x->stride, x->type, 0};
-  const int per16 = x->type == LINALG_FP32 ? 4 : 8;
-  d.vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->ld % per16 == 0 &&
-          x->stride % per16 == 0;
-  return d;
-}
-
 }  // namespace
 
 #define LIN_FOR_EACH_SMALL(F) \
@@ -687,9 +715,9 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
                  float rate, int steps, const float* coefficients, float eps, bool split,
                  cudaStream_t q) {
   SmallArgs g{};
-  g.x = device_side(x);
-  if (momentum != nullptr) g.momentum = device_side(momentum);
-  g.out = device_side(out);
+  g.x = device_matrix(x);
+  if (momentum != nullptr) g.momentum = device_matrix(momentum);
+  g.out = device_matrix(out);
   g.tall = m > n;
   g.s = int(g.tall ? n : m), g.len = int(g.tall ? m : n);
   g.pitch = (g.s + 15) / 16 * 16;
@@ -703,14 +731,8 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
   const int chunk = (g.len + g.ranks - 1) / g.ranks;
   g.cta_cols = (chunk + 63) / 64 * 64;
   g.steps = steps;
-  if (n % 8 == 0) {
-    const bool mo32 = momentum == nullptr || (momentum->type == LINALG_FP32 && g.momentum.vec);
-    const bool mo16 = momentum != nullptr && momentum->type == LINALG_BF16 && g.momentum.vec;
-    if (g.x.vec && x->type == LINALG_BF16) g.in_path = mo32 ? 1 : (mo16 ? 3 : 0);
-    if (g.x.vec && x->type == LINALG_FP32) g.in_path = mo32 ? 2 : 0;
-    if (g.out.vec && out->type == LINALG_BF16) g.out_path = 1;
-    if (g.out.vec && out->type == LINALG_FP32) g.out_path = 2;
-  }
+  g.in_path = input_path(g.x, momentum != nullptr ? &g.momentum : nullptr, n);
+  g.out_path = output_path(g.out, n);
   g.beta = float(beta), g.gain = float(1.0 - beta), g.nesterov = nesterov;
   g.decay = decay, g.rate = rate;
   g.scale = split ? 64.f : 32.f, g.eps = eps;

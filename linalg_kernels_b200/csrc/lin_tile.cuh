@@ -78,18 +78,6 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "memory");
   return ok != 0;
 }
-// Whether the phase has completed, without waiting (try_wait suspends the thread for a while).
-__device__ __forceinline__ bool test_bar(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // The same without ordering memory: for a drained accumulator, whose reads tcgen05.wait::ld and
 // tcgen05.fence::before_thread_sync have ordered (a release costs ~1000 cycles here).
 __device__ __forceinline__ void arrive_leader_relaxed(uint32_t addr) {
@@ -360,7 +348,6 @@ __device__ __forceinline__ void write_direct(const Out& g, float (&v)[32], int l
 // The epilogue of one warp's 32 rows x COLS columns (a multiple of 64).
 template <int COLS, int BUFS, bool SPLIT>
 struct WarpEpilogue {
-  static constexpr int P = SPLIT ? 2 : 1;
   static constexpr int BOXES = COLS / 64;
   static_assert(!SPLIT || (BOXES == 1 && BUFS == 2), "planes take a buffer each");
   uint8_t* bufs;        // BUFS boxes of this warp, 1024-byte aligned
