@@ -22,10 +22,11 @@
 // covers at most 192 columns of K, so it needs no drain.
 //
 // Bound by latency: per step three dependent chains MMA -> TMEM read -> convert -> shared memory,
-// ~4400 cycles for a 128 x 128 tile (2000 of them MMAs), beside ~9000 for reading and the norm and
-// ~5000 for writing. One 128 x 128 matrix takes 21 us (the products of lin_gemm.cu, 17 launches,
-// took 86), 1024 of 64 x 64 take 35 us, 0.48 TB/s (423 us), an optimiser step on 512 x 128
-// in full precision over 4 CTAs 76 us (203 us).
+// ~5500 cycles for a 128 x 128 tile (2000 of them MMAs), beside ~9000 for reading and the norm and
+// ~5000 for writing. One 128 x 128 matrix takes 25 us (the products of lin_gemm.cu, 17 launches,
+// took 86), 1024 of 64 x 64 take 43 us, 0.39 TB/s (423 us), an optimiser step on 512 x 128
+// in full precision over 4 CTAs 78 us (203 us). The diagonals in FP32 cost 3.5 us of the 25 and
+// 8 us of the 43.
 #include "lin_chip.cuh"
 #include "lin_small.cuh"
 
