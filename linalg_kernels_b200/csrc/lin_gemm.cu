@@ -156,7 +156,15 @@ struct Walker {
       w.k0 = start[w.index];
       w.k_len = start[w.index + 1] - w.k0;
     }
-    if (g.symmetric) {
+    if (g.symmetric < 0) {
+      // BN = 512: row tile tm holds tm / 2 + 1 column tiles; rows 2i and 2i + 1 start at i (i + 1)
+      int i = int((sqrtf(4.f * float(r) + 1.f) - 1.f) * 0.5f);
+      while (i * (i + 1) > r) --i;
+      while ((i + 1) * (i + 2) <= r) ++i;
+      const int rem = r - i * (i + 1);
+      w.tm = 2 * i + (rem > i);
+      w.tn = rem > i ? rem - i - 1 : rem;
+    } else if (g.symmetric) {
       // row tile tm holds min(ratio * (tm + 1), tiles_n) column tiles; ratio = 256 / BN
       const int ratio = g.symmetric;
       int tm = int((sqrtf(8.f * float(r / ratio) + 1.f) - 1.f) * 0.5f);
@@ -181,8 +189,13 @@ struct Walker {
 
 // Epilogue buffers per warp: two hold C's boxes (and the two planes) of a batch's products; ragged
 // products have no C and need the group tables' space.
+template <int BN, int MODE>
+constexpr int kBuffers = BN == 512 ? 1 : (MODE == kBatch || BN == 128 ? 2 : 1);
+constexpr int kWideGroups = 124;  // groups whose tables fit beside BN = 512's stages
+template <int BN>
+constexpr int kTableEntries = (BN == 512 ? kWideGroups : kMaxGroups) + 4;
 template <int BN, int MODE, bool SPLIT>
-using ProductCfg = Cfg<BN, MODE == kBatch || BN == 128 ? 2 : 1, MODE == kBatch ? 0 : kTableBytes,
+using ProductCfg = Cfg<BN, kBuffers<BN, MODE>, MODE == kBatch ? 0 : 2 * kTableEntries<BN> * 4,
                        SPLIT ? 2 : 1>;
 
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
@@ -194,7 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                    const __grid_constant__ CUtensorMap map_c, const Args g, int* status) {
   using C = ProductCfg<BN, MODE, SPLIT>;
   constexpr int S = C::STAGES;
-  constexpr int kBufs = MODE == kBatch || BN == 128 ? 2 : 1;
+  constexpr int kBufs = kBuffers<BN, MODE>;
+  constexpr bool WIDE = BN == 512;
+  constexpr int HALVES = WIDE ? 2 : 1;  // accumulators of one tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -209,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* c_bars = clean + S;      // [2 * kEpiWarps] C's boxes
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_bars + 2 * kEpiWarps);
   int* start = reinterpret_cast<int*>(smem + size_t(S) * C::STAGE + C::EPI + 512);
-  int* first = start + kMaxGroups + 4;
+  int* first = start + kTableEntries<BN>;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -263,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         walk.at(t, w);
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
         const int a_row = w.row0 + w.tm * kTileM + int(rank) * 128;
-        const int b_row = w.tn * BN + int(rank) * (BN / 2);
+        const int b_row = w.tn * BN + int(rank) * (WIDE ? 128 : BN / 2);
         constexpr int planes = SPLIT ? 2 : 1;
         const int za = MODE == kBatch ? w.index * planes : 0;
         const int zb = MODE == kRaggedK ? 0 : w.index * planes;
@@ -296,11 +311,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             } else {
               tma_load_pair(pa, &map_a, kx, a_row, za + p, bar);
             }
-            if (BMN) {
-              tma_load_pair(pb, &map_b, b_row, kx, zb + p, bar);
-              if (BN == 256) tma_load_pair(pb + 8192, &map_b, b_row + 64, kx, zb + p, bar);
-            } else {
-              tma_load_pair(pb, &map_b, kx, b_row, zb + p, bar);
+#pragma unroll
+            for (int d = 0; d < HALVES; ++d) {
+              const int row = b_row + d * 256;
+              if (BMN) {
+                tma_load_pair(pb + d * 16384, &map_b, row, kx, zb + p, bar);
+                if (BN >= 256) tma_load_pair(pb + d * 16384 + 8192, &map_b, row + 64, kx, zb + p, bar);
+              } else {
+                tma_load_pair(pb + d * 16384, &map_b, kx, row, zb + p, bar);
+              }
             }
           }
         }
@@ -321,6 +340,62 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         walk.at(t, w);
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
         if (num_k == 0) continue;
+        if constexpr (WIDE) {
+          // Two accumulators of one tile. The first blocks are summed into D0 while the epilogue
+          // still drains the last tile's D1, and the last blocks into D0 before D1, so that the
+          // epilogue starts on D0 under D1's MMAs: as many blocks as there are stages.
+          auto ready = [&](int kb) {
+            ok = ok && wait_bar(&full[(kt + kb) % S], ((kt + kb) / S) & 1u, status);
+            tc_fence_after();
+            return ok;
+          };
+          auto block = [&](int kb, int d) {
+            const uint8_t* sa = smem + size_t((kt + kb) % S) * C::STAGE;
+            const uint8_t* sb = sa + C::A_BYTES + d * 16384;
+            const uint64_t da = AMN ? sw128_desc_mn(sa) : sw128_desc(sa);
+            const uint64_t db = BMN ? sw128_desc_mn(sb) : sw128_desc(sb);
+            const int left = w.k_len - kb * kBlockK;
+            const int slabs = left >= kBlockK ? kBlockK / 16 : (left + 15) / 16;
+#pragma unroll
+            for (int kk = 0; kk < kBlockK / 16; ++kk) {
+              if (kk >= slabs) break;
+              mma_pair(tmem + d * 256u, da + uint64_t(kk * (AMN ? 2048 : 32) / 16),
+                       db + uint64_t(kk * (BMN ? 2048 : 32) / 16), g.idesc, (kb | kk) ? 1u : 0u);
+            }
+          };
+          auto drained = [&](int d) {
+            if (round > 0) ok = ok && wait_bar(&tempty[d], (round - 1) & 1u, status);
+            tc_fence_after();
+          };
+          const int lead = num_k < S ? num_k : S;
+          const int tail = num_k - S > lead ? num_k - S : lead;
+          drained(0);
+          for (int kb = 0; kb < lead && ok; ++kb)
+            if (ready(kb)) block(kb, 0);
+          if (ok && tail == num_k) commit_pair(&tfull[0]);
+          drained(1);
+          for (int kb = 0; kb < lead && ok; ++kb) {
+            block(kb, 1);
+            commit_pair(&empty[(kt + kb) % S]);
+          }
+          for (int kb = lead; kb < tail && ok; ++kb)
+            if (ready(kb)) {
+              block(kb, 0);
+              block(kb, 1);
+              commit_pair(&empty[(kt + kb) % S]);
+            }
+          for (int kb = tail; kb < num_k && ok; ++kb)
+            if (ready(kb)) block(kb, 0);
+          if (ok && tail < num_k) commit_pair(&tfull[0]);
+          for (int kb = tail; kb < num_k && ok; ++kb) {
+            block(kb, 1);
+            commit_pair(&empty[(kt + kb) % S]);
+          }
+          if (ok) commit_pair(&tfull[1]);
+          kt += uint32_t(num_k);
+          ++round;
+          continue;
+        }
         const int rounds = SPLIT ? num_k : 1;  // split: an accumulator per K block
         for (int r = 0; r < rounds && ok; ++r, ++round) {
           const uint32_t buf = round & 1u;
@@ -401,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; half of the columns
-    constexpr int kCols = BN / 2;
+    constexpr int kCols = WIDE ? 128 : BN / 2;  // of one accumulator
     using Epi = WarpEpilogue<kCols, kBufs, SPLIT>;
     Epi ep{epi + (warp - 4) * kBufs * kBoxBytes, c_bars + 2 * (warp - 4), 0u, lane};
     uint32_t round = 0;
@@ -435,7 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
         };
 #pragma unroll 1
-        for (int c = 0; c < kCols; c += 64) {
+        for (int i = 0; i < HALVES * kCols; i += 64) {
+          const int c = i < kCols ? i : i - kCols + 256;
           if (by_box) {
             ep.template box<false>(o, c / 64, row_base, col0 + c, false, status, zeros);
           } else {
@@ -450,6 +526,43 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         continue;
       }
       bool ok = true;
+      if constexpr (WIDE) {
+#pragma unroll 1
+        for (int d = 0; d < 2 && ok; ++d) {
+          ok = wait_bar(&tfull[d], round & 1u, status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t acc = tmem + uint32_t(d * 256 + half * kCols) + (uint32_t(q * 32) << 16);
+          // of a symmetric result only the 256-wide blocks on and below the diagonal are written
+          // here (those below twice)
+          const int block = w.tn * 2 + d;
+          if (!(kC && g.symmetric && block > w.tm)) {
+            if (by_box) {
+#pragma unroll 1
+              for (int b = 0; b < Epi::BOXES; ++b)
+                ep.template box<kC>(o, b, row_base, col0 + d * 256 + b * 64,
+                                    kC && g.symmetric && block < w.tm, status,
+                                    [&](int h, float (&v)[32]) {
+                                      tmem_ld32(acc + uint32_t(b * 64 + h * 32), v);
+                                    });
+            } else if constexpr (!kC) {
+#pragma unroll 1
+              for (int c = 0; c < kCols; c += 32) {
+                float v[32];
+                tmem_ld32(acc + uint32_t(c), v);
+                ep.direct(o, row_base, col0 + d * 256 + c, v);
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_leader_relaxed(leader_addr(&tempty[d]));
+        }
+        if (!ok) break;
+        ++round;
+        continue;
+      }
       if (kC || SPLIT) ep.load_c(o, row_base, col0);
       if constexpr (SPLIT) {
         float sum[2][32];
@@ -536,7 +649,7 @@ cudaError_t set_smem() {
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 int launch(const Product& p, cudaStream_t q) {
   CUtensorMap ma, mb;
-  if (!make_operand_map(&ma, p.a, p.bf16, 128) || !make_operand_map(&mb, p.b, p.bf16, BN / 2))
+  if (!make_operand_map(&ma, p.a, p.bf16, 128) || !make_operand_map(&mb, p.b, p.bf16, BN == 128 ? 64 : 128))
     return CHOL_ERR_UNSUPPORTED;
   Args g{};
   g.m = int(p.m), g.n = int(p.n), g.k = int(p.k), g.batch = int(p.batch);
@@ -545,10 +658,12 @@ int launch(const Product& p, cudaStream_t q) {
   int64_t per = int64_t(g.tiles_m) * g.tiles_n;
   if (p.symmetric) {
     const int ratio = kTileM / BN;
-    g.symmetric = ratio;
+    g.symmetric = BN == 512 ? -1 : ratio;
     per = 0;
-    for (int tm = 0; tm < g.tiles_m; ++tm)
-      per += ratio * (tm + 1) < g.tiles_n ? ratio * (tm + 1) : g.tiles_n;
+    for (int tm = 0; tm < g.tiles_m; ++tm) {
+      const int row = BN == 512 ? tm / 2 + 1 : ratio * (tm + 1);
+      per += row < g.tiles_n ? row : g.tiles_n;
+    }
   }
   int64_t total = per * p.batch;
   if (MODE == kRaggedM)  // an upper bound: every group may end in a partial tile
@@ -583,7 +698,8 @@ int launch(const Product& p, cudaStream_t q) {
   g.total_rows = int(p.total_rows), g.fill = p.fill;
   const uint32_t type = p.bf16 ? 1u : 0u;
   g.idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(AMN) << 15) |
-            (uint32_t(BMN) << 16) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+            (uint32_t(BMN) << 16) | (uint32_t((BN < 256 ? BN : 256) >> 3) << 17) |
+            (uint32_t(kTileM >> 4) << 24);
   int64_t pairs = g_sms / 2;
   if (pairs > total) pairs = total;
   return chol::status_from(chol::launch_pdl(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
@@ -599,6 +715,27 @@ bool narrow(const Product& p) {
   const int64_t tm = p.mode == kRaggedM ? (p.total_rows + kTileM - 1) / kTileM + p.batch / 2
                                         : ((p.m + kTileM - 1) / kTileM) * p.batch;
   return tm * ((p.n + 255) / 256) < g_sms / 2;
+}
+
+// BN = 512: a quarter less to load per product (48 KB per 1024 cycles of MMAs instead of 64), for an
+// epilogue that is only partly hidden. By cycles per tile: ~730 per block of K at 256 (bound by the
+// loads), ~1060 at 512 and 4500 more for its epilogue.
+bool wide(const Product& p) {
+  if (p.split || p.beta != 0.f || p.n < 512) return false;
+  if (p.mode != kBatch && p.batch > kWideGroups) return false;
+  const int64_t pairs = g_sms / 2;
+  const int64_t tm = p.mode == kRaggedM ? (p.total_rows + kTileM - 1) / kTileM + p.batch / 2
+                                        : (p.m + kTileM - 1) / kTileM;
+  const int64_t count = p.mode == kRaggedM ? 1 : p.batch;
+  int64_t t256 = tm * ((p.n + 255) / 256), t512 = tm * ((p.n + 511) / 512);
+  if (p.symmetric) {
+    t256 = tm * (tm + 1) / 2;
+    t512 = (tm / 2) * (tm / 2 + 1) + (tm & 1) * (tm / 2 + 1);
+  }
+  const int64_t k = p.mode == kRaggedK ? p.total_rows / p.batch : p.k;
+  const int64_t blocks = (k + kBlockK - 1) / kBlockK;
+  auto rounds = [&](int64_t tiles) { return (tiles * count + pairs - 1) / pairs; };
+  return rounds(t512) * (blocks * 1060 + 4500) < rounds(t256) * blocks * 730;
 }
 
 }  // namespace
@@ -628,11 +765,12 @@ int launch_product(const Product& p, cudaStream_t q) {
   const int64_t lim = 0x7fffffffLL - 512;
   if (p.m > lim || p.n > lim || p.k > lim || p.batch > lim || p.total_rows > lim)
     return CHOL_ERR_UNSUPPORTED;
-  const bool small = narrow(p);
+  const bool small = narrow(p), large = !small && wide(p);
 #define LIN_CASE(AMN, BMN, MODE, EPI, SPLIT)                                                \
   if (p.a.mn_major == AMN && p.b.mn_major == BMN && p.mode == MODE && p.epilogue == EPI &&  \
       p.split == SPLIT) {                                                                   \
     if (SPLIT || small) return launch<128, AMN, BMN, MODE, EPI, SPLIT>(p, q);               \
+    if (large) return launch<SPLIT ? 128 : 512, AMN, BMN, MODE, EPI, SPLIT>(p, q);          \
     return launch<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>(p, q);                     \
   }
   LIN_FOR_EACH(LIN_CASE)
@@ -649,7 +787,8 @@ cudaError_t prepare_products() {
     return e;
 #define LIN_SET(AMN, BMN, MODE, EPI, SPLIT)                                                   \
   if ((e = set_smem<128, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;             \
-  if ((e = set_smem<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;
+  if ((e = set_smem<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e; \
+  if ((e = set_smem<SPLIT ? 128 : 512, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;
   LIN_FOR_EACH(LIN_SET)
   LIN_FOR_EACH_SPLIT(LIN_SET)
 #undef LIN_SET

@@ -35,7 +35,7 @@ constexpr int kBoxBytes = 32 * 128;  // one warp's 32 rows x 64 columns of 16 bi
 // operand in a stage.
 template <int BN, int BUFS, int TABLE_BYTES, int PLANES>
 struct Cfg {
-  static constexpr int STAGES = PLANES == 2 ? 3 : (BN == 256 ? 5 : 6);
+  static constexpr int STAGES = PLANES == 2 ? 3 : (BN == 512 ? 4 : (BN == 256 ? 5 : 6));
   static constexpr int A_PLANE = 128 * kBlockK * 2;
   static constexpr int B_PLANE = BN / 2 * kBlockK * 2;
   static constexpr int A_BYTES = PLANES * A_PLANE;
@@ -44,7 +44,7 @@ struct Cfg {
   static constexpr int EPI = kEpiWarps * BUFS * kBoxBytes;
   static constexpr int TABLE = TABLE_BYTES;
   static constexpr size_t SMEM = size_t(STAGES) * STAGE + EPI + 512 + TABLE + 1024;
-  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int TMEM_COLS = BN == 512 ? 512 : 2 * BN;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // group starts and first tiles

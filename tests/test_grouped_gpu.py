@@ -307,6 +307,45 @@ def test_two_queues():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+# pairs' tiles of 512 columns: of the rows' products, of their gradients and of the matrices'
+LARGE = [
+    ([3000, 1, 0, 4000, 4999], 0, 0, 1111, 1300),
+    ([2600, 2600], 0, 0, 1100, 2500),
+    ([1500, 3670], 7, 23, 1100, 2500),
+    ([4001, 3999], 0, 0, 1200, 2568),
+    ([1000] * 15 + [0], 130, 254, 2048, 2056),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"g{len(c[0])}r{sum(c[0])}k{c[3]}n{c[4]}")
+@pytest.mark.parametrize("transposed", [False, True])
+def test_large(case, transposed):
+    x, w, off, rows, k, n = _problem(case, torch.bfloat16, transposed)
+    offsets = torch.tensor(off, device=DEV)
+    x.requires_grad_()
+    w.requires_grad_()
+    y = grouped_matmul(x, w, offsets)
+    dy = _randn(3, rows, n)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x, w, y = x.detach(), w.detach(), y.detach()
+    want, size = _reference(x, w, off)
+    _close(y, want, size, k, "y")
+    want, size = _reference(dy, w.transpose(1, 2), off)
+    _close(dx, want, size, n, "dx")
+    want, size = _reference_outer(x, dy, off)
+    _close(dw, want, size, max(case[0]), "dw")
+    # given results of unaligned rows: not by boxes
+    out = torch.full((rows, n + 3), 2.0, device=DEV, dtype=torch.bfloat16)
+    grouped_matmul(x, w, offsets, out=out[:, 1:n + 1])
+    assert torch.equal(out[off[0]:off[-1], 1:n + 1], y[off[0]:off[-1]])
+    assert (out[:, 0] == 2).all() and (out[:, n + 1:] == 2).all()
+    assert (out[:off[0]] == 2).all() and (out[off[-1]:] == 2).all()
+    big = torch.full((len(off) - 1, k + 1, n + 3), 2.0, device=DEV, dtype=torch.bfloat16)
+    grouped_outer(x, dy, offsets, out=big[:, :k, 1:n + 1])
+    assert torch.equal(big[:, :k, 1:n + 1], dw)
+    assert (big[:, k] == 2).all() and (big[:, :, 0] == 2).all() and (big[:, :, n + 1:] == 2).all()
+
+
 def test_status_word_is_clear():
     import ctypes
     assert _lib.load().chol_status_check(

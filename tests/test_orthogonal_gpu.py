@@ -319,6 +319,34 @@ def test_large_batch_past_32_bit_offsets():
     assert not got[:-1].any()
 
 
+# pairs' tiles of 512 columns: of X X^T, of X^T X, of P X and of X P; ragged edges, a last column tile
+# that lies half outside, odd numbers of row tiles
+LARGE = [(2, 2304, 2600), (2, 2600, 2304), (1, 2600, 2700), (1, 2700, 2600), (7, 1290, 1400),
+         (7, 1400, 1290)]
+
+
+@pytest.mark.parametrize("shape", LARGE)
+def test_large(shape):
+    x = _input(sum(shape), shape, torch.bfloat16, 1e-3)
+    exact, tol = _tolerance(x, x.dtype, True)
+    got = orthogonalize(x)
+    assert _far(got, exact) <= tol
+    assert torch.equal(got, orthogonalize(x))
+
+
+@pytest.mark.parametrize("shape", [(1, 2600, 2700), (1, 2700, 2600)])
+def test_large_update(shape):
+    param = _input(1, shape, torch.bfloat16, 0.02)
+    grad, momentum = _input(2, shape, torch.bfloat16, 1e-3), _input(3, shape, torch.float32, 1e-3)
+    p64, g64 = param.double(), grad.double()
+    muon_update_(param, grad, momentum, lr=0.05, beta=0.9, nesterov=True, weight_decay=0.1)
+    o, tol = _tolerance(0.9 * momentum.double() + 0.1 * g64, torch.float32, True)
+    rate = 0.05 * math.sqrt(max(1.0, shape[-2] / shape[-1]))
+    want = (1 - 0.05 * 0.1) * p64 - rate * o
+    off = (param.double() - want).norm()
+    assert off <= (2.0 ** -8 + 3 * 2.0 ** -24) * want.norm() + rate * tol * o.norm()
+
+
 def test_status_word_is_clear():
     import ctypes
     assert _lib.load().chol_status_check(
