@@ -7,10 +7,13 @@
 // "MN-major" (the output's index contiguous), so X X^T, X^T X, S X, X S, x W, dy W^T and
 // x^T dy all run without a transposed copy.
 //
-// A pair of CTAs computes one 256 x BN tile (BN = 256 or 128): each CTA holds 128 rows of A, BN/2
-// rows of B and 128 x BN of the accumulator. The pair shares B, so a CTA writes and reads 32 KB of
+// A pair of CTAs computes one 256 x BN tile (BN = 512, 256 or 128): each CTA holds 128 rows of A,
+// BN/2 rows of B and 128 x BN of the accumulator. The pair shares B, so a CTA writes and reads 32 KB of
 // shared memory per 64 of K at BN = 256 instead of 48 KB; at 512 cycles of tensor work
 // that is 128 bytes a cycle, what shared memory can give (one CTA alone would need 192).
+//
+// BN = 512 (large products without C): both accumulators hold halves of one tile, D0 and D1, and a
+// CTA loads 48 KB per 64 of K for 1024 cycles of tensor work instead of 32 KB for 512.
 //
 //   warp 0       TMA producer: 128-byte-swizzled boxes of A and B into a ring of stages. Both CTAs'
 //                copies report to the full barrier of the pair's first CTA.
@@ -20,7 +23,8 @@
 //                CTA's part of the last block has landed, zeroes the slab's rows that belong to
 //                the next group (they may hold anything, NaN included). (Passing every stage
 //                through this warp cost the weight gradient of 16384 rows 398 us, against 250.)
-//   warps 4..11  epilogue, overlapped with the next tile (two accumulators): TMEM -> registers ->
+//   warps 4..11  epilogue, overlapped with the next tile (two accumulators; at BN = 512 with the
+//                last blocks' MMAs into D1 and the next tile's first into D0): TMEM -> registers ->
 //                boxes in shared memory -> TMA stores (lin_tile.cuh).
 //
 // The grid is persistent: one pair per two SMs, tiles round-robin. Groups' sizes are read from
@@ -156,25 +160,35 @@ struct Walker {
       w.k0 = start[w.index];
       w.k_len = start[w.index + 1] - w.k0;
     }
-    if (g.symmetric < 0) {
-      // BN = 512: row tile tm holds tm / 2 + 1 column tiles; rows 2i and 2i + 1 start at i (i + 1)
-      int i = int((sqrtf(4.f * float(r) + 1.f) - 1.f) * 0.5f);
-      while (i * (i + 1) > r) --i;
-      while ((i + 1) * (i + 2) <= r) ++i;
-      const int rem = r - i * (i + 1);
-      w.tm = 2 * i + (rem > i);
-      w.tn = rem > i ? rem - i - 1 : rem;
-    } else if (g.symmetric) {
-      // row tile tm holds min(ratio * (tm + 1), tiles_n) column tiles; ratio = 256 / BN
-      const int ratio = g.symmetric;
-      int tm = int((sqrtf(8.f * float(r / ratio) + 1.f) - 1.f) * 0.5f);
-      while (ratio * (tm * (tm + 1) / 2) > r) --tm;
-      while (ratio * ((tm + 1) * (tm + 2) / 2) <= r) ++tm;
-      w.tm = tm;
-      w.tn = r - ratio * (tm * (tm + 1) / 2);
+    if (g.symmetric) {
+      // in the same bands: the columns left of the band's triangle, then the triangle by rows (a step
+      // of 8192 x 8192: 2057 -> 1963 us, by rows alone each 74 tiles read all of X)
+      const int top = row_of(r) / kBand * kBand, left = g.symmetric * top;
+      int t = r - row_first(top);
+      const int h = g.tiles_m - top < kBand ? g.tiles_m - top : kBand;
+      if (t < h * left) {
+        w.tn = t / h;
+        w.tm = top + t - w.tn * h;
+      } else {
+        t -= h * left;
+        w.tm = row_of(t);
+        w.tn = left + t - row_first(w.tm);
+        w.tm += top;
+      }
     } else {
       band(r, g.tiles_m, w);
     }
+  }
+  // Of a symmetric result, row tile tm holds its tiles up to the diagonal: ratio (tm + 1) of them
+  // (the last row fewer, if its last ones lie outside); g.symmetric = ratio = 256 / BN.
+  __device__ __forceinline__ int row_first(int tm) const {  // tiles in the rows above
+    return g.symmetric * (tm * (tm + 1) / 2);
+  }
+  __device__ __forceinline__ int row_of(int r) const {
+    int tm = int((sqrtf(8.f * float(r / g.symmetric) + 1.f) - 1.f) * 0.5f);
+    while (row_first(tm) > r) --tm;
+    while (row_first(tm + 1) <= r) ++tm;
+    return tm;
   }
   // Bands of 8 row tiles, down each column of a band: the tiles in flight at a time then read
   // about as many rows of A as of B (8192^3 by offsets: 882 -> 842 us, 840 -> 777 with B MN-major).
@@ -341,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
         if (num_k == 0) continue;
         if constexpr (WIDE) {
-          // Two accumulators of one tile. The first blocks are summed into D0 while the epilogue
+          // The first blocks are summed into D0 while the epilogue
           // still drains the last tile's D1, and the last blocks into D0 before D1, so that the
           // epilogue starts on D0 under D1's MMAs: as many blocks as there are stages.
           auto ready = [&](int kb) {
@@ -534,25 +548,20 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t acc = tmem + uint32_t(d * 256 + half * kCols) + (uint32_t(q * 32) << 16);
-          // of a symmetric result only the 256-wide blocks on and below the diagonal are written
-          // here (those below twice)
-          const int block = w.tn * 2 + d;
-          if (!(kC && g.symmetric && block > w.tm)) {
-            if (by_box) {
+          const int gc0 = col0 + d * 256;
+          if (by_box) {
 #pragma unroll 1
-              for (int b = 0; b < Epi::BOXES; ++b)
-                ep.template box<kC>(o, b, row_base, col0 + d * 256 + b * 64,
-                                    kC && g.symmetric && block < w.tm, status,
-                                    [&](int h, float (&v)[32]) {
-                                      tmem_ld32(acc + uint32_t(b * 64 + h * 32), v);
-                                    });
-            } else if constexpr (!kC) {
+            for (int b = 0; b < Epi::BOXES; ++b)
+              ep.template box<false>(o, b, row_base, gc0 + b * 64, false, status,
+                                     [&](int h, float (&v)[32]) {
+                                       tmem_ld32(acc + uint32_t(b * 64 + h * 32), v);
+                                     });
+          } else if constexpr (!kC) {
 #pragma unroll 1
-              for (int c = 0; c < kCols; c += 32) {
-                float v[32];
-                tmem_ld32(acc + uint32_t(c), v);
-                ep.direct(o, row_base, col0 + d * 256 + c, v);
-              }
+            for (int c = 0; c < kCols; c += 32) {
+              float v[32];
+              tmem_ld32(acc + uint32_t(c), v);
+              ep.direct(o, row_base, gc0 + c, v);
             }
           }
           tc_fence_before();
@@ -649,7 +658,8 @@ cudaError_t set_smem() {
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 int launch(const Product& p, cudaStream_t q) {
   CUtensorMap ma, mb;
-  if (!make_operand_map(&ma, p.a, p.bf16, 128) || !make_operand_map(&mb, p.b, p.bf16, BN == 128 ? 64 : 128))
+  if (!make_operand_map(&ma, p.a, p.bf16, 128) ||
+      !make_operand_map(&mb, p.b, p.bf16, BN == 128 ? 64 : 128))
     return CHOL_ERR_UNSUPPORTED;
   Args g{};
   g.m = int(p.m), g.n = int(p.n), g.k = int(p.k), g.batch = int(p.batch);
@@ -658,12 +668,10 @@ int launch(const Product& p, cudaStream_t q) {
   int64_t per = int64_t(g.tiles_m) * g.tiles_n;
   if (p.symmetric) {
     const int ratio = kTileM / BN;
-    g.symmetric = BN == 512 ? -1 : ratio;
+    g.symmetric = ratio;
     per = 0;
-    for (int tm = 0; tm < g.tiles_m; ++tm) {
-      const int row = BN == 512 ? tm / 2 + 1 : ratio * (tm + 1);
-      per += row < g.tiles_n ? row : g.tiles_n;
-    }
+    for (int tm = 0; tm < g.tiles_m; ++tm)
+      per += ratio * (tm + 1) < g.tiles_n ? ratio * (tm + 1) : g.tiles_n;
   }
   int64_t total = per * p.batch;
   if (MODE == kRaggedM)  // an upper bound: every group may end in a partial tile
@@ -717,25 +725,25 @@ bool narrow(const Product& p) {
   return tm * ((p.n + 255) / 256) < g_sms / 2;
 }
 
-// BN = 512: a quarter less to load per product (48 KB per 1024 cycles of MMAs instead of 64), for an
-// epilogue that is only partly hidden. By cycles per tile: ~730 per block of K at 256 (bound by the
-// loads), ~1060 at 512 and 4500 more for its epilogue.
+// BN = 512: a quarter less to load per product (48 KB per 1024 cycles of MMAs instead of 64 KB), for
+// an epilogue that is only partly hidden: a tile takes 1.61 times a 256-wide one's time per block
+// of K and 3 blocks more. Measured, 256 -> 512: 8192^3 842 -> 685 us, 4096^3 112 -> 96, 16384 rows
+// in 16 groups, 2048 x 4096: 241 -> 219; the other way 5200 rows in 2 groups, 1100 x 2500: 68 and
+// 86, 32768 in 8, 768 x 2048: 94 and 97. Ragged rows' tile counts are known only nearly, so their
+// rounds count in fractions, with 0.65 for the last one. Symmetric results (and with C) stay at
+// 256: G and B of 4096 x 4096 gained 3 % of a step, of 8192 x 8192 lost 2 %.
 bool wide(const Product& p) {
-  if (p.split || p.beta != 0.f || p.n < 512) return false;
+  if (p.split || p.symmetric || p.beta != 0.f || p.n < 512) return false;
   if (p.mode != kBatch && p.batch > kWideGroups) return false;
-  const int64_t pairs = g_sms / 2;
-  const int64_t tm = p.mode == kRaggedM ? (p.total_rows + kTileM - 1) / kTileM + p.batch / 2
-                                        : (p.m + kTileM - 1) / kTileM;
-  const int64_t count = p.mode == kRaggedM ? 1 : p.batch;
-  int64_t t256 = tm * ((p.n + 255) / 256), t512 = tm * ((p.n + 511) / 512);
-  if (p.symmetric) {
-    t256 = tm * (tm + 1) / 2;
-    t512 = (tm / 2) * (tm / 2 + 1) + (tm & 1) * (tm / 2 + 1);
-  }
-  const int64_t k = p.mode == kRaggedK ? p.total_rows / p.batch : p.k;
-  const int64_t blocks = (k + kBlockK - 1) / kBlockK;
-  auto rounds = [&](int64_t tiles) { return (tiles * count + pairs - 1) / pairs; };
-  return rounds(t512) * (blocks * 1060 + 4500) < rounds(t256) * blocks * 730;
+  const int64_t pairs = g_sms / 2, k = p.mode == kRaggedK ? p.total_rows / p.batch : p.k;
+  const double blocks = double((k + kBlockK - 1) / kBlockK);
+  auto rounds = [&](int64_t bn) {
+    const int64_t tn = (p.n + bn - 1) / bn;
+    if (p.mode == kRaggedM)
+      return double(((p.total_rows + kTileM - 1) / kTileM + p.batch / 2) * tn) / pairs + 0.65;
+    return double(((p.m + kTileM - 1) / kTileM * tn * p.batch + pairs - 1) / pairs);
+  };
+  return rounds(512) * (blocks * 1.61 + 3.0) < rounds(256) * blocks;
 }
 
 }  // namespace

@@ -44,7 +44,7 @@ struct Cfg {
   static constexpr int EPI = kEpiWarps * BUFS * kBoxBytes;
   static constexpr int TABLE = TABLE_BYTES;
   static constexpr size_t SMEM = size_t(STAGES) * STAGE + EPI + 512 + TABLE + 1024;
-  static constexpr int TMEM_COLS = BN == 512 ? 512 : 2 * BN;
+  static constexpr int TMEM_COLS = BN == 512 ? 512 : 2 * BN;  // 512: one tile's, in two halves
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // group starts and first tiles

@@ -314,6 +314,8 @@ LARGE = [
     ([1500, 3670], 7, 23, 1100, 2500),
     ([4001, 3999], 0, 0, 1200, 2568),
     ([1000] * 15 + [0], 130, 254, 2048, 2056),
+    ([3000, 1, 0, 4000, 4999], 3, 6, 2001, 2037),
+    ([3000, 1, 0, 4000, 4999], 300, 6, 2000, 2040),
 ]
 
 
