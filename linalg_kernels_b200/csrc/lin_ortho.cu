@@ -9,13 +9,14 @@
 // Per step 3 m^2 n + m^3 multiply-adds (m the smaller side) instead of the full products'
 // 4 m^2 n + 2 m^3.
 //
-// a stands on B's diagonal, so that the third product reads no old X: one more rounding per row, of
-// the size of X's own.
+// In half precision a stands on B's diagonal, so that the third product reads no old X: one more
+// rounding per row, of the size of X's own. In full precision a X is added in FP32.
 //
 // Number format: X, G and B are fp16, scaled by a power of two, and not bf16: |X|, |G| <= ~1.3
 // and |B| <= ~3, so fp16's range is enough, and its 11 bits make each rounding 8 times smaller
 // than bf16's at the same tensor rate. With bf16 results the error is then the last rounding
-// to bf16 (the iteration adds ~6e-4 of the norm against that rounding's 1.7e-3). The scale keeps
+// to bf16 (the iteration's own 5e-4 to 1.3e-3 of the norm against that rounding's 1.7e-3). The
+// scale keeps
 // the small entries of a large matrix (~1 / sqrt(m n) at the start, ~1 / (m sqrt n) in
 // G) out of fp16's subnormals. Full precision (fp16 and fp32 results) keeps two planes,
 // x = hi + lo.
