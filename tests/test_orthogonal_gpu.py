@@ -334,6 +334,12 @@ def test_large(shape):
     assert torch.equal(got, orthogonalize(x))
 
 
+def test_large_in_half_precision_to_float32():
+    x = _input(4, (1, 2600, 2701))
+    exact, tol = _tolerance(x, x.dtype, True)
+    assert _far(orthogonalize(x, precision="half"), exact) <= tol
+
+
 @pytest.mark.parametrize("shape", [(1, 2600, 2700), (1, 2700, 2600)])
 def test_large_update(shape):
     param = _input(1, shape, torch.bfloat16, 0.02)
