@@ -350,11 +350,15 @@ template <int COLS, int BUFS, bool SPLIT>
 struct WarpEpilogue {
   static constexpr int BOXES = COLS / 64;
   static_assert(!SPLIT || (BOXES == 1 && BUFS == 2), "planes take a buffer each");
+  // Consecutive boxes use different buffers (buf(b), b = 0 .. BOXES - 1 over and over): one's stores may
+  // still read its buffer while the next is filled. With a single box per tile it is buffer 0 every
+  // time, however many there are.
+  static constexpr bool ALTERNATE = BUFS == 2 && BOXES == 2;
   uint8_t* bufs;        // BUFS boxes of this warp, 1024-byte aligned
   uint64_t* c_bar;      // [2] this warp's
   uint32_t c_phase;     // bit b: parity of the next wait on c_bar[b]
   int lane;
-  int newest = 0;       // stores of the box before, which uses the other buffer (if there are two)
+  int newest = 0;       // stores of the box before (ALTERNATE: from the other buffer)
 
   __device__ __forceinline__ uint8_t* buf(int b) const { return bufs + (b % BUFS) * kBoxBytes; }
 
@@ -468,7 +472,7 @@ struct WarpEpilogue {
     }
     const bool with_c = HAS_C && g.beta != 0.f;
     if (!with_c) {
-      if (lane == 0) boxes_read_but(BUFS == 2 ? newest : 0);
+      if (lane == 0) boxes_read_but(ALTERNATE ? newest : 0);
       __syncwarp();
     }
     newest = mirror ? 2 : 1;
