@@ -362,9 +362,13 @@ struct WarpEpilogue {
 
   __device__ __forceinline__ uint8_t* buf(int b) const { return bufs + (b % BUFS) * kBoxBytes; }
 
-  // C's boxes, ahead of the accumulator (needs a buffer per box).
+  // C's boxes, ahead of the accumulator (needs a buffer per box). The last tile's results may have
+  // passed through these buffers by ordinary stores with no copy behind them (write_direct): every
+  // lane orders its own before TMA writes there.
   __device__ __forceinline__ void load_c(const Out& g, int row_base, int col0) {
     if (g.beta == 0.f) return;
+    fence_proxy_async_smem();
+    __syncwarp();
     if (lane == 0) {
       boxes_read();
 #pragma unroll

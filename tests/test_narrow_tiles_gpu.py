@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from linalg_kernels_b200.grouped import grouped_matmul, grouped_outer
-from linalg_kernels_b200.orthogonal import orthogonalize
+from linalg_kernels_b200.orthogonal import muon_update_, orthogonalize
 from tests.test_grouped_gpu import _close, _problem, _randn, _reference, _reference_outer
 from tests.test_orthogonal_gpu import _far, _input, _tolerance
 
@@ -73,3 +73,20 @@ def test_orthogonalize(shape):
     assert _far(got, exact) <= tol
     for _ in range(4):
         assert torch.equal(orthogonalize(x), got)
+
+
+@pytest.mark.parametrize("shape", [(40, 300, 521), (30, 521, 300), (40, 300, 520)])
+def test_full_precision_to_unaligned_rows(shape):
+    """Several tiles per pair whose results go to the caller's rows through the buffers that the next
+    tile's old X is copied into."""
+    x = _input(sum(shape), shape)
+    exact, tol = _tolerance(x, x.dtype, False)
+    got = orthogonalize(x)
+    assert _far(got, exact) <= tol
+    for _ in range(4):
+        assert torch.equal(orthogonalize(x), got)
+    momentum, param = torch.zeros_like(x), torch.zeros_like(x)
+    muon_update_(param, x, momentum, lr=1.0, beta=0.0, nesterov=False, scale=1.0)
+    assert torch.equal(momentum, x)  # 0 * 0 + 1 * x
+    # 0 * 1 - 1 * 1 * o, every step exact but o
+    assert torch.equal(param, -got)
