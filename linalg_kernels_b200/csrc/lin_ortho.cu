@@ -186,12 +186,14 @@ struct Layout {
   size_t x_bytes, s_bytes, sums_bytes, total;
 };
 
-// Blocks per matrix of the first passes: about 4 chunks a thread, at most ~16 blocks per SM over the
-// batch.
+// Blocks per matrix of the first passes: about 4 chunks a thread, at most kPrepBlocks over the batch,
+// 16 for each of a B200's 148 SMs. Fixed, because the workspace holds a sum per block: its size is
+// asked for before any device is looked at, and callers keep it.
+constexpr int64_t kPrepBlocks = 148 * 16;
 int64_t prep_parts(int64_t batch, int64_t m, int64_t n) {
   const int64_t chunks = m * ((n + 7) / 8);
   int64_t parts = (chunks + kPrepThreads * 4 - 1) / (kPrepThreads * 4);
-  const int64_t cap = (int64_t(sm_count()) * 16 + batch - 1) / batch;
+  const int64_t cap = (kPrepBlocks + batch - 1) / batch;
   if (parts > cap) parts = cap;
   return parts < 1 ? 1 : parts;
 }
