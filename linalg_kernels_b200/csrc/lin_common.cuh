@@ -73,7 +73,9 @@ cudaError_t prepare_products();
 // Checks the device once (sm_100) and sets the kernels' shared-memory limits.
 int prepare_device(int dev);
 int prepare_current();
+// SMs of the device that this thread's call runs on (prepare_current sets it).
 int sm_count();
+void use_sm_count(int sms);
 
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

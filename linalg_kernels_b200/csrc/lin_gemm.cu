@@ -646,8 +646,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 // ------------------------------- host side --------------------------------------------
-int g_sms = 148;
-
 template <int BN, bool AMN, bool BMN, int MODE, int EPI, bool SPLIT>
 cudaError_t set_smem() {
   return cudaFuncSetAttribute(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
@@ -708,7 +706,7 @@ int launch(const Product& p, cudaStream_t q) {
   g.idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(AMN) << 15) |
             (uint32_t(BMN) << 16) | (uint32_t((BN < 256 ? BN : 256) >> 3) << 17) |
             (uint32_t(kTileM >> 4) << 24);
-  int64_t pairs = g_sms / 2;
+  int64_t pairs = sm_count() / 2;
   if (pairs > total) pairs = total;
   return chol::status_from(chol::launch_pdl(product_kernel<BN, AMN, BMN, MODE, EPI, SPLIT>,
                                             dim3(unsigned(2 * pairs)), dim3(kThreads),
@@ -722,7 +720,7 @@ bool narrow(const Product& p) {
   if (p.n <= 128) return true;
   const int64_t tm = p.mode == kRaggedM ? (p.total_rows + kTileM - 1) / kTileM + p.batch / 2
                                         : ((p.m + kTileM - 1) / kTileM) * p.batch;
-  return tm * ((p.n + 255) / 256) < g_sms / 2;
+  return tm * ((p.n + 255) / 256) < sm_count() / 2;
 }
 
 // BN = 512: a quarter less to load per product (48 KB per 1024 cycles of MMAs instead of 64 KB), for
@@ -735,7 +733,7 @@ bool narrow(const Product& p) {
 bool wide(const Product& p) {
   if (p.split || p.symmetric || p.beta != 0.f || p.n < 512) return false;
   if (p.mode != kBatch && p.batch > kWideGroups) return false;
-  const int64_t pairs = g_sms / 2, k = p.mode == kRaggedK ? p.total_rows / p.batch : p.k;
+  const int64_t pairs = sm_count() / 2, k = p.mode == kRaggedK ? p.total_rows / p.batch : p.k;
   const double blocks = double((k + kBlockK - 1) / kBlockK);
   auto rounds = [&](int64_t bn) {
     const int64_t tn = (p.n + bn - 1) / bn;
@@ -789,10 +787,6 @@ int launch_product(const Product& p, cudaStream_t q) {
 
 cudaError_t prepare_products() {
   cudaError_t e;
-  int dev = 0;
-  if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-  if ((e = cudaDeviceGetAttribute(&g_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
-    return e;
 #define LIN_SET(AMN, BMN, MODE, EPI, SPLIT)                                                   \
   if ((e = set_smem<128, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;             \
   if ((e = set_smem<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e; \
@@ -803,6 +797,10 @@ cudaError_t prepare_products() {
   return resolve_encode() ? cudaSuccess : cudaErrorNotSupported;
 }
 
-int sm_count() { return g_sms; }
+namespace {
+thread_local int t_sms = 148;
+}
+int sm_count() { return t_sms; }
+void use_sm_count(int sms) { t_sms = sms; }
 
 }  // namespace lin

@@ -374,12 +374,16 @@ int check_workspace(int64_t batch, int64_t m, int64_t n, bool split, const void*
 
 }  // namespace
 
+namespace {
+constexpr int kMaxDevices = 64;
+struct {
+  std::once_flag once;
+  int status, sms;
+} states[kMaxDevices];
+}  // namespace
+
 int prepare_device(int dev) {
-  static struct {
-    std::once_flag once;
-    int status;
-  } states[64];
-  if (dev < 0 || dev >= 64) return CHOL_ERR_DEVICE;
+  if (dev < 0 || dev >= kMaxDevices) return CHOL_ERR_DEVICE;
   std::call_once(states[dev].once, [dev]() {
     states[dev].status = chol::prepare_device_checked(dev);
     int prev = 0;
@@ -388,9 +392,10 @@ int prepare_device(int dev) {
       states[dev].status = CHOL_ERR_DEVICE;
       return;
     }
-    if (prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess ||
-        prepare_few() != cudaSuccess ||
-        prepare_mid_ortho() != cudaSuccess)
+    if (cudaDeviceGetAttribute(&states[dev].sms, cudaDevAttrMultiProcessorCount, dev) !=
+            cudaSuccess ||
+        prepare_products() != cudaSuccess || prepare_small_ortho() != cudaSuccess ||
+        prepare_few() != cudaSuccess || prepare_mid_ortho() != cudaSuccess)
       states[dev].status = CHOL_ERR_DEVICE;
     if (prev != dev) cudaSetDevice(prev);
   });
@@ -407,7 +412,9 @@ int prepare_current() {
     if (cudaSetDevice(dev) != cudaSuccess) return CHOL_ERR_DEVICE;
     bound = dev;
   }
-  return prepare_device(dev);
+  const int st = prepare_device(dev);
+  if (st == CHOL_OK) use_sm_count(states[dev].sms);
+  return st;
 }
 
 }  // namespace lin
