@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .orthogonal import _written
+from .orthogonal import _refuse_tangents, _written
 
 __all__ = ["grouped_matmul", "grouped_outer"]
 
@@ -210,14 +210,15 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     1024 groups.
 
     Differentiable in x and w (without ``out``): the gradient of a group without rows, and of rows
-    of no group, is zero; dy's rows of no group are not read. Runs on the current queue of x's
-    device.
+    of no group, is zero; dy's rows of no group are not read. Forward-mode tangents raise. Runs on the
+    current queue of x's device.
     """
     _check(x, "x", 2)
     _check(w, "w", 3, x)
     if w.shape[1] != x.shape[1]:
         raise ValueError(f"w must be (groups, {x.shape[1]}, n), got {tuple(w.shape)}")
     _check_offsets(offsets, x, w.shape[0])
+    _refuse_tangents("grouped_matmul", x, w, out)
     if out is not None:
         _check_out(out, (x.shape[0], w.shape[2]), x, "out", (x, w))
         _on_device(x, lambda: _matmul(_aligned(x), _aligned_weights(w), offsets, out))
@@ -243,6 +244,7 @@ def grouped_outer(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, *,
     groups = _check_offsets(offsets, a)
     if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad):
         raise RuntimeError("grouped_outer has no derivative: call it under torch.no_grad()")
+    _refuse_tangents("grouped_outer", a, b, out)
     if out is not None:
         _check_out(out, (groups, a.shape[1], b.shape[1]), a, "out", (a, b))
     result = _on_device(a, lambda: _outer(_aligned(a), _aligned(b), offsets, groups, out))

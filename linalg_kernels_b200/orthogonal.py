@@ -24,6 +24,7 @@ import math
 from collections.abc import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -47,6 +48,20 @@ def _check_tensor(t, name: str) -> None:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     if t.dim() < 2:
         raise ValueError(f"{name} must be (..., m, n), got shape {tuple(t.shape)}")
+
+
+def _dual_level() -> bool:
+    """Whether a forward_ad.dual_level is open (forward-mode derivatives ask for no requires_grad)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def _refuse_tangents(where: str, *tensors) -> None:
+    """A result without the tangent that its inputs carry would read as a zero derivative."""
+    if _dual_level() and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{where} has no forward-mode derivative: call it on a detached "
+                                   "tensor")
 
 
 def _batch_stride(t: torch.Tensor) -> int | None:
@@ -155,7 +170,7 @@ def _contiguous_call(x, steps, coefficients, eps, precision):
     """The common call (contiguous input, fresh output, one GPU) with arguments that an earlier call
     has checked: the host path paces calls of a few microseconds. None: not that case."""
     if type(x) is not torch.Tensor or not x.is_cuda or not x.is_contiguous() or \
-            x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()):
+            x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()) or _dual_level():
         return None
     kind = _TYPES.get(x.dtype)
     try:
@@ -194,8 +209,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     be ``x`` itself.
 
     A zero matrix gives zeros (with eps > 0); a matrix with a NaN or an infinity gives NaN and leaves the
-    others of the batch alone. It has no derivative: call it under ``torch.no_grad()`` or on a
-    detached tensor.
+    others of the batch alone. It has no derivative, in either mode: call it under ``torch.no_grad()``
+    or on a detached tensor (forward-mode tangents pass ``no_grad``; they raise).
     """
     if out is None and _one_device():
         out = _contiguous_call(x, steps, coefficients, eps, precision)
@@ -206,6 +221,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     _remember(steps, coefficients, eps, precision, coef)
     if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
         raise RuntimeError("orthogonalize has no derivative: call it under torch.no_grad()")
+    _refuse_tangents("orthogonalize", x, out)
     given = out is not None
     if not given:
         out = (torch.empty_like(x.transpose(-2, -1), memory_format=torch.contiguous_format)
@@ -300,6 +316,7 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
             raise ValueError("param, grad and momentum must have one shape and device")
         if name != "grad" and torch.is_grad_enabled() and t.requires_grad:
             raise RuntimeError(f"{name} requires grad: call muon_update_ under torch.no_grad()")
+    _refuse_tangents("muon_update_", param, grad, momentum)
     coef = _check_iteration(steps, coefficients, eps, precision)
     for v, name in ((lr, "lr"), (beta, "beta"), (weight_decay, "weight_decay")):
         if not math.isfinite(v):
