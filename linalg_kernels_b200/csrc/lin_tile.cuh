@@ -501,13 +501,18 @@ struct WarpEpilogue {
     return true;
   }
 
-  // SPLIT: sum += beta / alpha * C, of the boxes that load_c has asked for.
+  // SPLIT: sum = alpha * sum + beta * C, of the boxes that load_c has asked for (alpha may be zero).
   __device__ __forceinline__ bool add_c(const Out& g, float (&sum)[2][32], int* status) {
-    if (g.beta == 0.f) return true;
+    if (g.beta == 0.f) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[h][j] *= g.alpha;
+      return true;
+    }
     bool ok = wait_c(g, 0, status);
     ok = wait_c(g, 1, status) && ok;
     if (!ok) return false;
-    const float f = g.beta / g.alpha;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -519,14 +524,14 @@ struct WarpEpilogue {
           const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&as[e]));
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&bs[e]));
           float* p = sum[h] + c * 8 + 2 * e;
-          p[0] = fmaf(f, x.x + y.x, p[0]);
-          p[1] = fmaf(f, x.y + y.y, p[1]);
+          p[0] = fmaf(g.beta, x.x + y.x, g.alpha * p[0]);
+          p[1] = fmaf(g.beta, x.y + y.y, g.alpha * p[1]);
         }
       }
     return true;
   }
 
-  // SPLIT: alpha * sum as two planes, 64 columns from gc0. Nothing but the sums stays in registers
+  // SPLIT: add_c's result as two planes, 64 columns from gc0. Nothing but the sums stays in registers
   // (with packed copies they went to local memory, 2200 cycles for each drain).
   __device__ __forceinline__ void planes(const Out& g, int row_base, int gc0, bool mirror,
                                          const float (&sum)[2][32]) {
@@ -539,8 +544,8 @@ struct WarpEpilogue {
       uint32_t h[4], l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = g.alpha * sum[c >> 2][(c & 3) * 8 + 2 * e];
-        const float y = g.alpha * sum[c >> 2][(c & 3) * 8 + 2 * e + 1];
+        const float x = sum[c >> 2][(c & 3) * 8 + 2 * e];
+        const float y = sum[c >> 2][(c & 3) * 8 + 2 * e + 1];
         h[e] = pack<__half>(x, y);
         float a, b;
         unpack<__half>(h[e], a, b);
@@ -576,14 +581,16 @@ struct WarpEpilogue {
     }
   }
 
-  // 32 columns from gc0 straight to the caller's matrix.
+  // 32 columns from gc0 straight to the caller's matrix (SPLIT: as add_c left them).
   __device__ __forceinline__ void direct(const Out& g, int row_base, int gc0, float (&v)[32]) {
     if (gc0 >= g.n || row_base >= g.rows) return;
     if (lane == 0) boxes_read();
     __syncwarp();
     float* stage = reinterpret_cast<float*>(bufs);
+    if constexpr (!SPLIT) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= g.alpha;
+      for (int j = 0; j < 32; ++j) v[j] *= g.alpha;
+    }
     if (g.type == LINALG_BF16)
       write_direct<__nv_bfloat16>(g, v, lane, row_base, gc0, stage);
     else if (g.type == LINALG_FP16)
