@@ -50,7 +50,7 @@ extern "C" {
 #define CHOL_ERR_WAIT_TIMEOUT 4  /* a bounded device-side wait ran out (status word set) */
 #define CHOL_ERR_WORKSPACE 5     /* caller workspace missing or smaller than required */
 #define CHOL_ERR_DEVICE 6        /* no usable sm_100 device / CUDA runtime error */
-#define CHOL_ERR_UNSUPPORTED 7   /* size outside what this build supports */
+#define CHOL_ERR_UNSUPPORTED 7   /* size or value outside what this build supports */
 #define CHOL_ERR_SCRATCH_LIMIT 8 /* needs more scratch than chol_potrf_batched_noalloc_f32 has */
 
 /* Library version as MAJOR*10000 + MINOR*100 + PATCH. */

@@ -57,6 +57,11 @@ CHOL_API size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t
  *   X = x / (||x||_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T
  * (from the right with A = X^T X when m > n), and out = X. coefficients: 3 * steps host floats
  * (a, b, c of each step). x and out may be the same array; partial overlap is not allowed.
+ * The iterates are held in fp16, which gives the coefficients a range: with s_0 = 1 and
+ * s_k+1 = 65/64 max |t (a + b t^2 + c t^4)| over t in [0, s_k], every step must keep s_k^2 <= 63.9
+ * and |a + b t^2 + c t^4| <= 65504 (HALF), s_k^2 <= 15.9 and |b t^2 + c t^4| <= 31.9 (FULL), and
+ * the product |a_0 ... a_k| must not fall below 1/4 (but for a step of three zeros). Coefficients
+ * that may leave it for some matrix: CHOL_ERR_UNSUPPORTED.
  * A matrix with a NaN or an infinity yields NaN; the other matrices of the batch are not
  * affected. A zero matrix yields zeros (with eps > 0).
  */

@@ -711,7 +711,7 @@ const char* chol_strerror(int status) {
     case CHOL_ERR_WAIT_TIMEOUT: return "bounded device-side wait timed out";
     case CHOL_ERR_WORKSPACE: return "workspace missing or too small";
     case CHOL_ERR_DEVICE: return "no usable sm_100 CUDA device";
-    case CHOL_ERR_UNSUPPORTED: return "size not supported by this build";
+    case CHOL_ERR_UNSUPPORTED: return "size or value not supported by this build";
     case CHOL_ERR_SCRATCH_LIMIT:
       return "problem needs more scratch than the fixed buffer of the no-allocation entry point";
     default: return "unknown status";

@@ -86,9 +86,9 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 }
 
 // Eight values to fp16 (and the remainder plane): shared-memory chunks of 16 bytes. Saturating: an
-// infinity in one matrix would reach the others of its tile as 0 * inf in B X. (Only
-// coefficients with which the iteration diverges get there: 65504 stands for
-// singular values of G of 16 in full precision and 64 in half.)
+// infinity in one matrix would reach the others of its tile as 0 * inf in B X. (Coefficients that
+// could take a matrix there are refused, lin_ortho.cu: 65504 stands for singular values of G of 16
+// in full precision and 64 in half.)
 __device__ __forceinline__ uint32_t half2_sat(float a, float b) {
   uint32_t r;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));

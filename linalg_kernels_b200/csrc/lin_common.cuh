@@ -67,6 +67,10 @@ struct Product {
 
 constexpr int kMaxGroups = 1024;
 
+// Newton-Schulz in fp16 (one plane, or two with split): the scales of X and of B; G has X's squared.
+__host__ __device__ constexpr float x_scale(bool split) { return split ? 64.f : 32.f; }
+__host__ __device__ constexpr float b_scale(bool split) { return split ? 2048.f : 1.f; }
+
 int launch_product(const Product& p, cudaStream_t q);
 cudaError_t prepare_products();
 

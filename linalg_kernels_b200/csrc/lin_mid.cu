@@ -466,7 +466,7 @@ int launch_mid_ortho(const linalg_matrix* x, const linalg_matrix* momentum,
   g.out_path = output_path(g.out, n);
   g.beta = float(beta), g.gain = float(1.0 - beta);
   g.decay = decay, g.rate = rate;
-  g.scale = 32.f, g.eps = eps;
+  g.scale = x_scale(false), g.eps = eps;
   g.inv_x = 1.f / g.scale, g.inv_gram = g.inv_x * g.inv_x;
   for (int k = 0; k < 3 * steps; ++k) g.coef[k] = coefficients[k];
   const dim3 grid(unsigned(2 * batch)), block(T);

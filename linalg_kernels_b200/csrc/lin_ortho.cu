@@ -261,8 +261,8 @@ int iterate(const linalg_matrix* x, const linalg_matrix* momentum, const linalg_
   // largest; X's small ones (1 / sqrt(m n) at the start) clear of its subnormals. B, with a
   // on its diagonal, needs no scale: what its subnormals lose, 3e-8 per entry, is small against
   // the rounding of its diagonal; the planes of full precision keep 22 bits with 2048.
-  const float scale = split ? 64.f : 32.f, gram_scale = scale * scale;
-  const float poly_scale = split ? 2048.f : 1.f;
+  const float scale = x_scale(split), gram_scale = scale * scale;
+  const float poly_scale = b_scale(split);
 
   Prep p{};
   p.x = device_matrix(x);
@@ -355,6 +355,46 @@ int check_iteration(int64_t batch, int64_t m, int64_t n, int steps, const float*
   return CHOL_OK;
 }
 
+// Whether X, G and B stay within fp16's 65504 for every matrix under these coefficients. X's singular
+// values start at 1 at most (the Frobenius norm's bound); with s the largest at a step and u = s^2, no
+// entry of G passes u and none of B the largest |q| on [0, u], q(u) = b u + c u^2 (with a added where a
+// stands on B's diagonal); the next s is the largest |t (a + b t^2 + c t^4)| for t up to s. Beyond the
+// range the on-chip kernels would saturate and the products give infinities. Each s is taken
+// 1/64 larger, for the roundings of X. (G's limit is the narrower one: X's own is implied.)
+// And whether they stay clear of its smallest numbers: small singular values are multiplied by a in
+// each step, and the product of the steps' a down to any step must not fall below 1/4. (With a = 0, B
+// has no diagonal and X shrinks to its third power: (0, 2, -1) twice in half precision was 1e-2 off
+// for 100 x 1500.)
+bool in_range(int steps, const float* coefficients, bool split) {
+  const double top = 65504.0, scale = x_scale(split);
+  const double top_u = top / (scale * scale), top_b = top / b_scale(split);
+  double s = 1.0, least = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+    const double u = s * s;
+    if (!(u <= top_u)) return false;
+    if (a == 0.0 && b == 0.0 && c == 0.0) return true;  // zeros from here on, exactly
+    least *= fabs(a);
+    if (!(least >= 0.25)) return false;
+    auto q = [&](double x) { return fabs((split ? 0.0 : a) + (b + c * x) * x); };
+    double most = fmax(q(0.0), q(u));
+    if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < u) most = fmax(most, q(-b / (2.0 * c)));
+    if (!(most <= top_b)) return false;
+    auto p = [&](double x) { return fabs(sqrt(x) * (a + (b + c * x) * x)); };
+    s = p(u);
+    // extrema: a + 3 b x + 5 c x^2 = 0, the roots without cancellation
+    const double d = 9.0 * b * b - 20.0 * a * c;
+    if (d >= 0.0) {
+      const double h = -0.5 * (3.0 * b + copysign(sqrt(d), b));
+      const double roots[2] = {c != 0.0 ? h / (5.0 * c) : -1.0, h != 0.0 ? a / h : -1.0};
+      for (const double x : roots)
+        if (x > 0.0 && x < u) s = fmax(s, p(x));
+    }
+    s *= 1.0 + 1.0 / 64;
+  }
+  return true;
+}
+
 bool too_large(int64_t batch, int64_t m, int64_t n) {
   const int64_t lim = 1 << 24;  // planes * batch and tile counts stay within 32 bits
   return batch > lim || m > lim || n > lim;
@@ -443,6 +483,7 @@ int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64
                     (batch == 1 || x->stride == out->stride);
   if (!same && overlap(x, out, batch, m, n)) return CHOL_ERR_INVALID_ARG;
   const bool split = wants_split(precision, out->type);
+  if (!in_range(steps, coefficients, split)) return CHOL_ERR_UNSUPPORTED;
   if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
   if ((st = prepare_current()) != CHOL_OK) return st;
   return iterate(x, nullptr, out, batch, m, n, 0.f, 0, 1.f, 0.f, steps, coefficients, eps, split,
@@ -467,6 +508,7 @@ int linalg_muon_update(const linalg_matrix* param, const linalg_matrix* grad,
       overlap(grad, momentum, batch, m, n))
     return CHOL_ERR_INVALID_ARG;
   const bool split = wants_split(precision, param->type);
+  if (!in_range(steps, coefficients, split)) return CHOL_ERR_UNSUPPORTED;
   if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
   if ((st = prepare_current()) != CHOL_OK) return st;
   return iterate(grad, momentum, param, batch, m, n, beta, nesterov, decay, rate, steps,

@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
     // and the diagonal of a I + b G + c G G scales the rows of X in FP32 at the end.
     // Full: a X is added in FP32 at the end, not summed by the tensor core, whose rounding towards
     // zero would weigh on the largest term; and B keeps 22 bits with a scale of 2048.
-    constexpr float kPoly = SPLIT ? 2048.f : 1.f;
+    constexpr float kPoly = b_scale(SPLIT);
     const float fb = cb * g.inv_gram * kPoly, fc = cc * g.inv_gram * g.inv_gram * kPoly;
 #pragma unroll
     for (int n = 0; n < GROUPS; ++n) {
@@ -736,7 +736,7 @@ int launch_small(const linalg_matrix* x, const linalg_matrix* momentum, const li
   g.out_path = output_path(g.out, n);
   g.beta = float(beta), g.gain = float(1.0 - beta), g.nesterov = nesterov;
   g.decay = decay, g.rate = rate;
-  g.scale = split ? 64.f : 32.f, g.eps = eps;
+  g.scale = x_scale(split), g.eps = eps;
   g.inv_x = 1.f / g.scale, g.inv_gram = g.inv_x * g.inv_x;
   for (int k = 0; k < 3 * steps; ++k) g.coef[k] = coefficients[k];
   const size_t smem = smem_bytes(split, g.ranks, g.cta_cols);

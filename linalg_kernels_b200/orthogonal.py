@@ -208,6 +208,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     bfloat16 and ``"full"`` otherwise. out: written and returned instead of a new tensor; may
     be ``x`` itself.
 
+    The iterates are fp16 numbers: coefficients with which some matrix could leave their range (singular
+    values above ~8 in ``"half"``, ~4 in ``"full"``, where also ``|b s^2 + c s^4|`` stays below 32; a
+    product of the steps' ``|a|`` below 1/4, ``a = 0`` among them) raise ``CholeskyError``;
+    include/linalg_b200.h has the bounds.
+
     A zero matrix gives zeros (with eps > 0); a matrix with a NaN or an infinity gives NaN and leaves the
     others of the batch alone. It has no derivative, in either mode: call it under ``torch.no_grad()``
     or on a detached tensor (forward-mode tangents pass ``no_grad``; they raise).
