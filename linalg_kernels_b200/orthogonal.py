@@ -8,8 +8,8 @@ step around it.
 
 ``muon_update_`` is one whole step of that optimiser: momentum, direction, weights, in place.
 It takes a batch, so the matrices of one shape (the projections of every layer, or the experts'
-matrices whose gradient ``grouped.grouped_outer`` returns as one ``(experts, k, n)`` tensor) go
-through one call.
+matrices whose gradient ``grouped.grouped_outer`` returns as one ``(experts, k, n)`` tensor, passed as
+its ``.mT`` view) go through one call.
 
 Both run the hand-written sm_100a products of ``libchol_b200.so`` (include/linalg_b200.h). CPU
 tensors raise ``TypeError`` as in ``cholesky.custom_kernel``: there is no CPU path. The reference
@@ -310,7 +310,10 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
 
     param, grad, momentum: ``(..., m, n)`` CUDA tensors of one shape, each bfloat16, float16 or
     float32, not overlapping. param and momentum need contiguous rows (or columns, both then)
-    and one stride between matrices. scale: ``sqrt(max(1, m / n))`` when None. precision: as in
+    and one stride between matrices. scale: ``sqrt(max(1, m / n))`` when None, the usual
+    ``sqrt(max(1, out / in))`` for weights of ``(out, in)``. Weights of ``(in, out)``, as
+    ``grouped.grouped_matmul`` takes them, go in as views, ``w.mT`` with ``w.grad.mT`` and
+    ``momentum.mT`` (worked on as they lie), or with their scale. precision: as in
     ``orthogonalize``, by param's type when None; a float32 param whose update may carry an error
     of ~1e-3 of itself takes ``"half"``, at a third of the work. u is taken from the momentum as
     stored. Call it under ``torch.no_grad()``.
