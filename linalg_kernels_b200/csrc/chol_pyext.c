@@ -18,6 +18,7 @@
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "../../include/linalg_b200.h"
@@ -63,6 +64,12 @@ static linalg_matrix matrix(const int64_t* v) {
   const linalg_matrix x = {(void*)(uintptr_t)v[0], v[1], v[2], (int)v[3]};
   return x;
 }
+/* A positive eps stays positive: below the smallest FP32 number it would turn 0, and the zero matrix's
+   0 / (0 + eps) into NaN. */
+static float positive(double eps) {
+  const float e = (float)eps;
+  return e == 0.0f && eps > 0.0 ? FLT_TRUE_MIN : e;
+}
 /* The buffer holds what the call reads. */
 static int enough(const Py_buffer* coef, int64_t steps) {
   return steps >= 0 && steps <= LINALG_MAX_STEPS &&
@@ -79,7 +86,7 @@ static PyObject* orthogonalize(PyObject* self, PyObject* const* args, Py_ssize_t
   int st = CHOL_ERR_INVALID_ARG;
   if (enough(&coef, v[11]))
     st = linalg_orthogonalize(&x, &out, v[8], v[9], v[10], (int)v[11], (const float*)coef.buf,
-                              (float)f[0], (int)v[12], (void*)(uintptr_t)v[13], (size_t)v[14],
+                              positive(f[0]), (int)v[12], (void*)(uintptr_t)v[13], (size_t)v[14],
                               (void*)(uintptr_t)v[15]);
   PyBuffer_Release(&coef);
   return PyLong_FromLong(st);
@@ -96,7 +103,7 @@ static PyObject* muon_update(PyObject* self, PyObject* const* args, Py_ssize_t n
   if (enough(&coef, v[16]))
     st = linalg_muon_update(&param, &grad, &momentum, v[12], v[13], v[14], f[0], (int)v[15],
                             (float)f[1], (float)f[2], (int)v[16], (const float*)coef.buf,
-                            (float)f[3], (int)v[17], (void*)(uintptr_t)v[18], (size_t)v[19],
+                            positive(f[3]), (int)v[17], (void*)(uintptr_t)v[18], (size_t)v[19],
                             (void*)(uintptr_t)v[20]);
   PyBuffer_Release(&coef);
   return PyLong_FromLong(st);

@@ -119,8 +119,8 @@ def _coefficients(coefficients: tuple, steps: int) -> array.array:
 def _check_iteration(steps, coefficients, eps, precision):
     if not isinstance(steps, int) or not 1 <= steps <= _lib.LINALG_MAX_STEPS:
         raise ValueError(f"steps must be a whole number from 1 to {_lib.LINALG_MAX_STEPS}")
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError("eps must be finite and not negative")
+    if not 0 <= eps <= torch.finfo(torch.float32).max:
+        raise ValueError("eps must be a 32-bit number and not negative")
     if precision not in _PRECISIONS:
         raise ValueError("precision must be None, 'half' or 'full'")
     if type(coefficients) is not tuple or any(type(c) is list for c in coefficients):
