@@ -173,8 +173,8 @@ def _contiguous_call(x, steps, coefficients, eps, precision):
             x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()) or _dual_level():
         return None
     kind = _TYPES.get(x.dtype)
-    try:
-        plan = _plain.get((steps, coefficients, eps, precision))
+    try:  # (5.0 would find the plan of 5, and is refused)
+        plan = _plain.get((steps, coefficients, eps, precision)) if type(steps) is int else None
     except TypeError:  # coefficients as lists
         return None
     if kind is None or plan is None or _call is None:

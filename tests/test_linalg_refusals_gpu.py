@@ -46,3 +46,158 @@ def test_forward_mode_tangents():
     x.requires_grad_()
     grouped_matmul(x, w, offsets).sum().backward()
     assert x.grad is not None
+
+
+def test_iteration_arguments_every_time():
+    """The second call takes the short host path: it refuses the same."""
+    x = _ones(3, 8, 8)
+    for _ in range(2):
+        orthogonalize(x, 5)
+        orthogonalize(x, 1)
+        for steps in (5.0, 0, 33, "5", None, 1.0):
+            with pytest.raises(ValueError, match="steps"):
+                orthogonalize(x, steps)
+        for coefs in ((1.0, 2.0), (), None, 5, ((1.0, 2.0, 3.0),) * 3, (float("inf"), 0.0, 0.0)):
+            with pytest.raises(ValueError, match="coefficients"):
+                orthogonalize(x, 5, coefficients=coefs)
+        with pytest.raises(ValueError, match="precision"):
+            orthogonalize(x, precision="double")
+
+
+def test_orthogonalize_tensors():
+    x = _ones(3, 8, 12)
+    for t in (x.to(torch.float64), x.int(), x.cfloat()):
+        with pytest.raises(TypeError):
+            orthogonalize(t)
+    with pytest.raises(ValueError):
+        orthogonalize(x[0, 0])
+    with pytest.raises(TypeError):
+        orthogonalize(x, out=torch.empty(3, 8, 12, dtype=torch.bfloat16))
+    for out in (_ones(3, 8, 13), _ones(3, 12, 8), _ones(2, 8, 12), _ones(3, 8, 12, dtype=torch.float32)):
+        with pytest.raises(ValueError, match="shape, type"):
+            orthogonalize(x, out=out)
+    for out in (_ones(1, 8, 12).expand(3, 8, 12), _ones(3, 8, 24)[..., ::2], _ones(3, 1, 12).expand(3, 8, 12),
+                _ones(3, 8, 1).expand(3, 8, 12)):
+        with pytest.raises(ValueError, match="contiguous"):
+            orthogonalize(x, out=out)
+    for grad in (x.clone().requires_grad_(), torch.nn.Parameter(x.clone())):
+        with pytest.raises(RuntimeError, match="derivative"):
+            orthogonalize(grad)
+        with pytest.raises(RuntimeError, match="derivative"):
+            orthogonalize(x, out=grad)
+        with torch.no_grad():
+            assert torch.equal(orthogonalize(grad), orthogonalize(x))
+
+
+def test_muon_tensors():
+    p, g, m = _ones(2, 8, 12), _ones(2, 8, 12), _ones(2, 8, 12, dtype=torch.float32)
+    kept = [t.clone() for t in (p, g, m)]
+
+    def refused(error, match, *tensors, **kw):
+        with pytest.raises(error, match=match):
+            muon_update_(*tensors, **{"lr": 0.1, **kw})
+
+    refused(TypeError, "grad", p, g.double(), m)
+    refused(TypeError, "momentum", p, g, m.cpu())
+    refused(ValueError, "one shape", p, g[:1], m)
+    refused(ValueError, "one shape", p, g, m.mT.contiguous())
+    refused(ValueError, "columns", p, g, m.mT.contiguous().mT)  # rows and columns
+    refused(ValueError, "columns", p.mT.contiguous().mT, g, m)
+    refused(ValueError, "columns", p[:1].expand(2, 8, 12), g, m)
+    refused(ValueError, "overlap", p, p, m)
+    refused(ValueError, "overlap", p, g, p)
+    refused(ValueError, "overlap", p, g, g)
+    refused(ValueError, "overlap", m, p, m)
+    wide = _ones(3, 8, 12)
+    refused(ValueError, "overlap", wide[:2], wide[1:], m)
+    refused(RuntimeError, "param", p.clone().requires_grad_(), g, m)
+    refused(RuntimeError, "momentum", p, g, m.clone().requires_grad_())
+    for name in ("lr", "beta", "weight_decay", "scale"):
+        for bad in (float("nan"), float("inf")):
+            refused(ValueError, name, p, g, m, **{name: bad})
+    refused(ValueError, "steps", p, g, m, steps=0)
+    refused(ValueError, "eps", p, g, m, eps=-1.0)
+    refused(ValueError, "precision", p, g, m, precision="best")
+    for t, k in zip((p, g, m), kept):
+        assert torch.equal(t, k)
+    # a gradient that requires grad is read alone; parameters under no_grad are written
+    param = torch.nn.Parameter(p.clone())
+    with torch.no_grad():
+        muon_update_(param, g, m.clone(), lr=0.1)
+    muon_update_(p, g.clone().requires_grad_(), m, lr=0.1)
+    assert torch.equal(param.detach(), p)
+
+
+def test_grouped_tensors():
+    x, w, dy = _ones(6, 8), _ones(2, 8, 16), _ones(6, 16)
+    offsets = torch.tensor([0, 2, 6], device=DEV)
+
+    def refused(error, match, call, *args, **kw):
+        with pytest.raises(error, match=match):
+            call(*args, **kw)
+
+    for call, a, b in ((grouped_matmul, x, w), (grouped_outer, x, dy)):
+        refused(TypeError, "float16", call, a.float(), b.float(), offsets)
+        refused(ValueError, "type", call, a, b.half(), offsets)
+        refused(TypeError, "CUDA", call, a, b.cpu(), offsets)
+        refused(ValueError, "dimensions", call, a[None], b, offsets)
+        refused(ValueError, "dimensions", call, a, b[None], offsets)
+        refused(TypeError, "offsets", call, a, b, [0, 2, 6])
+        refused(TypeError, "offsets", call, a, b, offsets.float())
+        refused(TypeError, "offsets", call, a, b, offsets.short())
+        refused(ValueError, "device", call, a, b, offsets.cpu())
+        refused(ValueError, "contiguous", call, a, b, offsets[None])
+        refused(ValueError, "contiguous", call, a, b, offsets.repeat_interleave(2)[::2])
+        refused(ValueError, "contiguous", call, a, b, offsets[:0])
+    refused(ValueError, "3 entries", grouped_matmul, x, w, offsets[:2])
+    refused(ValueError, "w must be", grouped_matmul, x, w.mT, offsets)
+    refused(ValueError, "same rows", grouped_outer, x, dy[:5], offsets)
+    many = torch.zeros(1026, device=DEV, dtype=torch.int32)
+    refused(ValueError, "1024", grouped_matmul, x, w[:1].expand(1025, 8, 16), many)
+    refused(ValueError, "1024", grouped_outer, x, dy, many)
+    for out in (_ones(6, 17), _ones(7, 16), _ones(16, 6)):
+        refused(ValueError, "shape", grouped_matmul, x, w, offsets, out=out)
+    refused(ValueError, "type", grouped_matmul, x, w, offsets, out=_ones(6, 16, dtype=torch.float16))
+    refused(ValueError, "dimensions", grouped_matmul, x, w, offsets, out=_ones(1, 6, 16))
+    refused(ValueError, "rows", grouped_matmul, x, w, offsets, out=_ones(16, 6).T)
+    refused(ValueError, "rows", grouped_matmul, x, w, offsets, out=_ones(1, 16).expand(6, 16))
+    refused(ValueError, "rows", grouped_outer, x, dy, offsets, out=_ones(1, 8, 16).expand(2, 8, 16))
+    square = _ones(2, 6, 6)
+    refused(ValueError, "overlap", grouped_matmul, square[0], square, offsets, out=square[0])
+    refused(ValueError, "overlap", grouped_matmul, square[0].clone(), square, offsets, out=square[1])
+    big = _ones(40, 8)
+    refused(ValueError, "overlap", grouped_outer, big[:6], big[6:12], offsets,
+            out=big.view(-1)[64:192].view(2, 8, 8))
+    refused(ValueError, "k > 0", grouped_matmul, x[:, :0], w[:, :0], offsets, out=_ones(6, 16))
+    for a, b in ((x.clone().requires_grad_(), w), (x, w.clone().requires_grad_())):
+        refused(RuntimeError, "no_grad", grouped_matmul, a, b, offsets, out=_ones(6, 16))
+        with torch.no_grad():
+            grouped_matmul(a, b, offsets, out=_ones(6, 16))
+    refused(RuntimeError, "no_grad", grouped_matmul, x, w, offsets, out=_ones(6, 16).requires_grad_())
+    refused(RuntimeError, "no_grad", grouped_outer, x.clone().requires_grad_(), dy, offsets)
+    refused(RuntimeError, "no_grad", grouped_outer, x, dy, offsets, out=_ones(2, 8, 16).requires_grad_())
+    # operands changed between the passes
+    xx, ww = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = grouped_matmul(xx, ww, offsets)
+    with torch.no_grad():
+        ww.mul_(2)
+    refused(RuntimeError, "modified", y.sum().backward)
+    y = grouped_matmul(xx, ww, offsets)
+    with torch.no_grad():
+        muon_update_(ww, _ones(2, 8, 16), _ones(2, 8, 16), lr=0.1)
+    refused(RuntimeError, "modified", y.sum().backward)
+
+
+@pytest.mark.parametrize("precision", ["half", "full"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_muon_precision_argument(precision, dtype):
+    from tests.test_orthogonal_gpu import _input, _tolerance
+
+    for shape in ((2, 96, 200), (2, 300, 260)):
+        grad, momentum = _input(1, shape), torch.zeros(shape, device=DEV)
+        param = torch.zeros(shape, device=DEV, dtype=dtype)
+        muon_update_(param, grad, momentum, lr=1.0, beta=0.0, nesterov=False, scale=1.0,
+                     precision=precision)
+        exact, tol = _tolerance(grad, dtype, precision == "half")
+        off = (param.double() + exact).square().sum((-2, -1)).sqrt()
+        assert (off <= (tol + 3 * 2.0 ** -24) * exact.square().sum((-2, -1)).sqrt()).all()
