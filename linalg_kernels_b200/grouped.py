@@ -61,13 +61,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
             len(shape) < 3 or (not stride[0] & 7 and stride[0] >= cols + (rows - 1) * ld)):
         return t
     padded = t.new_empty(*shape[:-1], (cols + 7) // 8 * 8)[..., :cols]
-    return padded.copy_(t)
+    return padded.copy_(t.detach())
 
 
 def _aligned_weights(w: torch.Tensor) -> torch.Tensor:
     """The same for (groups, k, n) weights, in the order in which they lie in memory."""
     if _stored_transposed(w):
-        return _aligned(w.transpose(1, 2)).transpose(1, 2)
+        lies = w.transpose(1, 2)
+        rows = _aligned(lies)
+        return w if rows is lies else rows.transpose(1, 2)
     return _aligned(w)
 
 
@@ -147,27 +149,66 @@ def _on_device(t: torch.Tensor, call):
 
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets):
+    def forward(ctx, x, w, offsets, aligned):
         # the aligned operands serve the backward pass too: a copy is made once
-        x, w = _aligned(x), _aligned_weights(w)
-        ctx.save_for_backward(x, w, offsets)
-        return _matmul(x, w, offsets)
+        ax, aw, ctx.links = aligned
+        ctx.save_for_backward(ax, aw, offsets)
+        return _matmul(ax, aw, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):  # (autograd has made the device current)
+        _refuse_tangents("grouped_matmul's backward pass", dy)
         x, w, offsets = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = None
-        dy = _aligned(dy)
-        if need[0]:
-            dx = _matmul(dy, w.transpose(1, 2), offsets)
-        if need[1]:
-            if _stored_transposed(w):  # stored (groups, n, k): so is its gradient
-                dw = _outer(dy, x, offsets, w.shape[0]).transpose(1, 2)
-            else:
-                dw = _outer(x, dy, offsets, w.shape[0])
-        return dx, dw, None
+        with torch.no_grad():
+            rows = _aligned(dy)
+            if need[0]:
+                dx = _matmul(rows, w.transpose(1, 2), offsets)
+            if need[1]:
+                if _stored_transposed(w):  # stored (groups, n, k): so is its gradient
+                    dw = _outer(rows, x, offsets, w.shape[0]).transpose(1, 2)
+                else:
+                    dw = _outer(x, rows, offsets, w.shape[0])
+        if torch.is_grad_enabled():  # create_graph: dx hangs on w and dy, dw on x and dy
+            if dx is not None:
+                dx = _Once.apply(dx, dy, _origin(ctx, 1, w))
+            if dw is not None:
+                dw = _Once.apply(dw, dy, _origin(ctx, 0, x))
+        return dx, dw, None, None
+
+
+class _Once(torch.autograd.Function):
+    """A gradient and what it hangs on. It has no derivative: asking for one raises, where a detached
+    tensor would read as a constant. (torch's once_differentiable marks gradients only where dy
+    requires grad, and hangs them on nothing.)"""
+
+    @staticmethod
+    def forward(ctx, t, *on):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("grouped_matmul has no second derivative")
+
+
+def _differentiable(x, w, offsets):
+    ax, aw = _aligned(x), _aligned_weights(w)
+    return _GroupedMatmul.apply(x, w, offsets, (ax, aw, (_link(x, ax), _link(w, aw))))
+
+
+def _link(t: torch.Tensor, aligned: torch.Tensor) -> torch.Tensor | None:
+    """An empty tensor with t's place in the graph, where the backward pass keeps a copy of t instead."""
+    return t[:0].clone() if aligned is not t and t.grad_fn is not None else None
+
+
+def _origin(ctx, i: int, saved: torch.Tensor):
+    """A tensor with operand i's place in the graph, None for one that requires no grad."""
+    node = ctx.next_functions[i][0]
+    if node is None or saved.requires_grad:
+        return saved if node is not None else None
+    leaf = getattr(node, "variable", None)
+    return leaf if leaf is not None else ctx.links[i]
 
 
 def _check_out(out, shape, like, name, others):
@@ -210,8 +251,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     1024 groups.
 
     Differentiable in x and w (without ``out``): the gradient of a group without rows, and of rows
-    of no group, is zero; dy's rows of no group are not read. Forward-mode tangents raise. Runs on the
-    current queue of x's device.
+    of no group, is zero; dy's rows of no group are not read. Forward-mode tangents and second
+    derivatives raise. Runs on the current queue of x's device.
     """
     _check(x, "x", 2)
     _check(w, "w", 3, x)
@@ -225,7 +266,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
         _written(out)
         return out
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        return _on_device(x, lambda: _GroupedMatmul.apply(x, w, offsets))
+        return _on_device(x, lambda: _differentiable(x, w, offsets))
     return _on_device(x, lambda: _matmul(_aligned(x), _aligned_weights(w), offsets))
 
 
