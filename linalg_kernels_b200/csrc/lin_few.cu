@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const bool zeros = p.group >= g.groups;
       const uint32_t buf = round & 1u;
       if (!zeros) {
-        const bool ok = mbar_wait(&tfull[buf], (round >> 1) & 1u, status);
+        const bool ok = mbar_wait(&tfull[buf], (round >> 1) & 1u, status, limit_of(blocks_k));
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
       }

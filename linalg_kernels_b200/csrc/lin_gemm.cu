@@ -38,8 +38,8 @@
 // against 64 bits, 3 x 1001 x 601: 4.5e-6 with a drain per 256 of K, 2.3e-6 per 128, 1.4e-6 per 64,
 // where FP32 products have 3.0e-6.)
 //
-// Every wait is bounded (2 s of %globaltimer); one that runs out records
-// CHOL_ERR_WAIT_TIMEOUT in the library's status word and ends the launch.
+// Every wait is bounded (2 s of %globaltimer, and 2 us more for each K block that it spans); one that
+// runs out records CHOL_ERR_WAIT_TIMEOUT in the library's status word and ends the launch.
 #include <mutex>
 
 #include "lin_tile.cuh"
@@ -454,14 +454,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     // ---------------- kRaggedK: the last block of a group that ends inside a 16-wide slab --------
     if (MODE == kRaggedK) {
       uint32_t kt = 0, landed_phase = 0, clean_phase = 0;  // bit s: parity of the next wait
+      int64_t span = 0;  // K blocks loaded since the last wait
       bool ok = true;
       for (int t = pair; t < total && ok; t += pairs) {
         walk.at(t, w);
         const int num_k = (w.k_len + kBlockK - 1) / kBlockK;
         kt += uint32_t(num_k);
+        span += num_k;
         if ((w.k_len & 15) == 0) continue;
         const int s = int((kt - 1) % S);
-        ok = wait_bar(&landed[s], landed_phase >> s & 1u, status);
+        ok = wait_bar(&landed[s], landed_phase >> s & 1u, status, limit_of(span));
+        span = 0;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         landed_phase ^= 1u << s;
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       if constexpr (WIDE) {
 #pragma unroll 1
         for (int d = 0; d < 2 && ok; ++d) {
-          ok = wait_bar(&tfull[d], round & 1u, status);
+          ok = wait_bar(&tfull[d], round & 1u, status, limit_of(num_k));
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         if (!ok) break;
       } else {
         const uint32_t buf = round & 1u;
-        ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status);
+        ok = wait_bar(&tfull[buf], (round >> 1) & 1u, status, limit_of(num_k));
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t acc = tmem + buf * uint32_t(BN) + uint32_t(half * kCols) +

@@ -84,13 +84,19 @@ __device__ __forceinline__ void arrive_leader_relaxed(uint32_t addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                : "memory");
 }
+// The limit of a wait that spans `blocks` K blocks: 2 us each, five times what one takes where the loads'
+// latency paces it (356 ns), on top of the usual limit, which 5.6 million blocks alone would reach.
+__device__ __forceinline__ uint64_t limit_of(int64_t blocks) {
+  return kWaitLimitNs + uint64_t(blocks) * 2000;
+}
 // Bounded wait at cluster scope.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* status) {
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* status,
+                                         uint64_t limit = kWaitLimitNs) {
   if (try_wait_cluster(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t it = 0;; ++it) {
     if (try_wait_cluster(bar, parity)) return true;
-    if ((it & 255u) == 255u && global_ns() - t0 > kWaitLimitNs) {
+    if ((it & 255u) == 255u && global_ns() - t0 > limit) {
       atomicExch(status, CHOL_ERR_WAIT_TIMEOUT);
       return false;
     }
