@@ -769,6 +769,11 @@ bool wide(const Product& p) {
   F(false, false, kBatch, kMuon, true)               \
   F(false, true, kBatch, kMuon, true)
 
+// The widest tile of an instance. X^T X, the one batched product of two MN-major operands, is symmetric:
+// wide() leaves it at 256.
+template <bool AMN, bool BMN, int MODE, bool SPLIT>
+constexpr int kWidest = SPLIT ? 128 : (AMN && BMN && MODE == kBatch ? 256 : 512);
+
 int launch_product(const Product& p, cudaStream_t q) {
   if (!resolve_encode()) return CHOL_ERR_DEVICE;
   const int64_t lim = 0x7fffffffLL - 512;
@@ -779,7 +784,7 @@ int launch_product(const Product& p, cudaStream_t q) {
   if (p.a.mn_major == AMN && p.b.mn_major == BMN && p.mode == MODE && p.epilogue == EPI &&  \
       p.split == SPLIT) {                                                                   \
     if (SPLIT || small) return launch<128, AMN, BMN, MODE, EPI, SPLIT>(p, q);               \
-    if (large) return launch<SPLIT ? 128 : 512, AMN, BMN, MODE, EPI, SPLIT>(p, q);          \
+    if (large) return launch<kWidest<AMN, BMN, MODE, SPLIT>, AMN, BMN, MODE, EPI, SPLIT>(p, q); \
     return launch<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>(p, q);                     \
   }
   LIN_FOR_EACH(LIN_CASE)
@@ -793,7 +798,8 @@ cudaError_t prepare_products() {
 #define LIN_SET(AMN, BMN, MODE, EPI, SPLIT)                                                   \
   if ((e = set_smem<128, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;             \
   if ((e = set_smem<SPLIT ? 128 : 256, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e; \
-  if ((e = set_smem<SPLIT ? 128 : 512, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) return e;
+  if ((e = set_smem<kWidest<AMN, BMN, MODE, SPLIT>, AMN, BMN, MODE, EPI, SPLIT>()) != cudaSuccess) \
+    return e;
   LIN_FOR_EACH(LIN_SET)
   LIN_FOR_EACH_SPLIT(LIN_SET)
 #undef LIN_SET
