@@ -687,10 +687,13 @@ int launch(const Product& p, cudaStream_t q) {
   const int sector = p.out_type == LINALG_FP32 ? 8 : 16;
   g.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % sector == 0 &&
               p.out_stride % sector == 0;
-  // the output's boxes, where its type and alignment allow: by group rows when these are ragged
+  // the output's boxes, where its type and alignment allow: by group rows when these are ragged. A store
+  // ends on a 16-byte chunk, not on the map's last column, and would put zeros into up to seven
+  // elements behind it: the caller's rows have to be whole chunks (the workspace's are padded).
   CUtensorMap mo = ma, mm = ma, mc = ma;
   const int64_t planes = SPLIT ? 2 : 1;
-  if (EPI == kPlanes || (!SPLIT && EPI != kMuon && p.out_type != LINALG_FP32)) {
+  if (EPI == kPlanes ||
+      (!SPLIT && EPI != kMuon && p.out_type != LINALG_FP32 && p.n % 8 == 0)) {
     const Operand out{p.out, MODE == kRaggedM ? p.total_rows : p.m, p.n, p.ldo,
                       MODE == kRaggedM ? 1 : p.batch * planes, p.out_stride, false};
     const bool b16 = EPI != kPlanes && p.out_type == LINALG_BF16;
