@@ -55,6 +55,8 @@ def _check_offsets(offsets, like: torch.Tensor, groups: int | None = None) -> in
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` with contiguous rows that start on 16-byte boundaries (as the bulk copies need), a
     copy with padded rows where it has not."""
+    if t.is_neg():  # a lazy negation (imag of a conjugate): the sign is not in memory yet
+        t = t.resolve_neg()
     shape, stride = t.shape, t.stride()
     rows, cols, ld = shape[-2], shape[-1], stride[-2]
     if stride[-1] == 1 and not ld & 7 and ld >= cols and not t.data_ptr() & 15 and (
@@ -213,6 +215,8 @@ def _origin(ctx, i: int, saved: torch.Tensor):
 
 def _check_out(out, shape, like, name, others):
     _check(out, name, len(shape), like)
+    if out.is_neg():
+        raise ValueError(f"{name} must not be a lazy negation")
     if tuple(out.shape) != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(out.shape)}")
     if out.numel() == 0:

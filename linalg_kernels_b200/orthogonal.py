@@ -170,7 +170,8 @@ def _contiguous_call(x, steps, coefficients, eps, precision):
     """The common call (contiguous input, fresh output, one GPU) with arguments that an earlier call
     has checked: the host path paces calls of a few microseconds. None: not that case."""
     if type(x) is not torch.Tensor or not x.is_cuda or not x.is_contiguous() or \
-            x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()) or _dual_level():
+            x.dim() not in (2, 3) or (x.requires_grad and torch.is_grad_enabled()) or \
+            _dual_level() or x.is_neg():
         return None
     kind = _TYPES.get(x.dtype)
     try:  # (5.0 would find the plan of 5, and is refused)
@@ -236,9 +237,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
         _check_tensor(out, "out")
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
             raise ValueError("out must have x's shape, type and device")
+        if out.is_neg():
+            raise ValueError("out must not be a lazy negation")
     if x.numel() == 0:
         return out
-    source, target = x, out
+    source, target = x.resolve_neg(), out  # (a lazy negation's sign is not in memory yet)
     if _is_transposed(target):
         source, target = source.transpose(-2, -1), target.transpose(-2, -1)
     if not _is_rows(target, True):
@@ -322,6 +325,8 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
         _check_tensor(t, name)
         if t.shape != param.shape or t.device != param.device:
             raise ValueError("param, grad and momentum must have one shape and device")
+        if name != "grad" and t.is_neg():
+            raise ValueError(f"{name} must not be a lazy negation")
         if name != "grad" and torch.is_grad_enabled() and t.requires_grad:
             raise RuntimeError(f"{name} requires grad: call muon_update_ under torch.no_grad()")
     _refuse_tangents("muon_update_", param, grad, momentum)
@@ -335,7 +340,7 @@ def muon_update_(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor
         scale = math.sqrt(max(1.0, param.shape[-2] / param.shape[-1]))
     elif not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    p, g, mo = param, grad, momentum
+    p, g, mo = param, grad.resolve_neg(), momentum
     if _is_transposed(p):
         p, g, mo = p.transpose(-2, -1), g.transpose(-2, -1), mo.transpose(-2, -1)
     if not _is_rows(p, True) or not _is_rows(mo, True):

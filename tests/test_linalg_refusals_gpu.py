@@ -201,3 +201,38 @@ def test_muon_precision_argument(precision, dtype):
         exact, tol = _tolerance(grad, dtype, precision == "half")
         off = (param.double() + exact).square().sum((-2, -1)).sqrt()
         assert (off <= (tol + 3 * 2.0 ** -24) * exact.square().sum((-2, -1)).sqrt()).all()
+
+
+def test_lazy_negations():
+    """The imaginary part of a conjugate is a view whose sign is not in memory: inputs are resolved, results
+    refused."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    z = torch.randn(2, 40, 1, dtype=torch.complex64, device=DEV, generator=g)
+    v = z.conj().imag
+    assert v.is_neg()
+    for _ in range(2):
+        assert torch.equal(orthogonalize(v), orthogonalize(-z.imag))
+        t = torch._neg_view(_ones(2, 8, 12))
+        assert torch.equal(orthogonalize(t), -orthogonalize(_ones(2, 8, 12)))
+    p, m = _ones(2, 8, 12), _ones(2, 8, 12)
+    q, n = p.clone(), m.clone()
+    muon_update_(p, torch._neg_view(_ones(2, 8, 12)), m, lr=0.1)
+    muon_update_(q, -_ones(2, 8, 12), n, lr=0.1)
+    assert torch.equal(p, q) and torch.equal(m, n)
+    x, w, dy = _ones(6, 8), _ones(2, 8, 16), _ones(6, 16)
+    offsets = torch.tensor([0, 2, 6], device=DEV)
+    neg = torch._neg_view
+    y = grouped_matmul(x, w, offsets)
+    for a, b in ((neg(x), w), (x, neg(w)), (x, neg(w.mT.contiguous()).mT), (neg(x)[:, ::1], w)):
+        assert torch.equal(grouped_matmul(a, b, offsets), -y)
+    dw = grouped_outer(x, dy, offsets)
+    assert torch.equal(grouped_outer(neg(x), dy, offsets), -dw)
+    xx, ww = x.clone().requires_grad_(), w.clone().requires_grad_()
+    for d in torch.autograd.grad(grouped_matmul(xx, ww, offsets), (xx, ww), neg(dy)):
+        assert (d < 0).all()
+    for call in (lambda: orthogonalize(p, out=neg(q)), lambda: muon_update_(neg(p), q, n, lr=0.1),
+                 lambda: muon_update_(p, q, neg(n), lr=0.1),
+                 lambda: grouped_matmul(x, w, offsets, out=neg(dy)),
+                 lambda: grouped_outer(x, dy, offsets, out=neg(_ones(2, 8, 16)))):
+        with pytest.raises(ValueError, match="negation"):
+            call()
