@@ -8,7 +8,8 @@
 //
 // so a stage is 16 KB of weights and 2 to 8 KB of rows, and each CTA keeps ~180 KB of copies in
 // flight. Both orders of the weights are read as they lie (K-major or MN-major A operand).
-// Bound by HBM: one read of the weights of the groups that have rows.
+// Bound by HBM: one read of the weights of the groups that have rows, at 5.75 TB/s and 5 to 8 us beside
+// it (32, 64, 128 and 256 groups of 1024 x 2048: 31, 52, 98 and 192 us).
 //
 //   warp 0 TMA producer, warp 1 MMA issuer, warp 2 TMEM, warps 4..7 epilogue: TMEM lane = output
 //   column, so a warp stores 32 neighbouring columns of a row at a time.
@@ -288,8 +289,15 @@ cudaError_t set_few() {
 
 }  // namespace
 
-// Measured with 32 groups of 1024 x 2048 (bf16, us, here / 256-row tiles): 48 rows 31.7 / 35.2, 512
-// rows 33.7 / 35.4, 1024 rows 34.9 / 36.0, 2048 rows 48.0 / 36.7.
+// The groups' sizes are on the device, so the rule goes by their mean. Measured in bf16, us, here /
+// 256-row tiles, means of 1, 8, 24 and 32 rows, all groups alike:
+//     8 groups, 2048 x 4096     30 / 40    30 / 32    32 / 33    31 / 33
+//    32 groups, 1024 x 2048     32 / 40    32 / 35    34 / 35    34 / 35   (64 rows: 48 / 37)
+//   128 groups, 2048 x 768      84 / 88    85 / 96    87 / 97    86 / 97
+//   256 groups, 1024 x 1024    106 / 126  106 / 130  109 / 128  109 / 129
+// Where it loses: rows that gather in few groups, whose weights are then read once per row tile (128
+// groups, 2048 x 768, every row in one group: 43 / 21 at a mean of 8, 57 / 23 at 24; in half of the
+// groups 49 / 52 at 8, 85 / 55 at 24).
 bool few_better(const Product& p) {
   return p.mode == kRaggedM && p.total_rows <= 32 * p.batch;
 }

@@ -12,17 +12,20 @@
 // In half precision a stands on B's diagonal, so that the third product reads no old X: one more
 // rounding per row, of the size of X's own. In full precision a X is added in FP32.
 //
-// Number format: X, G and B are fp16, scaled by a power of two, and not bf16: |X|, |G| <= ~1.3
-// and |B| <= ~3, so fp16's range is enough, and its 11 bits make each rounding 8 times smaller
-// than bf16's at the same tensor rate. With bf16 results the error is then the last rounding
-// to bf16 (the iteration's own 5e-4 to 1.3e-3 of the norm against that rounding's 1.7e-3). The
-// scale keeps
-// the small entries of a large matrix (~1 / sqrt(m n) at the start, ~1 / (m sqrt n) in
-// G) out of fp16's subnormals. Full precision (fp16 and fp32 results) keeps two planes,
-// x = hi + lo.
+// Number format: X, G and B are fp16, scaled by a power of two, and not bf16: with the default
+// coefficients no entry of X passes 1.21, of G 1.46, of B 3.45, so fp16's range is enough, and its 11
+// bits make each rounding 8 times smaller than bf16's at the same tensor rate. With bf16 results the
+// error is then the last rounding to bf16 (on random matrices the iteration's own 5e-4 to 1.3e-3 of
+// the norm, 2.6e-3 for 32 x 8192, against that rounding's 1.7e-3). The roundings are noise of full
+// rank, and the iteration multiplies small singular values by up to 3.4 a step: a matrix of low rank
+// (an expert's gradient from few rows) gets noise in the directions that it lacks, 2.4e-2 of the norm
+// at rank 64 of 1024, 7e-2 at rank 4, 0.15 at rank 1 (with bf16 iterates 0.2, 0.5 and 1). Full precision
+// (fp16 and fp32 results) keeps two planes, x = hi + lo: 8e-7 to 3.3e-6 on random matrices, 2e-4 at
+// rank 1, about as FP32 products. The scale keeps the small entries of a large matrix (~1 / sqrt(m n)
+// at the start, ~1 / (m sqrt n) in G) out of fp16's subnormals.
 //
-// The norm is summed in FP64 per block and then over the blocks in a fixed order: the same
-// input gives the same bits, whatever runs beside it.
+// The squares of the norm are summed in FP32 by eights, then in FP64 per block and over the blocks in a
+// fixed order: the same input gives the same bits, whatever runs beside it.
 #include <math.h>
 
 #include <mutex>

@@ -24,9 +24,10 @@
 // Bound by latency: per step three dependent chains MMA -> TMEM read -> convert -> shared memory,
 // ~5500 cycles for a 128 x 128 tile (2000 of them MMAs), beside ~9000 for reading and the norm and
 // ~5000 for writing. One 128 x 128 matrix takes 25 us (the products of lin_gemm.cu, 17 launches,
-// took 86), 1024 of 64 x 64 take 43 us, 0.39 TB/s (423 us), an optimiser step on 512 x 128
-// in full precision over 4 CTAs 78 us (203 us). The diagonals in FP32 cost 3.5 us of the 25 and
-// 8 us of the 43.
+// took 86), an optimiser step on 512 x 128 in full precision over 4 CTAs 78 us (203 us). 1024 of
+// 64 x 64 take 43 us, 0.39 TB/s (423 us): their 512 tiles are resident at once, four CTAs an SM, and
+// share its issue slots for the conversions; the 64 registers that this leaves spill 156 bytes a
+// thread (192 in the step). The diagonals in FP32 cost 3.5 us of the 25 and 8 us of the 43.
 #include "lin_chip.cuh"
 #include "lin_small.cuh"
 
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(T, T == 256 ? (MUON ? 3 : 4) : 1)
     wait();
     // Half precision: G and B in shared memory are without their diagonals D, whose rounding would
     // be the largest error by far (small matrices have few entries to average it, and X X^T of
-    // a wide one is nearly a multiple of I: 32 x 4096 was 4.4e-3 off, now ~1e-3). With G = D + O,
+    // a wide one is nearly a multiple of I: 32 x 4096 was 4.4e-3 off in bf16, now 1.7e-3). With G = D + O,
     //   (G G)_ij = (O O)_ij + (d_i + d_j) O_ij  off the diagonal,  (O O)_ii + d_i^2  on it,
     // and the diagonal of a I + b G + c G G scales the rows of X in FP32 at the end.
     // Full: a X is added in FP32 at the end, not summed by the tensor core, whose rounding towards

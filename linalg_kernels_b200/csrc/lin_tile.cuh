@@ -538,7 +538,8 @@ struct WarpEpilogue {
   }
 
   // SPLIT: add_c's result as two planes, 64 columns from gc0. Nothing but the sums stays in registers
-  // (with packed copies they went to local memory, 2200 cycles for each drain).
+  // (with packed copies they went to local memory, 2200 cycles for each drain); only the instances
+  // that write the caller's matrix spill, 72 bytes, and 32 in the optimiser step.
   __device__ __forceinline__ void planes(const Out& g, int row_base, int gc0, bool mirror,
                                          const float (&sum)[2][32]) {
     if (gc0 >= g.n || row_base >= g.rows) return;

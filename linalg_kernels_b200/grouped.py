@@ -252,7 +252,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     non-decreasing within ``[0, rows]`` (values that are not are clamped: no row outside x is
     touched); groups may be empty. Rows of no group (padding in front of offsets[0] or behind
     offsets[-1]) are zero in the result; with ``out`` given they stay as they were. At most
-    1024 groups.
+    1024 groups. ``out`` needs k > 0 and contiguous rows, at any distance; nothing between them is
+    written.
 
     Differentiable in x and w (without ``out``): the gradient of a group without rows, and of rows
     of no group, is zero; dy's rows of no group are not read. Forward-mode tangents and second
