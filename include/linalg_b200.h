@@ -26,9 +26,11 @@ extern "C" {
 #define LINALG_PRECISION_AUTO 0 /* HALF for bf16 results, FULL for fp16 and fp32 results */
 #define LINALG_PRECISION_HALF 1 /* fp16 operands, FP32 accumulation: 0.5e-3 to 2.6e-3 of the result's
                                    norm on random matrices, more on those of low rank (2.4e-2 at rank
-                                   64 of 1024, 0.15 at rank 1) */
+                                   64 of 1024, 0.15 at rank 1). With a side above 2^18 the work is
+                                   FULL's all the same: sums that long fall short in HALF */
 #define LINALG_PRECISION_FULL 2 /* operands split into two fp16 numbers (22 bits), three products
-                                   per product: 1e-6 to 3.3e-6 of the result's norm, 2e-4 at rank 1 */
+                                   per product: 1e-6 to 3.3e-6 of the result's norm, 2e-4 at rank 1,
+                                   8e-5 with a side of 2^24 */
 
 #define LINALG_MAX_STEPS 32   /* Newton-Schulz steps of one call */
 #define LINALG_MAX_GROUPS 1024 /* groups of one grouped product */

@@ -403,9 +403,18 @@ bool too_large(int64_t batch, int64_t m, int64_t n) {
   return batch > lim || m > lim || n > lim;
 }
 
-bool wants_split(int precision, int type) {
-  if (precision == LINALG_PRECISION_AUTO) return type != LINALG_BF16;
-  return precision == LINALG_PRECISION_FULL;
+// Half precision sums all of G's K on the tensor core, which rounds towards zero after every 16 terms:
+// the diagonal falls short by up to (K / 16) 2^-23 of itself. Up to 2^18 columns that hides behind the
+// roundings to fp16; beyond (16 x 2^20 was 8e-3 off, 16 x 2^22 3e-2, 4 x 2^24 0.33) full
+// precision, which drains every 64, takes over at three times the products (2^20: 4e-6).
+constexpr int64_t kLongestHalf = int64_t(1) << 18;
+bool works_split(bool full, int64_t m, int64_t n) {
+  return full || m > kLongestHalf || n > kLongestHalf;
+}
+bool wants_split(int precision, int type, int64_t m, int64_t n) {
+  const bool full = precision == LINALG_PRECISION_AUTO ? type != LINALG_BF16
+                                                       : precision == LINALG_PRECISION_FULL;
+  return works_split(full, m, n);
 }
 
 int check_workspace(int64_t batch, int64_t m, int64_t n, bool split, const void* ws, size_t bytes) {
@@ -470,7 +479,7 @@ int linalg_prepare(int device) { return prepare_device(device); }
 
 size_t linalg_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int precision) {
   if (batch <= 0 || m <= 0 || n <= 0 || too_large(batch, m, n)) return 0;
-  return layout(batch, m, n, precision != LINALG_PRECISION_HALF).total;
+  return layout(batch, m, n, works_split(precision != LINALG_PRECISION_HALF, m, n)).total;
 }
 
 int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64_t batch,
@@ -485,7 +494,7 @@ int linalg_orthogonalize(const linalg_matrix* x, const linalg_matrix* out, int64
   const bool same = x->data == out->data && x->ld == out->ld && x->type == out->type &&
                     (batch == 1 || x->stride == out->stride);
   if (!same && overlap(x, out, batch, m, n)) return CHOL_ERR_INVALID_ARG;
-  const bool split = wants_split(precision, out->type);
+  const bool split = wants_split(precision, out->type, m, n);
   if (!in_range(steps, coefficients, split)) return CHOL_ERR_UNSUPPORTED;
   if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
   if ((st = prepare_current()) != CHOL_OK) return st;
@@ -510,7 +519,7 @@ int linalg_muon_update(const linalg_matrix* param, const linalg_matrix* grad,
   if (overlap(param, grad, batch, m, n) || overlap(param, momentum, batch, m, n) ||
       overlap(grad, momentum, batch, m, n))
     return CHOL_ERR_INVALID_ARG;
-  const bool split = wants_split(precision, param->type);
+  const bool split = wants_split(precision, param->type, m, n);
   if (!in_range(steps, coefficients, split)) return CHOL_ERR_UNSUPPORTED;
   if ((st = check_workspace(batch, m, n, split, workspace, workspace_bytes)) != CHOL_OK) return st;
   if ((st = prepare_current()) != CHOL_OK) return st;

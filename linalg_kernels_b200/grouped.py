@@ -246,14 +246,15 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     """``y[r] = x[r] @ w[e]`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of each group.
 
     x: ``(rows, k)``, w: ``(groups, k, n)``, bfloat16 or float16 CUDA tensors of one type; sums in
-    FP32, rounded once. w may be the transposed view of ``(groups, n, k)`` weights, read as it
-    lies. Rows that do not start on 16-byte boundaries (k or n not a multiple of 8) and other
-    layouts are copied first. offsets: ``(groups + 1,)`` int32 or int64 on the device,
-    non-decreasing within ``[0, rows]`` (values that are not are clamped: no row outside x is
-    touched); groups may be empty. Rows of no group (padding in front of offsets[0] or behind
-    offsets[-1]) are zero in the result; with ``out`` given they stay as they were. At most
-    1024 groups. ``out`` needs k > 0 and contiguous rows, at any distance; nothing between them is
-    written.
+    FP32, rounded once (the tensor core rounds its sums towards zero every 16 terms: at most
+    ``(terms / 16 + 2) * 2**-22`` of the sum of the terms' magnitudes, ~1e-3 for 2^16 terms of one
+    sign). w may be the transposed view of ``(groups, n, k)`` weights, read as it lies. Rows that do
+    not start on 16-byte boundaries (k or n not a multiple of 8) and other layouts are copied first.
+    offsets: ``(groups + 1,)`` int32 or int64 on the device, non-decreasing within ``[0, rows]``
+    (values that are not are clamped: no row outside x is touched); groups may be empty. Rows of no
+    group (padding in front of offsets[0] or behind offsets[-1]) are zero in the result; with
+    ``out`` given they stay as they were. At most 1024 groups. ``out`` needs k > 0 and contiguous
+    rows, at any distance; nothing between them is written.
 
     Differentiable in x and w (without ``out``): the gradient of a group without rows, and of rows
     of no group, is zero; dy's rows of no group are not read. Forward-mode tangents and second

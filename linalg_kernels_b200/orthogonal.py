@@ -210,7 +210,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, *,
     with the small singular values: 2.4e-2 at rank 64 of 1024, 7e-2 at rank 4, 0.15 at rank 1 (the
     first step on an expert's gradient from few rows, for example); ``"full"`` keeps those right.
     It works in split fp16, about as FP32 products would (1e-6 to 3.3e-6, 2e-4 at rank 1), at three
-    times the products. None takes ``"half"`` for bfloat16 and ``"full"`` otherwise. out: written and
+    times the products; so do matrices with a side above 2^18, whichever is given. None takes ``"half"`` for bfloat16 and ``"full"`` otherwise. out: written and
     returned instead of a new tensor; may be ``x`` itself.
 
     The iterates are fp16 numbers: coefficients with which some matrix could leave their range (singular
