@@ -1,4 +1,4 @@
-"""GPU: the training step of INTEGRATION.md, run as it stands there: a layer whose weights are stored
+"""GPU: the training step of the integration notes, run as it stands there: a layer whose weights are stored
 (groups, in, out) gets the update of the same layer stored (groups, out, in).
 
 Tolerance: test_expert_step_gpu.py's, from each side's own gradient.
