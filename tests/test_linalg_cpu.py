@@ -193,19 +193,3 @@ def test_layout_rules():
     assert a(x.T).stride(-1) == 1
     w = torch.zeros(3, 8, 16, dtype=torch.bfloat16)
     assert a(w) is w and a(w[:1].expand(3, 8, 16)).stride() == (128, 16, 1)
-
-
-def test_tangents_are_refused():
-    from torch.autograd import forward_ad
-
-    x = torch.ones(3, 4)
-    orthogonal._refuse_tangents("here", x, None)
-    with forward_ad.dual_level():
-        dual = forward_ad.make_dual(x, torch.ones(3, 4))
-        orthogonal._refuse_tangents("here", x, None, dual.detach())
-        for t in (dual, dual.mT, dual * 2):
-            with pytest.raises(RuntimeError, match="here"):
-                orthogonal._refuse_tangents("here", x, t)
-            with torch.no_grad(), pytest.raises(RuntimeError):  # tangents pass no_grad
-                orthogonal._refuse_tangents("here", t)
-    orthogonal._refuse_tangents("here", dual)
